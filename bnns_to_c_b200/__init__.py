@@ -60,6 +60,7 @@ def lib():
                           "(or __graft_entry__.build())")
     L = ctypes.CDLL(LIB_PATH)
     vp, ip, cp = ctypes.c_void_p, ctypes.c_int, ctypes.c_char_p
+    i64 = ctypes.c_int64
     sig = {
         "bnn_last_error": (cp, []),
         "bnn_load_ex": (ip, [cp, ctypes.POINTER(vp)]),
@@ -125,6 +126,17 @@ def lib():
         "bnn_bconv_last_kernel": (cp, []),
         "bnn_set_arena_poison": (ip, [ip]),
         "bnn_arena_poison": (ip, []),
+        "bnn_q4_layer_create": (ip, [ip] * 5 + [vp] * 4 + [ctypes.POINTER(vp)]),
+        "bnn_q4_layer_run": (ip, [vp, vp, i64, ip, vp, i64, vp]),
+        "bnn_q4_layer_destroy": (None, [vp]),
+        "bnn_kv_cache_create": (ip, [ip] * 8 + [ctypes.POINTER(vp)]),
+        "bnn_kv_cache_destroy": (None, [vp]),
+        "bnn_kv_cache_bytes": (ctypes.c_size_t, [vp]),
+        "bnn_kv_cache_write": (ip, [vp, vp, i64, i64, vp, i64, i64, ip, ip, vp, ip, vp, vp, vp]),
+        "bnn_kv_cache_read": (ip, [vp, vp, i64, i64, vp, i64, i64, ip, ip, vp, ip, vp, vp, vp]),
+        "bnn_kv_attend_work": (ctypes.c_size_t, [vp, ip, ip, ip]),
+        "bnn_kv_attend": (ip, [vp, vp, i64, i64, ip, ip, vp, vp, ip, vp, ip, ip, ctypes.c_float, vp, i64, i64,
+                               vp, vp, ctypes.c_size_t, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -475,6 +487,201 @@ class BconvLayer:
     def close(self):
         if getattr(self, "handle", None):
             lib().bnn_bconv_layer_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ---------------- low-bit operators (include/bnn_lowbit.h) ----------------
+_TYPES = {"bf16": 0, "fp16": 1}
+_TORCH_NAMES = ("torch.bfloat16", "torch.float16")
+
+
+def _stream(s):
+    return s if s is None or isinstance(s, int) else s.cuda_stream
+
+
+def _arg(ok, msg):
+    if not ok:
+        raise BnnError(BNN_ERR_ARG, msg)
+
+
+class _LowBit:
+    """What the low-bit handles share: the checks of the tensors they are given."""
+
+    def _tensor(self, t, name, kind, dims):
+        """A CUDA tensor of this handle's device; a flat one where `dims` is
+        None. Raises BnnError (BNN_ERR_ARG) on another."""
+        _arg(hasattr(t, "data_ptr"), f"{name}: a CUDA tensor is needed")
+        _arg(str(t.dtype) == kind, f"{name}: {t.dtype}, {kind} is needed")
+        _arg(t.is_cuda and t.get_device() == self.device if self.device >= 0 else True,
+             f"{name} is not on device {self.device}")
+        if dims is None:
+            _arg(t.is_contiguous(), f"{name}: not contiguous")
+        else:
+            _arg(t.dim() == len(dims), f"{name}: {tuple(t.shape)}, {len(dims)} dimensions are needed")
+            for have, want in zip(t.shape, dims):
+                _arg(want is None or have == want, f"{name}: shape {tuple(t.shape)}, {dims} is needed")
+        return t
+
+
+class Q4Linear(_LowBit):
+    """A 4-bit linear layer on device memory (``bnn_q4_layer_*``):
+    y = x @ ((q - z) * s).T + bias.
+
+    codes: uint8 [n_out, ceil(n_in / 2)], the even input in the low half of a
+    byte; scales: [n_out, ceil(n_in / group)] in the layer's type; zeros:
+    uint8 of that shape, or None for 8 everywhere; bias: float32 [n_out] or
+    None. Each a numpy array or a torch tensor, contiguous, on the host or
+    on `device`; scales of a numpy layer are given as 16-bit words for
+    bf16. They are not needed afterwards. device = -1: no device memory,
+    for checks on a machine without a GPU."""
+
+    def __init__(self, device, n_in, n_out, codes, scales, zeros=None, bias=None, group=128, dtype="bf16"):
+        _arg(dtype in _TYPES, f"dtype {dtype!r}: 'bf16' or 'fp16'")
+        _arg(n_in > 0 and n_out > 0 and group > 0, f"{n_in} inputs, {n_out} outputs, group {group}")
+        self.handle = None
+        ng = -(-n_in // group)
+        for a, name, shape, size in ((codes, "codes", (n_out, (n_in + 1) // 2), 1), (scales, "scales", (n_out, ng), 2),
+                                     (zeros, "zeros", (n_out, ng), 1), (bias, "bias", (n_out,), 4)):
+            if a is None and name in ("zeros", "bias"):
+                continue
+            torch_like = hasattr(a, "data_ptr")
+            _arg(torch_like or isinstance(a, np.ndarray), f"{name}: a numpy array or a tensor is needed")
+            _arg(tuple(a.shape) == shape, f"{name}: shape {tuple(a.shape)}, {shape} is needed")
+            _arg((a.element_size() if torch_like else a.itemsize) == size, f"{name}: {a.dtype} has another size")
+            if torch_like and name == "scales":
+                _arg(str(a.dtype) == _TORCH_NAMES[_TYPES[dtype]], f"scales: {a.dtype} in a layer of {dtype}")
+            _arg(a.is_contiguous() if torch_like else a.flags.c_contiguous, f"{name}: not contiguous")
+        h = ctypes.c_void_p()
+        _check(lib().bnn_q4_layer_create(device, n_in, n_out, group, _TYPES[dtype], _ptr(codes), _ptr(scales),
+                                         _ptr(zeros), _ptr(bias), ctypes.byref(h)))
+        self.handle, self.device = h.value, device
+        self.n_in, self.n_out, self.group, self.dtype = n_in, n_out, group, dtype
+        self._kind = _TORCH_NAMES[_TYPES[dtype]]
+
+    def run(self, d_x, d_y, stream=None):
+        """x [rows, n_in] -> y [rows, n_out], torch CUDA tensors of the
+        layer's type whose rows are contiguous, at any distance."""
+        self._tensor(d_x, "x", self._kind, (None, self.n_in))
+        rows = d_x.shape[0]
+        self._tensor(d_y, "y", self._kind, (rows, self.n_out))
+        xs, ys = d_x.stride(), d_y.stride()
+        _arg((xs[1] == 1 or self.n_in == 1) and (ys[1] == 1 or self.n_out == 1), "x, y: rows are not contiguous")
+        _check(_lib.bnn_q4_layer_run(self.handle, d_x.data_ptr(), xs[0], rows, d_y.data_ptr(), ys[0], _stream(stream)))
+
+    def close(self):
+        if getattr(self, "handle", None):
+            lib().bnn_q4_layer_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KVCache(_LowBit):
+    """A block-scaled key/value cache on device memory (``bnn_kv_cache_*``)
+    of `pages` pages, and the attention that reads it (``bnn_kv_attend``).
+    The tensors are torch CUDA tensors of the cache's device; keys, values,
+    queries and outputs have its type and contiguous heads, at any strides;
+    tables, starts, offsets and lengths are contiguous int32 tensors.
+    device = -1: no device memory, for checks on a machine without a GPU."""
+
+    def __init__(self, device, pages, page_tokens, kv_heads, head_dim, bits=8, group=0, dtype="bf16"):
+        _arg(dtype in _TYPES, f"dtype {dtype!r}: 'bf16' or 'fp16'")
+        self.handle = None
+        h = ctypes.c_void_p()
+        _check(lib().bnn_kv_cache_create(device, pages, page_tokens, kv_heads, head_dim, bits, group, _TYPES[dtype],
+                                         ctypes.byref(h)))
+        self.handle, self.device = h.value, device
+        self.pages, self.page_tokens, self.kv_heads, self.head_dim = pages, page_tokens, kv_heads, head_dim
+        self.bits, self.group, self.dtype = bits, group or head_dim, dtype
+        self._kind = _TORCH_NAMES[_TYPES[dtype]]
+
+    @property
+    def nbytes(self):
+        return lib().bnn_kv_cache_bytes(self.handle)
+
+    def _heads(self, t, name, rows, heads):
+        """Data pointer and strides of [rows, heads, head_dim]."""
+        self._tensor(t, name, self._kind, (rows, heads, self.head_dim))
+        s = t.stride()
+        _arg(s[2] == 1, f"{name}: heads are not contiguous")
+        return t.data_ptr(), s[0], s[1]
+
+    def _table(self, table, seqs):
+        self._tensor(table, "table", "torch.int32", (seqs, None))
+        _arg(table.is_contiguous(), "table: not contiguous")
+        return table.data_ptr(), table.shape[1]
+
+    def _rows(self, fn, k, v, table, start, offsets, stream):
+        seqs = self._tensor(start, "start", "torch.int32", (None,)).shape[0]
+        _arg(start.is_contiguous(), "start: not contiguous")
+        tokens = k.shape[0]
+        if offsets is not None:
+            self._tensor(offsets, "offsets", "torch.int32", (seqs + 1,))
+            _arg(offsets.is_contiguous(), "offsets: not contiguous")
+        _check(fn(self.handle, *self._heads(k, "k", tokens, self.kv_heads), *self._heads(v, "v", tokens, self.kv_heads),
+                  tokens, seqs, *self._table(table, seqs), start.data_ptr(),
+                  None if offsets is None else offsets.data_ptr(), _stream(stream)))
+
+    def write(self, d_k, d_v, table, start, offsets=None, stream=None):
+        """Store keys and values [tokens, kv_heads, head_dim]: row t belongs
+        to the sequence b with offsets[b] <= t < offsets[b + 1] and stands at
+        position start[b] + t - offsets[b]; without offsets row t is one
+        token of sequence t. table [sequences, pages of each]."""
+        self._rows(_lib.bnn_kv_cache_write, d_k, d_v, table, start, offsets, stream)
+
+    def read(self, d_k, d_v, table, start, offsets=None, stream=None):
+        """The values that such tokens have in the cache, into d_k and d_v;
+        rows without a place are left as they were."""
+        self._rows(_lib.bnn_kv_cache_read, d_k, d_v, table, start, offsets, stream)
+
+    def attend_work(self, n_seqs, q_heads, prefix_tokens=0):
+        """Bytes of workspace that such an `attend` needs."""
+        n = lib().bnn_kv_attend_work(self.handle, n_seqs, q_heads, prefix_tokens)
+        _arg(n > 0 or n_seqs == 0, lib().bnn_last_error().decode())
+        return n
+
+    def attend(self, d_q, lengths, table, d_out, work, lse=None, scale=None, prefix=None, prefix_tokens=0, stream=None):
+        """Single-token attention: q and out [sequences, q_heads, head_dim],
+        lengths [sequences], table [sequences, pages of each]; prefix: int32
+        pages of the prefix_tokens tokens that all sequences share; work: a
+        contiguous CUDA tensor of attend_work(...) bytes, for this call alone
+        until it has run; lse: float32 [sequences, q_heads] or None; scale:
+        head_dim ** -0.5 unless given."""
+        _arg(hasattr(d_q, "data_ptr") and d_q.dim() == 3, "q: a tensor [sequences, q_heads, head_dim] is needed")
+        seqs, heads = d_q.shape[0], d_q.shape[1]
+        self._tensor(lengths, "lengths", "torch.int32", (seqs,))
+        _arg(lengths.is_contiguous(), "lengths: not contiguous")
+        q, q_seq, q_head = self._heads(d_q, "q", seqs, heads)
+        out, o_seq, o_head = self._heads(d_out, "out", seqs, heads)
+        if lse is not None:
+            self._tensor(lse, "lse", "torch.float32", (seqs, heads))
+            _arg(lse.is_contiguous(), "lse: not contiguous")
+        pages = 0
+        if prefix is not None:
+            self._tensor(prefix, "prefix", "torch.int32", (None,))
+            _arg(prefix.is_contiguous(), "prefix: not contiguous")
+            pages = prefix.shape[0]
+        self._tensor(work, "work", str(work.dtype), None)
+        _check(_lib.bnn_kv_attend(
+            self.handle, q, q_seq, q_head, seqs, heads, lengths.data_ptr(), *self._table(table, seqs),
+            prefix.data_ptr() if pages else None, pages, prefix_tokens,
+            self.head_dim ** -0.5 if scale is None else scale, out, o_seq, o_head,
+            None if lse is None else lse.data_ptr(), work.data_ptr(), work.numel() * work.element_size(),
+            _stream(stream)))
+
+    def close(self):
+        if getattr(self, "handle", None):
+            lib().bnn_kv_cache_destroy(self.handle)
             self.handle = None
 
     def __del__(self):

@@ -41,4 +41,8 @@ int validate_topology(const Model* m, Topology* t, int stem_c = 0);
 // bnn_set_arena_poison set it.
 int arena_poison_byte();
 
+// A device allocation on the current device, counted by the fault injection
+// of bnn_debug_inject_fault like the engine's own; BNN_OK or BNN_ERR_OOM.
+int device_alloc(void** p, size_t bytes, const char* what);
+
 }  // namespace bnn

@@ -121,6 +121,13 @@ static cudaError_t dev_malloc(T** p, size_t bytes) {
     return cudaMalloc((void**)p, bytes);
 }
 
+int device_alloc(void** p, size_t bytes, const char* what) {
+    if (dev_malloc(p, bytes) == cudaSuccess) return BNN_OK;
+    cudaGetLastError();
+    *p = nullptr;
+    return set_error(BNN_ERR_OOM, "cudaMalloc %s: %zu bytes", what, bytes);
+}
+
 // name of the last binary-conv kernel this thread launched (with its
 // template parameters), for benchmarks and tests that must know which
 // implementation ran
