@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 
 import numpy as np
 
@@ -129,6 +130,7 @@ def lib():
         "bnn_q4_layer_create": (ip, [ip] * 5 + [vp] * 4 + [ctypes.POINTER(vp)]),
         "bnn_q4_layer_run": (ip, [vp, vp, i64, ip, vp, i64, vp]),
         "bnn_q4_layer_destroy": (None, [vp]),
+        "bnn_q4_device_error": (ip, [ip, ctypes.POINTER(ctypes.c_uint)]),
         "bnn_kv_cache_create": (ip, [ip] * 8 + [ctypes.POINTER(vp)]),
         "bnn_kv_cache_destroy": (None, [vp]),
         "bnn_kv_cache_bytes": (ctypes.c_size_t, [vp]),
@@ -498,7 +500,7 @@ class BconvLayer:
 
 # ---------------- low-bit operators (include/bnn_lowbit.h) ----------------
 _TYPES = {"bf16": 0, "fp16": 1}
-_TORCH_NAMES = ("torch.bfloat16", "torch.float16")
+_KINDS = {"bf16": "bfloat16", "fp16": "float16"}
 
 
 def _stream(s):
@@ -510,23 +512,39 @@ def _arg(ok, msg):
         raise BnnError(BNN_ERR_ARG, msg)
 
 
-class _LowBit:
-    """What the low-bit handles share: the checks of the tensors they are given."""
+def _torch_type(name):
+    """The torch dtype of that name; torch is loaded where a tensor is given."""
+    torch = sys.modules.get("torch")
+    return getattr(torch, name) if torch is not None else name
 
-    def _tensor(self, t, name, kind, dims):
-        """A CUDA tensor of this handle's device; a flat one where `dims` is
-        None. Raises BnnError (BNN_ERR_ARG) on another."""
-        _arg(hasattr(t, "data_ptr"), f"{name}: a CUDA tensor is needed")
-        _arg(str(t.dtype) == kind, f"{name}: {t.dtype}, {kind} is needed")
-        _arg(t.is_cuda and t.get_device() == self.device if self.device >= 0 else True,
-             f"{name} is not on device {self.device}")
-        if dims is None:
-            _arg(t.is_contiguous(), f"{name}: not contiguous")
-        else:
-            _arg(t.dim() == len(dims), f"{name}: {tuple(t.shape)}, {len(dims)} dimensions are needed")
-            for have, want in zip(t.shape, dims):
-                _arg(want is None or have == want, f"{name}: shape {tuple(t.shape)}, {dims} is needed")
-        return t
+
+class _LowBit:
+    """What the low-bit handles share: the checks of the tensors they are
+    given. A call tests all of them in one expression, since its cost is
+    what a decode step of small launches waits for; only where that is
+    false is the fault looked for, by `_explain`."""
+
+    def _types(self):
+        """The dtypes to compare with; true where they were not known yet
+        (a handle made before torch was loaded)."""
+        before = getattr(self, "_kind", None)
+        self._kind, self._int, self._float = (_torch_type(n) for n in (_KINDS[self.dtype], "int32", "float32"))
+        return before is not self._kind
+
+    def _explain(self, *tensors):
+        """Raises BnnError (BNN_ERR_ARG) for the first of (tensor, name,
+        type, shape, contiguous) that is not as it has to be. shape: None =
+        any, an entry of None = any extent; contiguous: whether the whole
+        tensor has to be, or its last axis."""
+        for t, name, kind, dims, whole in tensors:
+            _arg(hasattr(t, "data_ptr"), f"{name}: a tensor is needed")
+            _arg(kind is None or t.dtype is kind, f"{name}: {t.dtype}, {kind} is needed")
+            _arg(t.get_device() == self.device, f"{name}: on device {t.get_device()}, {self.device} is needed")
+            if dims is not None:
+                _arg(t.dim() == len(dims), f"{name}: {tuple(t.shape)}, {len(dims)} dimensions are needed")
+                _arg(all(want is None or have == want for have, want in zip(t.shape, dims)),
+                     f"{name}: shape {tuple(t.shape)}, {dims} is needed")
+            _arg(t.is_contiguous() if whole else t.stride(-1) == 1 or t.shape[-1] == 1, f"{name}: not contiguous")
 
 
 class Q4Linear(_LowBit):
@@ -555,24 +573,35 @@ class Q4Linear(_LowBit):
             _arg(tuple(a.shape) == shape, f"{name}: shape {tuple(a.shape)}, {shape} is needed")
             _arg((a.element_size() if torch_like else a.itemsize) == size, f"{name}: {a.dtype} has another size")
             if torch_like and name == "scales":
-                _arg(str(a.dtype) == _TORCH_NAMES[_TYPES[dtype]], f"scales: {a.dtype} in a layer of {dtype}")
+                _arg(a.dtype is _torch_type(_KINDS[dtype]), f"scales: {a.dtype} in a layer of {dtype}")
             _arg(a.is_contiguous() if torch_like else a.flags.c_contiguous, f"{name}: not contiguous")
         h = ctypes.c_void_p()
         _check(lib().bnn_q4_layer_create(device, n_in, n_out, group, _TYPES[dtype], _ptr(codes), _ptr(scales),
                                          _ptr(zeros), _ptr(bias), ctypes.byref(h)))
         self.handle, self.device = h.value, device
         self.n_in, self.n_out, self.group, self.dtype = n_in, n_out, group, dtype
-        self._kind = _TORCH_NAMES[_TYPES[dtype]]
+        self._run = _lib.bnn_q4_layer_run
+        self._types()
 
     def run(self, d_x, d_y, stream=None):
         """x [rows, n_in] -> y [rows, n_out], torch CUDA tensors of the
         layer's type whose rows are contiguous, at any distance."""
-        self._tensor(d_x, "x", self._kind, (None, self.n_in))
-        rows = d_x.shape[0]
-        self._tensor(d_y, "y", self._kind, (rows, self.n_out))
-        xs, ys = d_x.stride(), d_y.stride()
-        _arg((xs[1] == 1 or self.n_in == 1) and (ys[1] == 1 or self.n_out == 1), "x, y: rows are not contiguous")
-        _check(_lib.bnn_q4_layer_run(self.handle, d_x.data_ptr(), xs[0], rows, d_y.data_ptr(), ys[0], _stream(stream)))
+        try:
+            (rows, k), (y_rows, n), kind, dev = d_x.shape, d_y.shape, self._kind, self.device
+            (xs, x1), (ys, y1) = d_x.stride(), d_y.stride()
+            ok = (k == self.n_in and n == self.n_out and rows == y_rows and d_x.dtype is kind and d_y.dtype is kind
+                  and d_x.get_device() == dev and d_y.get_device() == dev and (x1 == 1 or k == 1) and (y1 == 1 or n == 1))
+        except (AttributeError, ValueError, TypeError):
+            ok = False
+        if not ok:
+            new = self._types()
+            self._explain((d_x, "x", self._kind, (None, self.n_in), False))
+            self._explain((d_y, "y", self._kind, (d_x.shape[0], self.n_out), False))
+            _arg(new, "arguments that do not go together")
+            return self.run(d_x, d_y, stream)
+        rc = self._run(self.handle, d_x.data_ptr(), xs, rows, d_y.data_ptr(), ys, _stream(stream))
+        if rc:
+            _check(rc)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -584,6 +613,13 @@ class Q4Linear(_LowBit):
             self.close()
         except Exception:
             pass
+
+
+def q4_wait_timeouts(device=0):
+    """Bounded waits of the 4-bit layers' tcgen05 kernel that gave up on `device`."""
+    n = ctypes.c_uint()
+    _check(lib().bnn_q4_device_error(device, ctypes.byref(n)))
+    return n.value
 
 
 class KVCache(_LowBit):
@@ -603,46 +639,54 @@ class KVCache(_LowBit):
         self.handle, self.device = h.value, device
         self.pages, self.page_tokens, self.kv_heads, self.head_dim = pages, page_tokens, kv_heads, head_dim
         self.bits, self.group, self.dtype = bits, group or head_dim, dtype
-        self._kind = _TORCH_NAMES[_TYPES[dtype]]
+        self._write, self._read, self._attend = _lib.bnn_kv_cache_write, _lib.bnn_kv_cache_read, _lib.bnn_kv_attend
+        self._types()
 
     @property
     def nbytes(self):
         return lib().bnn_kv_cache_bytes(self.handle)
 
-    def _heads(self, t, name, rows, heads):
-        """Data pointer and strides of [rows, heads, head_dim]."""
-        self._tensor(t, name, self._kind, (rows, heads, self.head_dim))
-        s = t.stride()
-        _arg(s[2] == 1, f"{name}: heads are not contiguous")
-        return t.data_ptr(), s[0], s[1]
-
-    def _table(self, table, seqs):
-        self._tensor(table, "table", "torch.int32", (seqs, None))
-        _arg(table.is_contiguous(), "table: not contiguous")
-        return table.data_ptr(), table.shape[1]
-
     def _rows(self, fn, k, v, table, start, offsets, stream):
-        seqs = self._tensor(start, "start", "torch.int32", (None,)).shape[0]
-        _arg(start.is_contiguous(), "start: not contiguous")
-        tokens = k.shape[0]
-        if offsets is not None:
-            self._tensor(offsets, "offsets", "torch.int32", (seqs + 1,))
-            _arg(offsets.is_contiguous(), "offsets: not contiguous")
-        _check(fn(self.handle, *self._heads(k, "k", tokens, self.kv_heads), *self._heads(v, "v", tokens, self.kv_heads),
-                  tokens, seqs, *self._table(table, seqs), start.data_ptr(),
-                  None if offsets is None else offsets.data_ptr(), _stream(stream)))
+        try:
+            (tokens, heads, dim), (seqs, width), kind, whole, dev = k.shape, table.shape, self._kind, self._int, self.device
+            (kt, kh, k1), (vt, vh, v1) = k.stride(), v.stride()
+            ok = (heads == self.kv_heads and dim == self.head_dim and v.shape == k.shape and k1 == 1 and v1 == 1
+                  and k.dtype is kind and v.dtype is kind and k.get_device() == dev and v.get_device() == dev
+                  and start.shape == (seqs,) and table.dtype is whole and start.dtype is whole and table.is_contiguous()
+                  and start.is_contiguous() and table.get_device() == dev and start.get_device() == dev)
+            off = None
+            if offsets is not None:
+                off = offsets.data_ptr()
+                ok = (ok and offsets.shape == (seqs + 1,) and offsets.dtype is whole and offsets.is_contiguous()
+                      and offsets.get_device() == dev)
+        except (AttributeError, ValueError, TypeError):
+            ok = False
+        if not ok:
+            new = self._types()
+            rows = (None, self.kv_heads, self.head_dim)
+            self._explain((k, "k", self._kind, rows, False))
+            self._explain((v, "v", self._kind, tuple(k.shape), False), (start, "start", self._int, (None,), True))
+            self._explain((table, "table", self._int, (start.shape[0], None), True))
+            if offsets is not None:
+                self._explain((offsets, "offsets", self._int, (start.shape[0] + 1,), True))
+            _arg(new, "arguments that do not go together")
+            return self._rows(fn, k, v, table, start, offsets, stream)
+        rc = fn(self.handle, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, tokens, seqs, table.data_ptr(), width, start.data_ptr(),
+                off, _stream(stream))
+        if rc:
+            _check(rc)
 
     def write(self, d_k, d_v, table, start, offsets=None, stream=None):
         """Store keys and values [tokens, kv_heads, head_dim]: row t belongs
         to the sequence b with offsets[b] <= t < offsets[b + 1] and stands at
         position start[b] + t - offsets[b]; without offsets row t is one
         token of sequence t. table [sequences, pages of each]."""
-        self._rows(_lib.bnn_kv_cache_write, d_k, d_v, table, start, offsets, stream)
+        self._rows(self._write, d_k, d_v, table, start, offsets, stream)
 
     def read(self, d_k, d_v, table, start, offsets=None, stream=None):
         """The values that such tokens have in the cache, into d_k and d_v;
         rows without a place are left as they were."""
-        self._rows(_lib.bnn_kv_cache_read, d_k, d_v, table, start, offsets, stream)
+        self._rows(self._read, d_k, d_v, table, start, offsets, stream)
 
     def attend_work(self, n_seqs, q_heads, prefix_tokens=0):
         """Bytes of workspace that such an `attend` needs."""
@@ -657,27 +701,41 @@ class KVCache(_LowBit):
         contiguous CUDA tensor of attend_work(...) bytes, for this call alone
         until it has run; lse: float32 [sequences, q_heads] or None; scale:
         head_dim ** -0.5 unless given."""
-        _arg(hasattr(d_q, "data_ptr") and d_q.dim() == 3, "q: a tensor [sequences, q_heads, head_dim] is needed")
-        seqs, heads = d_q.shape[0], d_q.shape[1]
-        self._tensor(lengths, "lengths", "torch.int32", (seqs,))
-        _arg(lengths.is_contiguous(), "lengths: not contiguous")
-        q, q_seq, q_head = self._heads(d_q, "q", seqs, heads)
-        out, o_seq, o_head = self._heads(d_out, "out", seqs, heads)
-        if lse is not None:
-            self._tensor(lse, "lse", "torch.float32", (seqs, heads))
-            _arg(lse.is_contiguous(), "lse: not contiguous")
-        pages = 0
-        if prefix is not None:
-            self._tensor(prefix, "prefix", "torch.int32", (None,))
-            _arg(prefix.is_contiguous(), "prefix: not contiguous")
-            pages = prefix.shape[0]
-        self._tensor(work, "work", str(work.dtype), None)
-        _check(_lib.bnn_kv_attend(
-            self.handle, q, q_seq, q_head, seqs, heads, lengths.data_ptr(), *self._table(table, seqs),
-            prefix.data_ptr() if pages else None, pages, prefix_tokens,
-            self.head_dim ** -0.5 if scale is None else scale, out, o_seq, o_head,
-            None if lse is None else lse.data_ptr(), work.data_ptr(), work.numel() * work.element_size(),
-            _stream(stream)))
+        try:
+            (seqs, heads, dim), (n, width), kind, whole, dev = d_q.shape, table.shape, self._kind, self._int, self.device
+            (qs, qh, q1), (os_, oh, o1) = d_q.stride(), d_out.stride()
+            ok = (dim == self.head_dim and d_out.shape == d_q.shape and n == seqs and lengths.shape == (seqs,) and q1 == 1
+                  and o1 == 1 and d_q.dtype is kind and d_out.dtype is kind and lengths.dtype is whole and table.dtype is whole
+                  and lengths.is_contiguous() and table.is_contiguous() and work.is_contiguous() and d_q.get_device() == dev
+                  and d_out.get_device() == dev and lengths.get_device() == dev and table.get_device() == dev
+                  and work.get_device() == dev)
+            p_lse, p_pre, pages = None, None, 0
+            if lse is not None:
+                p_lse = lse.data_ptr()
+                ok = (ok and lse.shape == (seqs, heads) and lse.dtype is self._float and lse.is_contiguous()
+                      and lse.get_device() == dev)
+            if prefix is not None:
+                p_pre, (pages,) = prefix.data_ptr(), prefix.shape
+                ok = ok and prefix.dtype is whole and prefix.is_contiguous() and prefix.get_device() == dev
+        except (AttributeError, ValueError, TypeError):
+            ok = False
+        if not ok:
+            new = self._types()
+            self._explain((d_q, "q", self._kind, (None, None, self.head_dim), False))
+            seqs, heads = d_q.shape[:2]
+            self._explain((d_out, "out", self._kind, tuple(d_q.shape), False), (lengths, "lengths", self._int, (seqs,), True),
+                          (table, "table", self._int, (seqs, None), True), (work, "work", None, None, True))
+            if lse is not None:
+                self._explain((lse, "lse", self._float, (seqs, heads), True))
+            if prefix is not None:
+                self._explain((prefix, "prefix", self._int, (None,), True))
+            _arg(new, "arguments that do not go together")
+            return self.attend(d_q, lengths, table, d_out, work, lse, scale, prefix, prefix_tokens, stream)
+        rc = self._attend(self.handle, d_q.data_ptr(), qs, qh, seqs, heads, lengths.data_ptr(), table.data_ptr(), width, p_pre,
+                          pages, prefix_tokens, self.head_dim ** -0.5 if scale is None else scale, d_out.data_ptr(), os_, oh,
+                          p_lse, work.data_ptr(), work.nbytes, _stream(stream))
+        if rc:
+            _check(rc)
 
     def close(self):
         if getattr(self, "handle", None):

@@ -66,7 +66,7 @@ __device__ __forceinline__ void cp_wait() {
 }
 __device__ __forceinline__ uint32_t movm_t(uint32_t a) {
     uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
     return d;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -112,7 +112,7 @@ __device__ __forceinline__ uint32_t pair8(uint32_t w) {  // bytes LO and LO + 1 
     return Fp16::sub2(__byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140), 0x64806480u);
 }
 __device__ __forceinline__ uint32_t pair4(uint32_t w, int nib) {  // nibbles at 4 * nib of both halves
-    return Fp16::sub2(((w >> (4 * nib)) & 0x000f000fu) | 0x64006400u, 0x64086408u);
+    return Fp16::sub2(and_or(w >> (4 * nib), 0x000f000fu, 0x64006400u), 0x64086408u);
 }
 
 template <int DP, int BITS>
@@ -664,8 +664,6 @@ Plan attend_plan(const bnn_kv_cache* c, int n_grp, int rg, bool partial) {
 
 template <int DP, int BITS, int NT>
 cudaError_t attend_launch(const AttendParams& p, const Plan& s, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(attend_kernel<DP, BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem);
-    if (e != cudaSuccess) return e;
     attend_kernel<DP, BITS, NT><<<s.ctas, 32 * kWarps, s.smem, st>>>(p);
     return cudaGetLastError();
 }
@@ -689,6 +687,26 @@ cudaError_t attend_one(const AttendParams& p, const Plan& s, cudaStream_t st) {
     return p.g.bits == 8 ? attend_dim<8>(p, s, st) : attend_dim<4>(p, s, st);
 }
 
+// the kernels of a cache may use all of an SM's shared memory: set once, when the cache is made
+template <int DP, int BITS>
+cudaError_t attend_setup_rows() {
+    constexpr int all = 226 * 1024;
+    cudaError_t e = cudaFuncSetAttribute(attend_kernel<DP, BITS, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, all);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<DP, BITS, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, all);
+    if constexpr (DP <= 128)
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<DP, BITS, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, all);
+    return e;
+}
+template <int BITS>
+cudaError_t attend_setup_dim(int dp) {
+    switch (dp) {
+        case 64: return attend_setup_rows<64, BITS>();
+        case 128: return attend_setup_rows<128, BITS>();
+        case 192: return attend_setup_rows<192, BITS>();
+        default: return attend_setup_rows<256, BITS>();
+    }
+}
+
 constexpr int kMaxSeqs = 16384;
 
 int attend_check(const bnn_kv_cache* c, int n_seqs, int q_heads, int prefix_tokens) {
@@ -700,6 +718,9 @@ int attend_check(const bnn_kv_cache* c, int n_seqs, int q_heads, int prefix_toke
 }
 
 }  // namespace
+
+cudaError_t attend_setup(const KvGeo& g) { return g.bits == 8 ? attend_setup_dim<8>(g.dp) : attend_setup_dim<4>(g.dp); }
+
 }  // namespace lowbit
 }  // namespace bnn
 

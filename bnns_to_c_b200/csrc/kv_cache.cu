@@ -203,6 +203,7 @@ int kv_create(bnn_kv_cache* c) {
     DeviceScope dev(c->device);
     if (dev.err != cudaSuccess) return cuda_error("bnn_kv_cache_create", dev.err);
     cudaError_t e = cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device);
+    if (e == cudaSuccess) e = attend_setup(g);
     if (e != cudaSuccess) return cuda_error("bnn_kv_cache_create", e);
     const int rc = device_alloc(&c->base, c->bytes, "of a key/value cache");
     if (rc) return rc;

@@ -1,6 +1,8 @@
 // kv_cache.h - the handle of the block-scaled key/value cache, shared by its
 // write and read (kv_cache.cu) and the attention (kv_attend.cu).
 #pragma once
+#include <cuda_runtime.h>
+
 #include "lowbit.h"
 
 struct bnn_kv_cache {
@@ -13,3 +15,10 @@ struct bnn_kv_cache {
     uint16_t *ks, *vs;  // their scales
     size_t bytes;
 };
+
+namespace bnn {
+namespace lowbit {
+// sets what the attention kernels of such a cache need on the current device
+cudaError_t attend_setup(const KvGeo& g);
+}  // namespace lowbit
+}  // namespace bnn

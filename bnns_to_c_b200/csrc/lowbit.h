@@ -17,11 +17,12 @@ namespace lowbit {
 
 // ---------------------------------------------------------------- 4-bit linear layer
 // A tile is 16 output rows x 64 inputs, 512 bytes: lane (r = lane / 4,
-// j = lane % 4) of a warp owns 16 of them, word i of its four being the A
-// fragment of one m16n8k16 step. The inputs of a step may come in any order
-// as long as both operands agree, and the order here lets a lane read its
-// part of x as 8 neighbouring values per 32 inputs: step i of lane j covers
-// inputs 32 * (i / 2) + 8 * j + 4 * (i % 2) + {0, 1 | 2, 3}.
+// j = lane % 4) of a warp owns 16 of them, word i of its four being the part
+// that it has of a 16 x 16 operand of the tensor cores: rows r and r + 8,
+// inputs 16 * i + 4 * j + 0..3. That is the A fragment of an m16n8k16
+// mma.sync (whose inputs may come in any order that x follows), and of
+// tcgen05.st.16x256b, which puts the 16 rows into tensor memory with the
+// inputs in their own order.
 // Word: nibble p (bits 4p and 16 + 4p) holds the pair of inputs 2 * (p / 2)
 // + {0, 1} of row r + 8 * (p % 2), so (word >> 4p) & 0x000f000f is register
 // a_p of the fragment, two codes at the bottom of two 16-bit halves.
@@ -43,8 +44,8 @@ LB_HD int64_t q4_words(const Q4Geo& g) { return (int64_t)g.tiles * g.kb * 128; }
 LB_HD int64_t q4_word(const Q4Geo& g, int tile, int kb, int lane) { return (((int64_t)tile * g.kb + kb) * 32 + lane) * 4; }
 // row and input of nibble `nib` (0..7) of word i of a lane, within the tile
 LB_HD int q4_row(int lane, int nib) { return (lane >> 2) + 8 * (nib & 1); }
-LB_HD int q4_in(int lane, int i, int nib) { return 32 * (i >> 1) + 8 * (lane & 3) + 4 * (i & 1) + 2 * ((nib >> 1) & 1) + (nib >> 2); }
-// scales and zero points: [tile][group][r][row r, row r + 8]
+LB_HD int q4_in(int lane, int i, int nib) { return 16 * i + 4 * (lane & 3) + 2 * ((nib >> 1) & 1) + (nib >> 2); }
+// place of a scale: [tile][group][r][row r, row r + 8]
 LB_HD int64_t q4_scale(const Q4Geo& g, int row, int grp) {
     return (((int64_t)(row >> 4) * g.ng + grp) * 8 + (row & 7)) * 2 + ((row >> 3) & 1);
 }

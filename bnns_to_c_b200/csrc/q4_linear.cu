@@ -1,5 +1,9 @@
 // q4_linear.cu - the 4-bit linear layer of include/bnn_lowbit.h.
+#include <cmath>
+#include <mutex>
 #include <new>
+
+#include <cuda.h>
 
 #include "lowbit_dev.cuh"
 
@@ -9,8 +13,7 @@ struct bnn_q4_layer {
     bnn::lowbit::Q4Geo geo;
     void* base;              // one allocation, in this order:
     const uint32_t* codes;   //   q4_words
-    const uint16_t* scales;  //   q4_scales, in the layer's type
-    const uint8_t* zeros;    //   q4_scales
+    const uint2* sz;         //   q4_scales / 2 times: scales and zero points of two rows
     const float* bias;       //   [n_out] or nullptr
 };
 
@@ -21,8 +24,8 @@ namespace {
 // ---------------------------------------------------------------- layout, once
 // Padding: an input behind the last has code = zero point (weight 0), a row
 // behind the last has scale 0.
-__global__ void q4_layout_kernel(Q4Geo g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, uint32_t* wo,
-                                 uint16_t* so, uint8_t* zo) {
+__global__ void q4_layout_kernel(Q4Geo g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, uint32_t magic,
+                                 uint32_t* wo, uint16_t* szo) {
     const int64_t words = q4_words(g), step = (int64_t)gridDim.x * blockDim.x;
     const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t half = ((int64_t)g.K + 1) / 2;
@@ -47,135 +50,562 @@ __global__ void q4_layout_kernel(Q4Geo g, const uint8_t* codes, const uint16_t* 
     for (int64_t s = first; s < (int64_t)g.tiles * 16 * g.ng; s += step) {
         const int row = (int)(s / g.ng), grp = (int)(s % g.ng);
         const int64_t at = q4_scale(g, row, grp);
-        so[at] = row < g.N ? scales[s] : (uint16_t)0;
-        zo[at] = row < g.N && zeros ? (uint8_t)(zeros[s] & 15u) : (uint8_t)8;
+        uint16_t* to = szo + (at >> 1) * 4 + (at & 1);  // a pair of rows: two scales, two zero points
+        to[0] = row < g.N ? scales[s] : (uint16_t)0;
+        to[2] = (uint16_t)(magic | (row < g.N && zeros ? zeros[s] & 15u : 8u));
     }
 }
 
 struct Q4Params {
     Q4Geo g;
     const uint4* w;
-    const uint32_t* s;  // pairs (row r, row r + 8)
-    const uint16_t* z;  // pairs
+    const uint2* sz;  // [tile][group][r]: scales of rows r and r + 8, then magic + zero point of both
     const float* bias;
     const uint16_t* x;
     int64_t xs;
     uint16_t* y;
     int64_t ys;
     int M;
-    bool vec;  // rows of x are 16-byte aligned
+    int gshift;       // group = 32 << gshift, or -1
+    bool vec4, vec8;  // rows of x start 8-byte, 16-byte aligned
 };
 
 // ---------------------------------------------------------------- rows on mma.sync
-// One CTA makes a tile of 16 outputs for 8 * NT rows of x; its 8 warps take
-// the 64-input blocks in turn and their sums are joined in shared memory.
+// Up to 16 rows: bound by reading the weights. A CTA makes MT tiles of 16
+// outputs for 8 * NT rows of x; its warps take chunks of U 64-input blocks in
+// turn and their sums are joined in shared memory. The weights of the next
+// chunk are on their way while one is multiplied: U * MT * 512 bytes a warp.
 // (q - z) is exact in 16 bits (|q - z| <= 15), so a group's sum of products
 // has only the rounding of 32-bit sums, and its scale is applied to that sum.
+// X: how x can be read: 2 = 8 bytes at a time, K a multiple of 64; 1 = 8 bytes
+// at a time; 0 = value by value.
 constexpr int kQ4Warps = 8;
 
-template <class A, int NT>
-__global__ void __launch_bounds__(32 * kQ4Warps) q4_rows_kernel(const Q4Params p) {
-    __shared__ float red[kQ4Warps][8 * NT][17];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+template <int MT, int U, int SZ>
+struct Q4Chunk {
+    uint4 w[U][MT];
+    uint2 sz[U][MT][SZ];
+};
+
+template <class A, int NT, int MT, int U, bool G32, int X>
+__global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Params p) {
+    extern __shared__ float red[];  // [warp][8 * NT][16 * MT + 1]
+    constexpr int PITCH = 16 * MT + 1;
+    constexpr int SZ = G32 ? 2 : 1;  // scales a block
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be one number a warp
     const int r = lane >> 2, j = lane & 3;
-    const int tile = blockIdx.x, m0 = blockIdx.y * 8 * NT;
+    const int tile0 = blockIdx.x * MT, m0 = blockIdx.y * 8 * NT;
     const Q4Geo g = p.g;
-    float acc[NT][4] = {};
-    for (int kb = warp; kb < g.kb; kb += kQ4Warps) {
-        const uint4 w4 = ldg_stream(p.w + ((int64_t)tile * g.kb + kb) * 32 + lane);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+    // Whole chunks first, U blocks at a time, the warps in turn; the blocks
+    // that are left over one at a time. A few blocks go one at a time, too.
+    const int whole = g.kb >= U * warps ? g.kb / U : 0;
+    int n = whole > warp ? (whole - warp + warps - 1) / warps : 0;
+    int kb = warp * U;
+
+    // rows of x behind the last are the first one again: a row has columns of
+    // its own in the products, and these are not stored
+    const uint16_t* xr[NT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = kb * 64 + h * 32, grp = min(k / g.group, g.ng - 1);
-            const int64_t at = ((int64_t)tile * g.ng + grp) * 8 + r;
-            const uint32_t zz = p.z[at], ss = p.s[at];
-            const uint32_t z0 = (zz & 0xffu) * 0x00010001u | A::kMagic, z1 = (zz >> 8) * 0x00010001u | A::kMagic;
-            uint4 xv[NT];
+    for (int t = 0; t < NT; ++t) {
+        const int m = m0 + t * 8 + r;
+        xr[t] = p.x + (m < p.M ? m * p.xs : 0) + 4 * j;
+    }
+    const uint4* wr[MT];
+    const uint2* sr[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int tile = min(tile0 + i, g.tiles - 1);  // a tile behind the last repeats it, unused
+        wr[i] = p.w + (int64_t)tile * g.kb * 32 + lane;
+        sr[i] = p.sz + (int64_t)tile * g.ng * 8 + r;
+    }
+    float acc[MT][NT][4] = {};
+    using Chunk = Q4Chunk<MT, U, SZ>;
+    const auto fetch = [&](Chunk& c, int at, int count) {
+#pragma unroll
+        for (int u = 0; u < count; ++u) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) c.w[u][i] = __ldcs(wr[i] + (at + u) * 32);
+#pragma unroll
+            for (int h = 0; h < SZ; ++h) {
+                int grp = p.gshift >= 0 ? (2 * (at + u) + h) >> p.gshift : (2 * (at + u) + h) / (g.group >> 5);
+                if (G32) grp = min(grp, g.ng - 1);  // the second half of the last block may be padding alone
+#pragma unroll
+                for (int i = 0; i < MT; ++i) c.sz[u][i][h] = __ldg(sr[i] + grp * 8);
+            }
+        }
+    };
+    const auto multiply = [&](const Chunk& q, int at, int count) {
+#pragma unroll
+        for (int u = 0; u < count; ++u) {
+            uint2 xv[4][NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const int m = m0 + t * 8 + r, kk = k + 8 * j;
-                xv[t] = m < p.M && kk < g.K ? load8(p.x + m * p.xs + kk, g.K - kk, p.vec) : make_uint4(0, 0, 0, 0);
+                const uint16_t* xp = xr[t] + (at + u) * 64;
+                const int left = g.K - (at + u) * 64 - 4 * j;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (X == 2 || (X == 1 && e * 16 < left)) xv[e][t] = __ldg(reinterpret_cast<const uint2*>(xp + e * 16));
+                    else xv[e][t] = X == 0 ? load4(xp + e * 16, left - e * 16) : make_uint2(0, 0);
+                }
             }
-            float c[NT][4] = {};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t v = w[h * 2 + i];
-                uint32_t a[4];
+            for (int i = 0; i < MT; ++i) {
+                const uint32_t w[4] = {q.w[u][i].x, q.w[u][i].y, q.w[u][i].z, q.w[u][i].w};
+                float c[NT][4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    a[q] = A::sub2(((v >> (4 * q)) & 0x000f000fu) | A::kMagic, q & 1 ? z1 : z0);
+                for (int e = 0; e < 4; ++e) {
+                    const uint2 sz = q.sz[u][i][G32 ? e >> 1 : 0];
+                    const uint32_t z0 = __byte_perm(sz.y, 0, 0x1010), z1 = __byte_perm(sz.y, 0, 0x3232);
+                    uint32_t a[4];
+                    A::weights(a, w[e], z0, z1);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) A::mma(c[t], a, i ? xv[t].z : xv[t].x, i ? xv[t].w : xv[t].y);
+                    for (int t = 0; t < NT; ++t) {
+                        if (e == 0 || (G32 && e == 2)) A::mma0(c[t], a, xv[e][t].x, xv[e][t].y);
+                        else A::mma(c[t], a, xv[e][t].x, xv[e][t].y);
+                    }
+                    if (e == 3 || (G32 && e == 1)) {
+                        const float2 s = A::unpack(sz.x);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            acc[i][t][0] = fmaf(s.x, c[t][0], acc[i][t][0]);
+                            acc[i][t][1] = fmaf(s.x, c[t][1], acc[i][t][1]);
+                            acc[i][t][2] = fmaf(s.y, c[t][2], acc[i][t][2]);
+                            acc[i][t][3] = fmaf(s.y, c[t][3], acc[i][t][3]);
+                        }
+                    }
+                }
             }
-            const uint16_t sh0 = (uint16_t)ss, sh1 = (uint16_t)(ss >> 16);
-            const float s0 = A::to_float(*reinterpret_cast<const typename A::T*>(&sh0));
-            const float s1 = A::to_float(*reinterpret_cast<const typename A::T*>(&sh1));
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                acc[t][0] = fmaf(s0, c[t][0], acc[t][0]);
-                acc[t][1] = fmaf(s0, c[t][1], acc[t][1]);
-                acc[t][2] = fmaf(s1, c[t][2], acc[t][2]);
-                acc[t][3] = fmaf(s1, c[t][3], acc[t][3]);
-            }
+        }
+    };
+    {
+        Chunk c0, c1;
+        const int step = warps * U;
+        if (n > 0) fetch(c0, kb, U);
+        while (n > 0) {
+            if (n > 1) fetch(c1, kb + step, U);
+            multiply(c0, kb, U);
+            kb += step;
+            if (--n == 0) break;
+            if (n > 1) fetch(c0, kb + step, U);
+            multiply(c1, kb, U);
+            kb += step;
+            --n;
+        }
+        for (kb = whole * U + warp; kb < g.kb; kb += warps) {
+            fetch(c0, kb, 1);
+            multiply(c0, kb, 1);
         }
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) red[warp][t * 8 + 2 * j + (e & 1)][r + 8 * (e >> 1)] = acc[t][e];
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                red[(warp * 8 * NT + t * 8 + 2 * j + (e & 1)) * PITCH + 16 * i + r + 8 * (e >> 1)] = acc[i][t][e];
     __syncthreads();
-    for (int i = threadIdx.x; i < 128 * NT; i += blockDim.x) {
-        const int m = m0 + (i >> 4), n = tile * 16 + (i & 15);
+    for (int i = threadIdx.x; i < 128 * NT * MT; i += blockDim.x) {
+        const int t = i / (16 * MT), o = i % (16 * MT), m = m0 + t, n = tile0 * 16 + o;
         if (m >= p.M || n >= g.N) continue;
         float v = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kQ4Warps; ++k) v += red[k][i >> 4][i & 15];
+        for (int k = 0; k < warps; ++k) v += red[(k * 8 * NT + t) * PITCH + o];
         if (p.bias) v += p.bias[n];
-        const typename A::T o = A::from_float(v);
-        p.y[m * p.ys + n] = *reinterpret_cast<const uint16_t*>(&o);
+        const typename A::T out = A::from_float(v);
+        p.y[m * p.ys + n] = *reinterpret_cast<const uint16_t*>(&out);
     }
 }
 
-template <class A, int NT>
+template <class A, int NT, int MT, int U, bool G32, int X>
 cudaError_t q4_launch(const Q4Params& p, cudaStream_t st) {
-    const dim3 grid((unsigned)p.g.tiles, (unsigned)cdiv64(p.M, 8 * NT));
-    q4_rows_kernel<A, NT><<<grid, 32 * kQ4Warps, 0, st>>>(p);
+    const dim3 grid((unsigned)cdiv64(p.g.tiles, MT), (unsigned)cdiv64(p.M, 8 * NT));
+    // warps of a CTA: as many as there are chunks, 4 where the tiles alone
+    // give every SM several CTAs
+    const int warps = p.g.kb < kQ4Warps ? p.g.kb : kQ4Warps;
+    q4_rows_kernel<A, NT, MT, U, G32, X><<<grid, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st>>>(p);
     return cudaGetLastError();
 }
+template <class A, int NT, int MT, int U>
+cudaError_t q4_forms(const Q4Params& p, cudaStream_t st) {
+    const int x = !p.vec4 || p.g.K % 4 ? 0 : p.g.K % 64 ? 1 : 2;
+    if (p.g.group % 64)
+        return x == 2 ? q4_launch<A, NT, MT, U, true, 2>(p, st) : x == 1 ? q4_launch<A, NT, MT, U, true, 1>(p, st) : q4_launch<A, NT, MT, U, true, 0>(p, st);
+    return x == 2 ? q4_launch<A, NT, MT, U, false, 2>(p, st) : x == 1 ? q4_launch<A, NT, MT, U, false, 1>(p, st) : q4_launch<A, NT, MT, U, false, 0>(p, st);
+}
+// ---------------------------------------------------------------- tiles on tcgen05
+// More rows: bound by the products. A CTA makes 128 outputs x NTOK rows of x
+// (of K, or of a cluster's share of K): D[output][row] in tensor memory. The
+// weights are the A operand: eight warps turn codes into (q - z) * s in 16
+// bits and store them into tensor memory as they come from their word
+// (16x256b), so that shared memory carries x alone: B, 64 inputs a stage,
+// 128-byte swizzle, by TMA, or by four warps where x is not aligned for it.
+// One thread issues the products. With weights in shared memory, too, its
+// 128 bytes a clock would hold an NTOK = 256 tile to two thirds of the rate.
+// Rounding a weight to 16 bits costs 2^-9 (bf16; fp16 2^-12) of a product, as
+// much as the rounding of the result costs; the products' errors are
+// independent, so the result stays within sqrt(2) of its own rounding.
+constexpr int kTileWarps = 13;  // 0-7 weights, then results; 8 products; 9-12 x
+constexpr int kTileStages = 4;
+__device__ unsigned int g_q4_wait_timeouts = 0;
+
+struct Q4TileParams {
+    Q4Params q;
+    int shares;  // of K: CTAs of a cluster
+    bool tma;
+};
+
+constexpr int q4_tile_cols(int ntok) { return ntok + 32 * kTileStages <= 256 ? 256 : 512; }
+constexpr int q4_tile_smem(int ntok) {
+    const int ring = kTileStages * ntok * 128;
+    // at most two CTAs an SM where tensor memory has room for two: a third
+    // would wait for its columns with the rest of its cluster waiting for it
+    return ring < 78 * 1024 ? 78 * 1024 : ring;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// into the shared memory of CTA `rank` of the cluster
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+}
+
+template <class A, int NTOK, bool G32>
+__global__ void __launch_bounds__(32 * kTileWarps, NTOK == 256 ? 1 : 2)
+    q4_tiles_kernel(const Q4TileParams tp, const __grid_constant__ CUtensorMap map) {
+    constexpr int S = kTileStages, STAGE = NTOK * 128, COLS = q4_tile_cols(NTOK);
+    extern __shared__ __align__(1024) uint8_t ring[];
+    __shared__ __align__(8) uint64_t bars[3 * S + 1];
+    __shared__ uint32_t tmem_s;
+    __shared__ int gave_up;
+    const Q4Params& p = tp.q;
+    const Q4Geo& g = p.g;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int tile0 = blockIdx.x * 8, m0 = blockIdx.y * NTOK;
+    const int share = tp.shares > 1 ? (int)cluster_rank() : 0;
+    const int kb0 = (int)((int64_t)g.kb * share / tp.shares), nk = (int)((int64_t)g.kb * (share + 1) / tp.shares) - kb0;
+    const uint32_t full_w = smem_addr(bars), full_x = full_w + 8 * S, empty = full_x + 8 * S, done = empty + 8 * S;
+    if (warp == 8) t5_alloc(smem_addr(&tmem_s), COLS);
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            bar_init(full_w + 8 * s, 8);
+            bar_init(full_x + 8 * s, tp.tma ? 1 : 4);
+            bar_init(empty + 8 * s, 1);
+        }
+        bar_init(done, 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    t5_before();
+    __syncthreads();
+    t5_after();
+    const uint32_t tmem = tmem_s;
+
+    if (warp < 8) {
+        // 16 outputs a warp: lanes 32 * (warp % 4) + 16 * (warp / 4) of tensor memory
+        const int tile = min(tile0 + 2 * (warp & 3) + (warp >> 2), g.tiles - 1);
+        const uint4* wp = p.w + ((int64_t)tile * g.kb + kb0) * 32 + lane;
+        const uint2* sp = p.sz + (int64_t)tile * g.ng * 8 + (lane >> 2);
+        const uint32_t to = tmem + NTOK + ((uint32_t)(32 * (warp & 3) + 16 * (warp >> 2)) << 16);
+        constexpr int AHEAD = 2;
+        uint4 w[AHEAD];
+        uint2 sz[AHEAD][G32 ? 2 : 1];
+        const auto fetch = [&](int slot, int it) {
+            w[slot] = __ldcs(wp + it * 32);
+#pragma unroll
+            for (int h = 0; h < (G32 ? 2 : 1); ++h) {
+                const int b = 2 * (kb0 + it) + h;
+                sz[slot][h] = __ldg(sp + min(p.gshift >= 0 ? b >> p.gshift : b / (g.group >> 5), g.ng - 1) * 8);
+            }
+        };
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+            if (a < nk) fetch(a, a);
+        for (int it0 = 0; it0 < nk; it0 += AHEAD) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int it = it0 + a, s = it % S;
+                if (it >= nk) break;
+                uint32_t v[16];
+                const uint32_t ww[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint2 q = sz[a][G32 ? e >> 1 : 0];
+                    const uint32_t s0 = __byte_perm(q.x, 0, 0x1010), s1 = __byte_perm(q.x, 0, 0x3232);
+                    uint32_t f[4];
+                    A::weights(f, ww[e], __byte_perm(q.y, 0, 0x1010), __byte_perm(q.y, 0, 0x3232));
+                    v[4 * e] = A::mul2(f[0], s0), v[4 * e + 1] = A::mul2(f[2], s0);
+                    v[4 * e + 2] = A::mul2(f[1], s1), v[4 * e + 3] = A::mul2(f[3], s1);
+                }
+                if (it + AHEAD < nk) fetch(a, it + AHEAD);
+                if (it >= S) {
+                    if (!__all_sync(0xffffffffu, bar_wait(empty + 8 * s, (it / S - 1) & 1, &gave_up))) {
+                        it0 = nk;
+                        break;
+                    }
+                    t5_after();
+                }
+                t5_st_16x256b_x4(to + 32 * s, v);
+                t5_wait_st();
+                t5_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(full_w + 8 * s);
+            }
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = (1u << 4) | (A::kMmaType << 7) | (A::kMmaType << 10) | ((uint32_t)(NTOK >> 3) << 17) | (8u << 24);
+            for (int it = 0; it < nk; ++it) {
+                const int s = it % S;
+                if (!bar_wait(full_x + 8 * s, (it / S) & 1, &gave_up) || !bar_wait(full_w + 8 * s, (it / S) & 1, &gave_up)) break;
+                t5_after();
+                // K-major, 128-byte swizzle: 8 rows of 128 bytes 1024 bytes apart
+                const uint64_t b = (uint64_t)((smem_addr(ring) + s * STAGE) >> 4 & 0x3fffu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t5_mma_ts(tmem, tmem + NTOK + 32 * s + 8 * e, b + 2 * e, idesc, it > 0 || e > 0);
+                t5_commit(empty + 8 * s);
+            }
+            t5_commit(done);
+        }
+    } else if (tp.tma) {
+        if (warp == 9 && lane == 0) {
+            int it = 0;
+            for (; it < nk; ++it) {
+                const int s = it % S;
+                if (it >= S && !bar_wait(empty + 8 * s, (it / S - 1) & 1, &gave_up)) break;
+                bar_arrive_tx(full_x + 8 * s, STAGE);
+                tma_2d(smem_addr(ring) + s * STAGE, &map, (kb0 + it) * 64, m0, full_x + 8 * s);
+            }
+            // copies that nothing waits for any more still have to land before the CTA ends
+            if (it < nk)
+                for (int o = it > S ? it - S : 0; o < it; ++o) {
+                    int alone = 0;
+                    bar_wait(full_x + 8 * (o % S), (o / S) & 1, &alone);
+                }
+        }
+    } else {
+        for (int it = 0; it < nk; ++it) {
+            const int s = it % S;
+            if (it >= S && !__all_sync(0xffffffffu, bar_wait(empty + 8 * s, (it / S - 1) & 1, &gave_up))) break;
+            uint8_t* st = ring + s * STAGE;
+            for (int i = tid - 32 * 9; i < NTOK * 8; i += 128) {
+                const int row = i >> 3, c = i & 7, m = m0 + row, k = (kb0 + it) * 64 + 8 * c;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (m < p.M && k < g.K) {
+                    const uint16_t* x = p.x + m * p.xs + k;
+                    if (p.vec4 && k + 8 <= g.K) {
+                        const uint2 lo = __ldg(reinterpret_cast<const uint2*>(x)), hi = __ldg(reinterpret_cast<const uint2*>(x) + 1);
+                        v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    } else {
+                        v = load8(x, g.K - k, false);
+                    }
+                }
+                *reinterpret_cast<uint4*>(st + row * 128 + ((c ^ (row & 7)) << 4)) = v;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(full_x + 8 * s);
+        }
+    }
+    __syncwarp();
+
+    // results
+    bool ok = true;
+    if (warp < 8) {
+        ok = __all_sync(0xffffffffu, bar_wait(done, 0, &gave_up));
+        t5_after();
+    }
+    const int n = tile0 * 16 + 32 * (warp & 3) + lane;
+    constexpr int HALF = NTOK / 2;
+    const int c0 = HALF * (warp >> 2);
+    if (tp.shares == 1) {
+        if (warp < 8 && ok) {
+            const float bias = p.bias && n < g.N ? p.bias[n] : 0.0f;
+#pragma unroll 1
+            for (int c = c0; c < c0 + HALF; c += 16) {
+                uint32_t v[16];
+                t5_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c, v);
+                if (n < g.N) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (m0 + c + i < p.M) {
+                            const typename A::T o = A::from_float(__uint_as_float(v[i]) + bias);
+                            p.y[(m0 + c + i) * p.ys + n] = *reinterpret_cast<const uint16_t*>(&o);
+                        }
+                }
+            }
+        }
+    } else {
+        // Each CTA joins NTOK / shares of the rows, in the order of the
+        // shares; the others' sums come into its ring, which all are done with.
+        const int mine = NTOK / tp.shares;
+        cluster_sync();
+        if (warp < 8 && ok) {
+#pragma unroll 1
+            for (int c = c0; c < c0 + HALF; c += 16) {
+                uint32_t v[16];
+                t5_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c, v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    st_cluster(smem_addr(ring) + ((share * mine + (c + i) % mine) * 128 + 32 * (warp & 3) + lane) * 4, (c + i) / mine,
+                               __uint_as_float(v[i]));
+            }
+        }
+        cluster_sync();
+        const float* sums = reinterpret_cast<const float*>(ring);
+        for (int i = tid; i < mine * 128; i += 32 * kTileWarps) {
+            const int m = m0 + share * mine + (i >> 7), o = tile0 * 16 + (i & 127);
+            if (m >= p.M || o >= g.N) continue;
+            float v = 0.0f;
+            for (int r = 0; r < tp.shares; ++r) v += sums[r * mine * 128 + i];
+            if (p.bias) v += p.bias[o];
+            const typename A::T out = A::from_float(v);
+            p.y[m * p.ys + o] = *reinterpret_cast<const uint16_t*>(&out);
+        }
+    }
+    t5_before();
+    __syncthreads();
+    if (warp == 8) {
+        if (gave_up) {  // products may still be running
+            int alone = 0;
+            bar_wait(done, 0, &alone);
+            if (lane == 0) atomicAdd(&g_q4_wait_timeouts, 1u);
+        }
+        t5_after();
+        t5_free(tmem, COLS);
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)f;
+        cudaGetLastError();
+    });
+    return fn;
+}
+
+template <class A, int NTOK, bool G32>
+cudaError_t q4_tiles_launch(const Q4TileParams& p, const CUtensorMap& map, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cdiv64(p.q.g.tiles, 8), (unsigned)cdiv64(p.q.M, NTOK), (unsigned)p.shares);
+    cfg.blockDim = dim3(32 * kTileWarps);
+    cfg.dynamicSmemBytes = q4_tile_smem(NTOK);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = (unsigned)p.shares;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, q4_tiles_kernel<A, NTOK, G32>, p, map);
+}
+
+// Rows a tile and shares of K: the pair with the least estimated clocks, of
+// the busiest SM: a 64-input block of a tile costs 2 * NTOK of products or
+// 160 of weights, a CTA 3000 to start and end, a joined one 1500 more.
+void q4_tiles_choose(const Q4Params& p, int* ntok, int* shares) {
+    double best = 1e30;
+    for (int t = 32; t <= 256; t *= 2) {
+        if (t > 32 && t / 2 >= p.M) break;
+        for (int c = 1; c <= 8; c *= 2) {
+            if (c > 1 && p.g.kb < 8 * c) break;
+            const int64_t ctas = cdiv64(p.g.tiles, 8) * cdiv64(p.M, t) * c;
+            const double busiest = (double)cdiv64(ctas, 148), at_once = t == 256 ? 1 : 2;
+            const double clocks = busiest * ((double)p.g.kb / c) * (t < 80 ? 160 : 2 * t) + ceil(busiest / at_once) * 3000 + (c > 1 ? 1500 : 0);
+            if (clocks < best) best = clocks, *ntok = t, *shares = c;
+        }
+    }
+}
+
+template <class A, bool G32>
+cudaError_t q4_tiles(const Q4Params& p, cudaStream_t st) {
+    Q4TileParams tp{};
+    tp.q = p;
+    int ntok = 32;
+    q4_tiles_choose(p, &ntok, &tp.shares);
+    CUtensorMap map{};
+    EncodeTiledFn fn = p.vec8 ? encode_tiled() : nullptr;
+    if (fn) {
+        const cuuint64_t dims[2] = {(cuuint64_t)p.g.K, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.xs * 2};
+        const cuuint32_t box[2] = {64, (cuuint32_t)ntok}, step[2] = {1, 1};
+        tp.tma = p.xs * 2 < (1ll << 40) &&
+                 fn(&map, A::kTmaType, 2, (void*)p.x, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    switch (ntok) {
+        case 32: return q4_tiles_launch<A, 32, G32>(tp, map, st);
+        case 64: return q4_tiles_launch<A, 64, G32>(tp, map, st);
+        case 128: return q4_tiles_launch<A, 128, G32>(tp, map, st);
+        default: return q4_tiles_launch<A, 256, G32>(tp, map, st);
+    }
+}
+template <class A, bool G32>
+cudaError_t q4_tiles_setup() {
+    cudaError_t e = cudaFuncSetAttribute(q4_tiles_kernel<A, 32, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize, q4_tile_smem(32));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(q4_tiles_kernel<A, 64, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize, q4_tile_smem(64));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(q4_tiles_kernel<A, 128, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize, q4_tile_smem(128));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(q4_tiles_kernel<A, 256, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize, q4_tile_smem(256));
+    return e;
+}
+
 template <class A>
 cudaError_t q4_run(const Q4Params& p, cudaStream_t st) {
-    if (p.M <= 8) return q4_launch<A, 1>(p, st);
-    if (p.M <= 16) return q4_launch<A, 2>(p, st);
-    return q4_launch<A, 4>(p, st);
+    // Two tiles a CTA share their loads of x, where there are tiles enough
+    // for every SM. 8192 x 8192, one row: 11.6 us against 13.4 of one tile a
+    // CTA; 4096 x 4096: 5.9 against 5.0.
+    if (p.M <= 8) return p.g.tiles >= 3 * 148 ? q4_forms<A, 1, 2, 2>(p, st) : q4_forms<A, 1, 1, 4>(p, st);
+    if (p.M <= 16) return q4_forms<A, 2, 2, 1>(p, st);
+    return p.g.group % 64 ? q4_tiles<A, true>(p, st) : q4_tiles<A, false>(p, st);
 }
 
 int q4_create(bnn_q4_layer* L, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias) {
     const Q4Geo& g = L->geo;
     DeviceScope dev(L->device);
-    if (dev.err != cudaSuccess) return cuda_error("bnn_q4_layer_create", dev.err);
+    cudaError_t e = dev.err;
+    if (e == cudaSuccess) e = q4_tiles_setup<Bf16, false>();
+    if (e == cudaSuccess) e = q4_tiles_setup<Bf16, true>();
+    if (e == cudaSuccess) e = q4_tiles_setup<Fp16, false>();
+    if (e == cudaSuccess) e = q4_tiles_setup<Fp16, true>();
+    if (e != cudaSuccess) return cuda_error("bnn_q4_layer_create", e);
     const auto up = [](int64_t n) { return (size_t)((n + 255) & ~(int64_t)255); };
-    const size_t bw = up(q4_words(g) * 4), bs = up(q4_scales(g) * 2), bz = up(q4_scales(g)), bb = bias ? up((int64_t)g.N * 4) : 0;
-    int rc = device_alloc(&L->base, bw + bs + bz + bb, "of a 4-bit layer");
+    const size_t bw = up(q4_words(g) * 4), bs = up(q4_scales(g) * 4), bb = bias ? up((int64_t)g.N * 4) : 0;
+    int rc = device_alloc(&L->base, bw + bs + bb, "of a 4-bit layer");
     if (rc) return rc;
     char* at = (char*)L->base;
     L->codes = (const uint32_t*)at;
-    L->scales = (const uint16_t*)(at + bw);
-    L->zeros = (const uint8_t*)(at + bw + bs);
-    L->bias = bias ? (const float*)(at + bw + bs + bz) : nullptr;
+    L->sz = (const uint2*)(at + bw);
+    L->bias = bias ? (const float*)(at + bw + bs) : nullptr;
     // the caller's arrays (host or device memory) in device memory, for the layout kernel
     const int64_t half = ((int64_t)g.K + 1) / 2, ns = (int64_t)g.N * g.ng;
     const size_t rw = up(g.N * half), rs = up(ns * 2), rz = zeros ? up(ns) : 0;
     void* tmp = nullptr;
     if ((rc = device_alloc(&tmp, rw + rs + rz, "of a 4-bit layer's raw arrays"))) return rc;
     uint8_t *dw = (uint8_t*)tmp, *ds = dw + rw, *dz = ds + rs;
-    cudaError_t e = cudaMemcpy(dw, codes, g.N * half, cudaMemcpyDefault);
+    e = cudaMemcpy(dw, codes, g.N * half, cudaMemcpyDefault);
     if (e == cudaSuccess) e = cudaMemcpy(ds, scales, ns * 2, cudaMemcpyDefault);
     if (e == cudaSuccess && zeros) e = cudaMemcpy(dz, zeros, ns, cudaMemcpyDefault);
     if (e == cudaSuccess && bias) e = cudaMemcpy((void*)L->bias, bias, (size_t)g.N * 4, cudaMemcpyDefault);
     if (e == cudaSuccess) {
         const int64_t blocks = cdiv64(q4_words(g), 256);
         q4_layout_kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256>>>(
-            g, dw, (const uint16_t*)ds, zeros ? dz : nullptr, (uint32_t*)L->codes, (uint16_t*)L->scales, (uint8_t*)L->zeros);
+            g, dw, (const uint16_t*)ds, zeros ? dz : nullptr, (L->type == BNN_BF16 ? Bf16::kMagic : Fp16::kMagic) & 0xffffu,
+            (uint32_t*)L->codes, (uint16_t*)L->sz);
         e = cudaGetLastError();
     }
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -229,15 +659,18 @@ BNN_API int bnn_q4_layer_run(const bnn_q4_layer* L, const void* d_x, int64_t x_s
     Q4Params p{};
     p.g = g;
     p.w = (const uint4*)L->codes;
-    p.s = (const uint32_t*)L->scales;
-    p.z = (const uint16_t*)L->zeros;
+    p.sz = L->sz;
     p.bias = L->bias;
     p.x = (const uint16_t*)d_x;
     p.xs = x_stride;
     p.y = (uint16_t*)d_y;
     p.ys = y_stride;
     p.M = rows;
-    p.vec = aligned(d_x, 16) && (rows == 1 || x_stride % 8 == 0);
+    p.vec4 = aligned(d_x, 8) && (rows == 1 || x_stride % 4 == 0);
+    p.vec8 = aligned(d_x, 16) && (rows == 1 || x_stride % 8 == 0);
+    p.gshift = -1;
+    for (int i = 0; i < 20; ++i)
+        if (g.group == 32 << i) p.gshift = i;
     const cudaError_t e = L->type == BNN_BF16 ? q4_run<Bf16>(p, (cudaStream_t)stream) : q4_run<Fp16>(p, (cudaStream_t)stream);
     return e == cudaSuccess ? BNN_OK : cuda_error("bnn_q4_layer_run", e);
 }
@@ -249,4 +682,12 @@ BNN_API void bnn_q4_layer_destroy(bnn_q4_layer* L) {
         cudaFree(L->base);
     }
     delete L;
+}
+
+BNN_API int bnn_q4_device_error(int device, unsigned int* wait_timeouts) {
+    if (!wait_timeouts) return set_error(BNN_ERR_ARG, "NULL argument");
+    DeviceScope dev(device);
+    if (dev.err != cudaSuccess) return cuda_error("bnn_q4_device_error", dev.err);
+    const cudaError_t e = cudaMemcpyFromSymbol(wait_timeouts, g_q4_wait_timeouts, sizeof(unsigned int));
+    return e == cudaSuccess ? BNN_OK : cuda_error("bnn_q4_device_error", e);
 }

@@ -51,10 +51,19 @@ int bnn_q4_layer_create(int device, int n_in, int n_out, int group, int type,
 
 /* rows >= 0 vectors: x [rows] at a distance of x_stride elements (>= n_in)
  * -> y [rows] at y_stride (>= n_out), both in the layer's type, any
- * alignment of the type. x and y must not overlap. */
+ * alignment of the type. x and y must not overlap. Up to 16 rows the codes
+ * are multiplied exactly and a group's scale is applied to its 32-bit sum;
+ * with more rows each weight (q - z) * s is rounded to the type first (tensor
+ * memory operands), which adds half a step of the type to each product. */
 int bnn_q4_layer_run(const bnn_q4_layer *L, const void *d_x, int64_t x_stride,
                      int rows, void *d_y, int64_t y_stride, void *stream);
 void bnn_q4_layer_destroy(bnn_q4_layer *L);
+
+/* Number of CTAs of that kernel whose bounded wait (mbarriers of its TMA /
+ * tcgen05 pipeline) gave up on `device` since the library was loaded: the
+ * counterpart of bnn_device_error. Expected to stay 0; another number means
+ * that some output of a layer is not to be trusted. */
+int bnn_q4_device_error(int device, unsigned int *wait_timeouts);
 
 /* ---------------- block-scaled key/value cache ----------------
  * `pages` pages of page_tokens (16, 32, 64, 128 or 256) tokens. A token has

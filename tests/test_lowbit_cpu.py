@@ -34,7 +34,7 @@ def test_layouts_pages_and_split_under_the_sanitizers(tmp_path):
 def test_header_functions_are_exported():
     src = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "bnn_lowbit.h")).read(), flags=re.S)
     names = sorted(set(re.findall(r"\b(bnn_(?:q4|kv)_\w+)\s*\(", src)))
-    assert len(names) == 10
+    assert len(names) == 11
     L = ctypes.CDLL(bn.LIB_PATH)
     assert not [n for n in names if not hasattr(L, n)]
 
@@ -93,7 +93,7 @@ def test_linear_binding_checks_its_tensors():
         assert e.value.code == ARG
     x, y = torch.zeros(2, 65, dtype=torch.bfloat16), torch.zeros(2, 16, dtype=torch.bfloat16)
     for a, b, text in ((x.half(), y, "x: torch.float16"), (x[:, :64], y, "x: shape"), (x, y[:1], "y: shape"), (x[0], y, "dimensions"),
-                       (torch.zeros(65, 2, dtype=torch.bfloat16).T, y, "contiguous"), (np.zeros((2, 65)), y, "CUDA tensor")):
+                       (torch.zeros(65, 2, dtype=torch.bfloat16).T, y, "contiguous"), (np.zeros((2, 65)), y, "a tensor is needed")):
         with pytest.raises(bn.BnnError, match=text) as e:
             layer.run(a, b)
         assert e.value.code == ARG
@@ -200,7 +200,7 @@ def test_cache_binding_checks_its_tensors():
     for kw, text in (({"d_q": q[:, :7]}, "multiple|shape"), ({"d_out": out[:2]}, "out: shape"), ({"lengths": lengths[:2]}, "lengths: shape"),
                      ({"lse": half(3, 8)}, "lse: torch.float16"), ({"work": work[:100]}, "workspace"),
                      ({"prefix_tokens": 40}, "prefix"), ({"prefix": whole(1), "prefix_tokens": 40}, "prefix of 40"),
-                     ({"scale": float("nan")}, "finite"), ({"d_q": q[0]}, "q: a tensor")):
+                     ({"scale": float("nan")}, "finite"), ({"d_q": q[0]}, "q: .*dimensions")):
         with pytest.raises(bn.BnnError, match=text) as e:
             c.attend(**{**dict(d_q=q, lengths=lengths, table=table, d_out=out, work=work), **kw})
         assert e.value.code == ARG
