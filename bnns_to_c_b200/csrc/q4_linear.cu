@@ -67,7 +67,7 @@ struct Q4Params {
     int64_t ys;
     int M;
     int gshift;       // group = 32 << gshift, or -1
-    bool vec4, vec8;  // rows of x start 8-byte, 16-byte aligned
+    bool vec2, vec4, vec8;  // rows of x start 4-byte, 8-byte, 16-byte aligned
 };
 
 // ---------------------------------------------------------------- rows on mma.sync
@@ -244,8 +244,17 @@ cudaError_t q4_forms(const Q4Params& p, cudaStream_t st) {
 // Rounding a weight to 16 bits costs 2^-9 (bf16; fp16 2^-12) of a product, as
 // much as the rounding of the result costs; the products' errors are
 // independent, so the result stays within sqrt(2) of its own rounding.
-constexpr int kTileWarps = 13;  // 0-7 weights, then results; 8 products; 9-12 x
-constexpr int kTileStages = 4;
+// Codes to tensor memory is a chain of about 800 clocks a stage (arithmetic,
+// store, wait, hand over), so two groups of eight warps take the stages in
+// turn. One thread's products start 70 to 100 clocks apart, so below NTOK =
+// 256 (128 clocks a product) two threads take the stages in turn, with sums
+// of their own that are added at the end.
+constexpr int kGroups = 2, kWWarps = 8 * kGroups;
+constexpr int kAhead = 4;   // stages of a group whose codes are on their way
+constexpr int kXWarps = 8;  // that load x where TMA cannot
+constexpr int q4_issuers(int ntok) { return ntok == 256 ? 1 : 2; }
+constexpr int q4_tile_threads(int ntok) { return 32 * (kWWarps + q4_issuers(ntok) + kXWarps); }
+constexpr int q4_stages(int ntok) { return ntok == 256 ? 6 : 8; }
 __device__ unsigned int g_q4_wait_timeouts = 0;
 
 struct Q4TileParams {
@@ -254,12 +263,11 @@ struct Q4TileParams {
     bool tma;
 };
 
-constexpr int q4_tile_cols(int ntok) { return ntok + 32 * kTileStages <= 256 ? 256 : 512; }
+constexpr int kTileCols = 512;  // of tensor memory: NTOK sums an issuer, 32 a stage of weights
+// one CTA an SM: two would want the same columns
 constexpr int q4_tile_smem(int ntok) {
-    const int ring = kTileStages * ntok * 128;
-    // at most two CTAs an SM where tensor memory has room for two: a third
-    // would wait for its columns with the rest of its cluster waiting for it
-    return ring < 78 * 1024 ? 78 * 1024 : ring;
+    const int ring = q4_stages(ntok) * ntok * 128;
+    return ring < 116 * 1024 ? 116 * 1024 : ring;
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -270,17 +278,36 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-// into the shared memory of CTA `rank` of the cluster
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
-    uint32_t to;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+// from the shared memory of CTA `rank` of the cluster
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
+    uint32_t from;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(from));
+    return v;
+}
+
+// 16 columns of this thread's lane, over the issuers
+template <int NTOK, int ISS>
+__device__ __forceinline__ void tile_sums(float* v, uint32_t at, int nk) {
+    uint32_t r[16];
+    t5_ld16(at, r);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    if (ISS == 2 && nk > 1) {  // the second one had a stage
+        t5_ld16(at + NTOK, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] += __uint_as_float(r[i]);
+    }
 }
 
 template <class A, int NTOK, bool G32>
-__global__ void __launch_bounds__(32 * kTileWarps, NTOK == 256 ? 1 : 2)
+__global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     q4_tiles_kernel(const Q4TileParams tp, const __grid_constant__ CUtensorMap map) {
-    constexpr int S = kTileStages, STAGE = NTOK * 128, COLS = q4_tile_cols(NTOK);
+    constexpr int S = q4_stages(NTOK), STAGE = NTOK * 128;
+    constexpr int ISS = q4_issuers(NTOK), WW = kWWarps, XW = WW + ISS;  // warps: weights 0 ..; products WW ..; x XW ..
+    constexpr int WCOL = NTOK * ISS;                                     // first column of the weights
+    static_assert(WCOL + 32 * S <= kTileCols && S % kGroups == 0 && S % ISS == 0, "stages");
     extern __shared__ __align__(1024) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[3 * S + 1];
     __shared__ uint32_t tmem_s;
@@ -292,14 +319,14 @@ __global__ void __launch_bounds__(32 * kTileWarps, NTOK == 256 ? 1 : 2)
     const int share = tp.shares > 1 ? (int)cluster_rank() : 0;
     const int kb0 = (int)((int64_t)g.kb * share / tp.shares), nk = (int)((int64_t)g.kb * (share + 1) / tp.shares) - kb0;
     const uint32_t full_w = smem_addr(bars), full_x = full_w + 8 * S, empty = full_x + 8 * S, done = empty + 8 * S;
-    if (warp == 8) t5_alloc(smem_addr(&tmem_s), COLS);
+    if (warp == WW) t5_alloc(smem_addr(&tmem_s), kTileCols);
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
             bar_init(full_w + 8 * s, 8);
-            bar_init(full_x + 8 * s, tp.tma ? 1 : 4);
+            bar_init(full_x + 8 * s, 1);
             bar_init(empty + 8 * s, 1);
         }
-        bar_init(done, 1);
+        bar_init(done, ISS);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -308,80 +335,95 @@ __global__ void __launch_bounds__(32 * kTileWarps, NTOK == 256 ? 1 : 2)
     t5_after();
     const uint32_t tmem = tmem_s;
 
-    if (warp < 8) {
-        // 16 outputs a warp: lanes 32 * (warp % 4) + 16 * (warp / 4) of tensor memory
-        const int tile = min(tile0 + 2 * (warp & 3) + (warp >> 2), g.tiles - 1);
+    if (warp < WW) {
+        // 16 outputs a warp: lanes 32 * (warp % 4) + 16 * (warp / 4 % 2) of tensor memory
+        const int tile = min(tile0 + 2 * (warp & 3) + (warp >> 2 & 1), g.tiles - 1);
         const uint4* wp = p.w + ((int64_t)tile * g.kb + kb0) * 32 + lane;
         const uint2* sp = p.sz + (int64_t)tile * g.ng * 8 + (lane >> 2);
-        const uint32_t to = tmem + NTOK + ((uint32_t)(32 * (warp & 3) + 16 * (warp >> 2)) << 16);
-        constexpr int AHEAD = 2;
-        uint4 w[AHEAD];
-        uint2 sz[AHEAD][G32 ? 2 : 1];
+        const uint32_t to = tmem + WCOL + ((uint32_t)(32 * (warp & 3) + 16 * (warp >> 2 & 1)) << 16);
+        const int first = warp >> 3;
+        uint4 w[kAhead];
+        uint2 sz[kAhead][G32 ? 2 : 1];
         const auto fetch = [&](int slot, int it) {
             w[slot] = __ldcs(wp + it * 32);
 #pragma unroll
             for (int h = 0; h < (G32 ? 2 : 1); ++h) {
                 const int b = 2 * (kb0 + it) + h;
-                sz[slot][h] = __ldg(sp + min(p.gshift >= 0 ? b >> p.gshift : b / (g.group >> 5), g.ng - 1) * 8);
+                int grp = p.gshift >= 0 ? b >> p.gshift : b / (g.group >> 5);
+                if (G32) grp = min(grp, g.ng - 1);
+                sz[slot][h] = __ldg(sp + grp * 8);
             }
         };
+        const auto weights = [&](uint32_t* v, int slot) {
+            const uint32_t ww[4] = {w[slot].x, w[slot].y, w[slot].z, w[slot].w};
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-            if (a < nk) fetch(a, a);
-        for (int it0 = 0; it0 < nk; it0 += AHEAD) {
+            for (int e = 0; e < 4; ++e) {
+                const uint2 q = sz[slot][G32 ? e >> 1 : 0];
+                const uint32_t s0 = __byte_perm(q.x, 0, 0x1010), s1 = __byte_perm(q.x, 0, 0x3232);
+                uint32_t f[4];
+                A::weights(f, ww[e], __byte_perm(q.y, 0, 0x1010), __byte_perm(q.y, 0, 0x3232));
+                v[4 * e] = A::mul2(f[0], s0), v[4 * e + 1] = A::mul2(f[2], s0);
+                v[4 * e + 2] = A::mul2(f[1], s1), v[4 * e + 3] = A::mul2(f[3], s1);
+            }
+        };
+        int it = first, s = first, ph = 1;  // ph: parity of the wait for a free stage; the first round passes
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int it = it0 + a, s = it % S;
+        for (int a = 0; a < kAhead; ++a)
+            if (it + a * kGroups < nk) fetch(a, it + a * kGroups);
+        while (it < nk) {
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
                 if (it >= nk) break;
                 uint32_t v[16];
-                const uint32_t ww[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint2 q = sz[a][G32 ? e >> 1 : 0];
-                    const uint32_t s0 = __byte_perm(q.x, 0, 0x1010), s1 = __byte_perm(q.x, 0, 0x3232);
-                    uint32_t f[4];
-                    A::weights(f, ww[e], __byte_perm(q.y, 0, 0x1010), __byte_perm(q.y, 0, 0x3232));
-                    v[4 * e] = A::mul2(f[0], s0), v[4 * e + 1] = A::mul2(f[2], s0);
-                    v[4 * e + 2] = A::mul2(f[1], s1), v[4 * e + 3] = A::mul2(f[3], s1);
+                weights(v, a);
+                if (it + kAhead * kGroups < nk) fetch(a, it + kAhead * kGroups);
+                if (!__all_sync(0xffffffffu, bar_wait(empty + 8 * s, ph, &gave_up))) {
+                    it = nk;
+                    break;
                 }
-                if (it + AHEAD < nk) fetch(a, it + AHEAD);
-                if (it >= S) {
-                    if (!__all_sync(0xffffffffu, bar_wait(empty + 8 * s, (it / S - 1) & 1, &gave_up))) {
-                        it0 = nk;
-                        break;
-                    }
-                    t5_after();
-                }
+                t5_after();
                 t5_st_16x256b_x4(to + 32 * s, v);
                 t5_wait_st();
                 t5_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(full_w + 8 * s);
+                it += kGroups;
+                s += kGroups;
+                if (s >= S) s -= S, ph ^= 1;
             }
         }
-    } else if (warp == 8) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = (1u << 4) | (A::kMmaType << 7) | (A::kMmaType << 10) | ((uint32_t)(NTOK >> 3) << 17) | (8u << 24);
-            for (int it = 0; it < nk; ++it) {
-                const int s = it % S;
-                if (!bar_wait(full_x + 8 * s, (it / S) & 1, &gave_up) || !bar_wait(full_w + 8 * s, (it / S) & 1, &gave_up)) break;
-                t5_after();
+    } else if (warp < XW) {
+        // The whole warp goes through the loop, so that addresses and
+        // descriptors stay in uniform registers; one thread issues.
+        const bool leader = elect_one();
+        constexpr uint32_t idesc = (1u << 4) | (A::kMmaType << 7) | (A::kMmaType << 10) | ((uint32_t)(NTOK >> 3) << 17) | (8u << 24);
+        const int issuer = warp - WW;
+        const uint32_t d = tmem + NTOK * issuer;
+        int s = issuer, ph = 0;
+        for (int it = issuer; it < nk; it += ISS) {
+            const bool there = bar_wait(full_x + 8 * s, ph, &gave_up) && bar_wait(full_w + 8 * s, ph, &gave_up);
+            if (!__all_sync(0xffffffffu, there)) break;
+            t5_after();
+            if (leader) {
                 // K-major, 128-byte swizzle: 8 rows of 128 bytes 1024 bytes apart
                 const uint64_t b = (uint64_t)((smem_addr(ring) + s * STAGE) >> 4 & 0x3fffu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t5_mma_ts(tmem, tmem + NTOK + 32 * s + 8 * e, b + 2 * e, idesc, it > 0 || e > 0);
+                for (int e = 0; e < 4; ++e) t5_mma_ts(d, tmem + WCOL + 32 * s + 8 * e, b + 2 * e, idesc, it >= ISS || e > 0);
                 t5_commit(empty + 8 * s);
             }
-            t5_commit(done);
+            __syncwarp();
+            s += ISS;
+            if (s >= S) s -= S, ph ^= 1;
         }
+        if (leader) t5_commit(done);
     } else if (tp.tma) {
-        if (warp == 9 && lane == 0) {
-            int it = 0;
+        if (warp == XW && lane == 0) {
+            int it = 0, s = 0, ph = 1;
             for (; it < nk; ++it) {
-                const int s = it % S;
-                if (it >= S && !bar_wait(empty + 8 * s, (it / S - 1) & 1, &gave_up)) break;
+                if (!bar_wait(empty + 8 * s, ph, &gave_up)) break;
                 bar_arrive_tx(full_x + 8 * s, STAGE);
                 tma_2d(smem_addr(ring) + s * STAGE, &map, (kb0 + it) * 64, m0, full_x + 8 * s);
+                if (++s == S) s = 0, ph ^= 1;
             }
             // copies that nothing waits for any more still have to land before the CTA ends
             if (it < nk)
@@ -391,23 +433,34 @@ __global__ void __launch_bounds__(32 * kTileWarps, NTOK == 256 ? 1 : 2)
                 }
         }
     } else {
-        for (int it = 0; it < nk; ++it) {
+        // a stage a warp: 8 values of a row a lane, in pieces of what x is aligned to
+        for (int it = warp - XW; it < nk; it += kXWarps) {
             const int s = it % S;
-            if (it >= S && !__all_sync(0xffffffffu, bar_wait(empty + 8 * s, (it / S - 1) & 1, &gave_up))) break;
+            if (!__all_sync(0xffffffffu, bar_wait(empty + 8 * s, (it / S & 1) ^ 1, &gave_up))) break;
             uint8_t* st = ring + s * STAGE;
-            for (int i = tid - 32 * 9; i < NTOK * 8; i += 128) {
-                const int row = i >> 3, c = i & 7, m = m0 + row, k = (kb0 + it) * 64 + 8 * c;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (m < p.M && k < g.K) {
-                    const uint16_t* x = p.x + m * p.xs + k;
-                    if (p.vec4 && k + 8 <= g.K) {
-                        const uint2 lo = __ldg(reinterpret_cast<const uint2*>(x)), hi = __ldg(reinterpret_cast<const uint2*>(x) + 1);
-                        v = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                    } else {
-                        v = load8(x, g.K - k, false);
+            const int k0 = (kb0 + it) * 64;
+#pragma unroll 1
+            for (int i0 = lane; i0 < NTOK * 8; i0 += 32 * 4) {
+                uint4 v[4];
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const int i = i0 + 32 * a, m = m0 + (i >> 3), k = k0 + 8 * (i & 7);
+                    v[a] = make_uint4(0, 0, 0, 0);
+                    if (m < p.M && k < g.K) {
+                        const uint16_t* x = p.x + m * p.xs + k;
+                        if (p.vec2 && k + 8 <= g.K) {
+                            const uint32_t* x2 = reinterpret_cast<const uint32_t*>(x);
+                            v[a] = make_uint4(__ldg(x2), __ldg(x2 + 1), __ldg(x2 + 2), __ldg(x2 + 3));
+                        } else {
+                            v[a] = load8(x, g.K - k, false);
+                        }
                     }
                 }
-                *reinterpret_cast<uint4*>(st + row * 128 + ((c ^ (row & 7)) << 4)) = v;
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const int i = i0 + 32 * a, row = i >> 3, c = i & 7;
+                    *reinterpret_cast<uint4*>(st + row * 128 + ((c ^ (row & 7)) << 4)) = v[a];
+                }
             }
             fence_proxy_async();
             __syncwarp();
@@ -418,25 +471,25 @@ __global__ void __launch_bounds__(32 * kTileWarps, NTOK == 256 ? 1 : 2)
 
     // results
     bool ok = true;
-    if (warp < 8) {
+    if (warp < WW) {
         ok = __all_sync(0xffffffffu, bar_wait(done, 0, &gave_up));
         t5_after();
     }
     const int n = tile0 * 16 + 32 * (warp & 3) + lane;
-    constexpr int HALF = NTOK / 2;
-    const int c0 = HALF * (warp >> 2);
+    const int c0 = 16 * (warp >> 2);  // columns a warp: 16 of every 4 * WW
+    constexpr int CSTEP = 4 * WW;
     if (tp.shares == 1) {
-        if (warp < 8 && ok) {
+        if (warp < WW && ok) {
             const float bias = p.bias && n < g.N ? p.bias[n] : 0.0f;
 #pragma unroll 1
-            for (int c = c0; c < c0 + HALF; c += 16) {
-                uint32_t v[16];
-                t5_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c, v);
+            for (int c = c0; c < NTOK; c += CSTEP) {
+                float v[16];
+                tile_sums<NTOK, ISS>(v, tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c, nk);
                 if (n < g.N) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (m0 + c + i < p.M) {
-                            const typename A::T o = A::from_float(__uint_as_float(v[i]) + bias);
+                            const typename A::T o = A::from_float(v[i] + bias);
                             p.y[(m0 + c + i) * p.ys + n] = *reinterpret_cast<const uint16_t*>(&o);
                         }
                 }
@@ -444,42 +497,48 @@ __global__ void __launch_bounds__(32 * kTileWarps, NTOK == 256 ? 1 : 2)
         }
     } else {
         // Each CTA joins NTOK / shares of the rows, in the order of the
-        // shares; the others' sums come into its ring, which all are done with.
-        const int mine = NTOK / tp.shares;
-        cluster_sync();
-        if (warp < 8 && ok) {
+        // shares: every one leaves its sums in its ring, and reads its
+        // part of the others', 16 bytes at a time.
+        float* sums = reinterpret_cast<float*>(ring);  // [row of x][128 outputs]
+        if (warp < WW && ok) {
 #pragma unroll 1
-            for (int c = c0; c < c0 + HALF; c += 16) {
-                uint32_t v[16];
-                t5_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c, v);
+            for (int c = c0; c < NTOK; c += CSTEP) {
+                float v[16];
+                tile_sums<NTOK, ISS>(v, tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c, nk);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    st_cluster(smem_addr(ring) + ((share * mine + (c + i) % mine) * 128 + 32 * (warp & 3) + lane) * 4, (c + i) / mine,
-                               __uint_as_float(v[i]));
+                for (int i = 0; i < 16; ++i) sums[(c + i) * 128 + 32 * (warp & 3) + lane] = v[i];
             }
         }
         cluster_sync();
-        const float* sums = reinterpret_cast<const float*>(ring);
-        for (int i = tid; i < mine * 128; i += 32 * kTileWarps) {
-            const int m = m0 + share * mine + (i >> 7), o = tile0 * 16 + (i & 127);
-            if (m >= p.M || o >= g.N) continue;
-            float v = 0.0f;
-            for (int r = 0; r < tp.shares; ++r) v += sums[r * mine * 128 + i];
-            if (p.bias) v += p.bias[o];
-            const typename A::T out = A::from_float(v);
-            p.y[m * p.ys + o] = *reinterpret_cast<const uint16_t*>(&out);
+        const int mine = NTOK / tp.shares;
+        for (int i = tid; i < mine * 32; i += q4_tile_threads(NTOK)) {
+            const int c = share * mine + (i >> 5), o = 4 * (i & 31), m = m0 + c, out = tile0 * 16 + o;
+            if (m >= p.M || out >= g.N) continue;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int r = 0; r < tp.shares; ++r) {
+                const float4 x = ld_cluster(smem_addr(sums + c * 128 + o), r);
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+            }
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (out + k < g.N) {
+                    const typename A::T w = A::from_float(e[k] + (p.bias ? p.bias[out + k] : 0.0f));
+                    p.y[m * p.ys + out + k] = *reinterpret_cast<const uint16_t*>(&w);
+                }
         }
+        cluster_sync();  // nobody leaves while its sums are read
     }
     t5_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == WW) {
         if (gave_up) {  // products may still be running
             int alone = 0;
             bar_wait(done, 0, &alone);
             if (lane == 0) atomicAdd(&g_q4_wait_timeouts, 1u);
         }
         t5_after();
-        t5_free(tmem, COLS);
+        t5_free(tmem, kTileCols);
     }
 }
 
@@ -504,7 +563,7 @@ template <class A, int NTOK, bool G32>
 cudaError_t q4_tiles_launch(const Q4TileParams& p, const CUtensorMap& map, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cdiv64(p.q.g.tiles, 8), (unsigned)cdiv64(p.q.M, NTOK), (unsigned)p.shares);
-    cfg.blockDim = dim3(32 * kTileWarps);
+    cfg.blockDim = dim3(q4_tile_threads(NTOK));
     cfg.dynamicSmemBytes = q4_tile_smem(NTOK);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -516,9 +575,10 @@ cudaError_t q4_tiles_launch(const Q4TileParams& p, const CUtensorMap& map, cudaS
     return cudaLaunchKernelEx(&cfg, q4_tiles_kernel<A, NTOK, G32>, p, map);
 }
 
-// Rows a tile and shares of K: the pair with the least estimated clocks, of
-// the busiest SM: a 64-input block of a tile costs 2 * NTOK of products or
-// 160 of weights, a CTA 3000 to start and end, a joined one 1500 more.
+// Rows a tile and shares of K: the pair with the least estimated clocks of
+// the busiest SM: a 64-input stage costs 560 (NTOK = 256) or 300 (fewer), and
+// more where x is loaded by hand; a CTA 4000 to start and end, a joined one
+// 1500 more.
 void q4_tiles_choose(const Q4Params& p, int* ntok, int* shares) {
     double best = 1e30;
     for (int t = 32; t <= 256; t *= 2) {
@@ -526,8 +586,9 @@ void q4_tiles_choose(const Q4Params& p, int* ntok, int* shares) {
         for (int c = 1; c <= 8; c *= 2) {
             if (c > 1 && p.g.kb < 8 * c) break;
             const int64_t ctas = cdiv64(p.g.tiles, 8) * cdiv64(p.M, t) * c;
-            const double busiest = (double)cdiv64(ctas, 148), at_once = t == 256 ? 1 : 2;
-            const double clocks = busiest * ((double)p.g.kb / c) * (t < 80 ? 160 : 2 * t) + ceil(busiest / at_once) * 3000 + (c > 1 ? 1500 : 0);
+            const double stage = (t <= 128 ? 300 : 560) * (p.vec8 ? 1.0 : p.vec2 ? 1 + t / 128.0 : 1 + t / 64.0);
+            // clusters of one CTA an SM do not fill every GPC
+            const double clocks = (double)cdiv64(ctas, c == 1 ? 148 : c == 2 ? 144 : c == 4 ? 136 : 128) * ((double)p.g.kb / c * stage + 4000 + (c > 1 ? 1500 : 0));
             if (clocks < best) best = clocks, *ntok = t, *shares = c;
         }
     }
@@ -666,6 +727,7 @@ BNN_API int bnn_q4_layer_run(const bnn_q4_layer* L, const void* d_x, int64_t x_s
     p.y = (uint16_t*)d_y;
     p.ys = y_stride;
     p.M = rows;
+    p.vec2 = aligned(d_x, 4) && (rows == 1 || x_stride % 2 == 0);
     p.vec4 = aligned(d_x, 8) && (rows == 1 || x_stride % 4 == 0);
     p.vec8 = aligned(d_x, 16) && (rows == 1 || x_stride % 8 == 0);
     p.gshift = -1;
