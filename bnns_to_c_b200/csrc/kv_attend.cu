@@ -43,7 +43,8 @@ struct AttendParams {
     int rt;                  // tiles of 8 * NT rows they make
     float scale_log2;        // scale * log2(e)
     bool partial;            // leave every item to the join kernel
-    int32_t* pre;            // [n_grp + 1]: blocks before each group, for the join
+    bool second;             // runs beside the prefix's kernel
+    int2* owners;            // [group][kv head][tile]: first and last CTA of an item, for the join
     float* pacc;             // [slot][row][dp] sums of exp2(s - m) * value
     float2* pml;             // [slot][row] (m, sum of exp2(s - m))
     int stages;
@@ -105,54 +106,98 @@ __device__ __forceinline__ void lds_part(uint32_t* w, const uint8_t* base, int o
     }
 }
 
-// codes to fp16 pairs: a byte or nibble in the low mantissa bits of 1024
-// gives 1024 + it, and the subtraction leaves the code, exactly
+// Codes as fp16 pairs. A byte or a nibble put into the mantissa of a power
+// of two is that power plus the code and its offset, exactly. Keys stay so:
+// a sum of products starts at -(power + offset) * (sum of q) instead of 0.
+// (That sum is at most 18 times as large as the sum of |q code|, so it costs
+// 4 of the 24 bits of a 32-bit sum.) Values have it subtracted: their weights
+// are all positive, and the sum over thousands of tokens would grow with it.
+template <int BITS>
+constexpr float kKeyOffset = BITS == 8 ? 1024.0f + 128.0f : 64.0f + 8.0f;
 template <int LO>
-__device__ __forceinline__ uint32_t pair8(uint32_t w) {  // bytes LO and LO + 1 of w
-    return Fp16::sub2(__byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140), 0x64806480u);
+__device__ __forceinline__ uint32_t bytes2(uint32_t w) {  // bytes LO and LO + 1 of w on 1024
+    return __byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140);
 }
-__device__ __forceinline__ uint32_t pair4(uint32_t w, int nib) {  // nibbles at 4 * nib of both halves
-    return Fp16::sub2(and_or(w >> (4 * nib), 0x000f000fu, 0x64006400u), 0x64086408u);
+// the four nibble pairs of a word on 64: bits 4-7 of a half are worth 1 there
+__device__ __forceinline__ void nibbles4(uint32_t* a, uint32_t w) {
+    a[0] = and_or(w << 4, 0x00f000f0u, 0x54005400u);
+    a[1] = and_or(w, 0x00f000f0u, 0x54005400u);
+    a[2] = and_or(w >> 4, 0x00f000f0u, 0x54005400u);
+    a[3] = and_or(w >> 8, 0x00f000f0u, 0x54005400u);
 }
 
-template <int DP, int BITS>
+// Shared memory: prefix sums | row factors | start values of the score sums |
+// (m, l) of the warps | q fragments | stages, later the warps' sums.
 struct AttendSmem {
-    static constexpr int ROW = DP * BITS / 8;
-    static constexpr int CODES = kSub * ROW;  // bytes of 16 rows
-    __host__ __device__ static int stage(int ng) { return 2 * CODES + ((2 * ng * kSub * 2 + 127) & ~127); }
-    __host__ __device__ static int qfrag(int nt) { return DP / 32 * nt * 512; }
-    __host__ __device__ static int merge(int nt) { return kWarps * 8 * nt * (DP + 8) * 4; }
-    // prefix sums | row factors | row (m, l) of the warps | q fragments | stages, later the warps' sums
-    __host__ __device__ static int head(int n_grp, int nt) {
-        return (((n_grp + 1) * 4 + 127) & ~127) + 128 * ((8 * nt * 4 + 127) / 128) + kWarps * 8 * nt * 8;
-    }
-    __host__ __device__ static int bytes(int n_grp, int nt, int ng, int stages) {
-        const int ring = kWarps * stages * stage(ng), m = merge(nt);
-        return head(n_grp, nt) + qfrag(nt) + (ring > m ? ring : m);
-    }
+    int factor, start, ml, q, ring, stage, bytes;
 };
+__host__ __device__ inline AttendSmem attend_smem(const KvGeo& g, int n_grp, int nt, int stages) {
+    const int rows = 8 * nt;
+    AttendSmem s;
+    s.factor = ((n_grp + 1) * 4 + 127) & ~127;
+    s.start = s.factor + 128 * ((rows * 4 + 127) / 128);
+    s.ml = s.start + g.ngp * rows * 4;
+    s.q = s.ml + kWarps * rows * 8;
+    s.ring = s.q + g.dp / 32 * nt * 512;
+    s.stage = 2 * kSub * g.row + ((2 * g.ngp * kSub * 2 + 127) & ~127);
+    const int ring = kWarps * stages * s.stage, merge = kWarps * rows * (g.dp + 8) * 4;
+    s.bytes = s.ring + (ring > merge ? ring : merge);
+    return s;
+}
 
-template <int DP, int BITS, int NT>
+template <int N>
+__device__ __forceinline__ void load_scales(float* f, const uint16_t* at) {  // N bf16, N a power of two, aligned
+    if constexpr (N == 1) {
+        f[0] = bf16_float(at[0]);
+    } else {
+        uint32_t w[N / 2];
+        if constexpr (N == 2) w[0] = *reinterpret_cast<const uint32_t*>(at);
+        if constexpr (N == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            w[0] = v.x, w[1] = v.y;
+        }
+        if constexpr (N == 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(at);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+
+// DP: head_dim rounded up; NT: tiles of 8 query rows; BPG: 32-blocks of
+// channels that share a scale (8: all).
+template <int DP, int BITS, int NT, int BPG>
 __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) attend_kernel(const AttendParams p) {
-    using S = AttendSmem<DP, BITS>;
-    constexpr int NB = DP / 32, R = 8 * NT, ROW = S::ROW;
+    constexpr int NB = DP / 32, R = 8 * NT, ROW = DP * BITS / 8, CODES = kSub * ROW;
+    constexpr int NG = (NB + BPG - 1) / BPG, NGP = NG <= 1 ? 1 : NG <= 2 ? 2 : NG <= 4 ? 4 : 8;
     constexpr int KP = ROW / 4, VP = ROW / 8;  // a lane's bytes of a key's, a value's row
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int warp_sum[kWarps];
     const KvGeo g = p.g;
+    const AttendSmem at = attend_smem(g, p.n_grp, NT, p.stages);
     int* pre = reinterpret_cast<int*>(smem);
-    float* factor = reinterpret_cast<float*>(smem + (((p.n_grp + 1) * 4 + 127) & ~127));
-    float2* wml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(factor) + 128 * ((R * 4 + 127) / 128));
-    uint4* qf = reinterpret_cast<uint4*>(smem + S::head(p.n_grp, NT));
-    uint8_t* ring = reinterpret_cast<uint8_t*>(qf) + S::qfrag(NT);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float* factor = reinterpret_cast<float*>(smem + at.factor);
+    float* start = reinterpret_cast<float*>(smem + at.start);  // [group][row]
+    float2* wml = reinterpret_cast<float2*>(smem + at.ml);
+    uint4* qf = reinterpret_cast<uint4*>(smem + at.q);
+    uint8_t* ring = smem + at.ring;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int r = lane >> 2, j = lane & 3;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-    // blocks before each group
+    // blocks before each group, and the size of a block
+    int block = kBlock;
     {
         const int per = (p.n_grp + 32 * kWarps - 1) / (32 * kWarps), b0 = tid * per, b1 = min(p.n_grp, b0 + per);
+        bool longer = false;
+        for (int b = b0; b < b1; ++b) longer |= grp_len(p, b) > kShort;
+        if (!__syncthreads_or(longer)) block = kShort;
         int sum = 0;
-        for (int b = b0; b < b1; ++b) sum += (grp_len(p, b) + kBlock - 1) / kBlock;
+        for (int b = b0; b < b1; ++b) sum += (grp_len(p, b) + block - 1) / block;
         int inc = sum;
         for (int s = 1; s < 32; s <<= 1) {
             const int o = __shfl_up_sync(0xffffffffu, inc, s);
@@ -160,17 +205,15 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
         }
         if (lane == 31) warp_sum[warp] = inc;
         __syncthreads();
-        int at = inc - sum;
-        for (int w = 0; w < warp; ++w) at += warp_sum[w];
+        int to = inc - sum;
+        for (int w = 0; w < warp; ++w) to += warp_sum[w];
         for (int b = b0; b < b1; ++b) {
-            pre[b] = at;
-            at += (grp_len(p, b) + kBlock - 1) / kBlock;
+            pre[b] = to;
+            to += (grp_len(p, b) + block - 1) / block;
         }
-        if (b0 < p.n_grp && b1 == p.n_grp) pre[p.n_grp] = at;
+        if (b0 < p.n_grp && b1 == p.n_grp) pre[p.n_grp] = to;
         __syncthreads();
     }
-    if (blockIdx.x == 0)
-        for (int b = tid; b <= p.n_grp; b += 32 * kWarps) p.pre[b] = pre[b];
     const int items = g.heads * p.rt;  // of a group
     const int64_t units = (int64_t)pre[p.n_grp] * items;
     const int ctas = split_ctas(units, gridDim.x);
@@ -209,54 +252,103 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
         const int len = grp_len(p, grp);
         const int rows = min(R, p.rg - tile * R);
         const int64_t row0 = (int64_t)grp * p.rg + tile * R;  // row i of the item: query row (row0 + i)
+        if (blk0 == 0 && tid == 0)
+            p.owners[(int64_t)grp * items + item] = make_int2(blockIdx.x, split_owner(units, u + nb - 1, ctas));
+
+        const int sub0 = blk0 * (block / kSub), sub1 = min(blk1 * (block / kSub), (len + kSub - 1) / kSub);
+        uint8_t* mine = ring + warp * p.stages * at.stage;
+        const int32_t* row_table = p.table + (int64_t)grp * p.width;
+        // copies of one 16-token block into a stage; its page
+        const auto fetch = [&](int sub, uint8_t* to) -> int {
+            const int pos = sub * kSub, page = kv_page(g, row_table, p.width, pos);
+            if (page < 0) return -1;
+            const int tok = pos & (g.pt - 1);
+            const int64_t from = kv_row(g, page, head, tok);
+            const uint32_t dst = smem_addr(to);
+            static_assert(CODES % 512 == 0, "whole pieces for every lane");
+#pragma unroll
+            for (int c = 0; c < CODES / 512; ++c) {
+                const int o = (c * 32 + lane) * 16;
+                cp16(dst + swz<ROW>(o), p.kc + from + o);
+                cp16(dst + CODES + swz<ROW>(o), p.vc + from + o);
+            }
+            if (lane < 4 * NGP) {  // 32 * NGP bytes of scales of each
+                const int of = lane >= 2 * NGP, c = of ? lane - 2 * NGP : lane;
+                cp16(dst + 2 * CODES + lane * 16, (of ? p.vs : p.ks) + kv_scale(g, page, head, 0, tok) + 8 * c);
+            }
+            return page;
+        };
+        // the first blocks are on their way while q is made ready
+        uint32_t there = 0;  // of the stages: whether their block has a page
+        int ahead = sub0 + warp;
+        for (int s = 0; s < p.stages - 1; ++s, ahead += kWarps) {
+            if (ahead < sub1 && fetch(ahead, mine + s * at.stage) >= 0) there |= 1u << s;
+            cp_commit();
+        }
 
         // q as B fragments of fp16, each row scaled by a power of two that
         // puts its largest value in [2^9, 2^10): exact but for values
         // 2^-24 and less of the row's largest
-        for (int i = warp; i < R; i += kWarps) {
-            float x[8] = {};
-            if (i < rows && 8 * lane < g.dim) {
-                const int64_t at = row0 + i;
-                const uint4 v = load8(p.q + at / p.share * p.q_seq + (head * p.share + at % p.share) * p.q_head + 8 * lane,
-                                      g.dim - 8 * lane, p.q_vec);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        {
+            uint4 v[R / kWarps];
+#pragma unroll
+            for (int k = 0; k < R / kWarps; ++k) {
+                const int i = warp + k * kWarps;
+                const int64_t row = row0 + i;
+                v[k] = make_uint4(0, 0, 0, 0);
+                if (i < rows && 8 * lane < g.dim)
+                    v[k] = load8(p.q + row / p.share * p.q_seq + (head * p.share + row % p.share) * p.q_head + 8 * lane,
+                                 g.dim - 8 * lane, p.q_vec);
+            }
+#pragma unroll
+            for (int k = 0; k < R / kWarps; ++k) {
+                const int i = warp + k * kWarps;
+                const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                float x[8];
+                uint32_t top = 0;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const float2 f = unpack2(w[c], p.fp16);
                     x[2 * c] = f.x, x[2 * c + 1] = f.y;
+                    top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
                 }
-            }
-            uint32_t top = 0;
+                top = __reduce_max_sync(0xffffffffu, top);
+                const int e = (int)(top >> 23);  // 127 + exponent of the largest; 255: not finite
+                const int sh = top == 0 || e == 255 ? 0 : max(-126, min(126, 9 + 127 - e));
+                const float up = __int_as_float((127 + sh) << 23);
+                uint32_t h[4];
+                float sum = 0.0f;  // of the values as they are multiplied
 #pragma unroll
-            for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(x[c]) & 0x7fffffffu);
-            top = __reduce_max_sync(0xffffffffu, top);
-            const int e = (int)(top >> 23);  // 127 + exponent of the largest; 255: not finite
-            const int sh = top == 0 || e == 255 ? 0 : max(-126, min(126, 9 + 127 - e));
-            const float up = __int_as_float((127 + sh) << 23);
-            if (lane < DP / 8) {
-                uint4 v;
-                v.x = pack2(x[0] * up, x[1] * up, true);
-                v.y = pack2(x[2] * up, x[3] * up, true);
-                v.z = pack2(x[4] * up, x[5] * up, true);
-                v.w = pack2(x[6] * up, x[7] * up, true);
-                qf[((lane >> 2) * NT + (i >> 3)) * 32 + (i & 7) * 4 + (lane & 3)] = v;
+                for (int c = 0; c < 4; ++c) {
+                    h[c] = pack2(x[2 * c] * up, x[2 * c + 1] * up, true);
+                    const float2 f = unpack2(h[c], true);
+                    sum += f.x + f.y;
+                }
+                if (lane < DP / 8) qf[((lane >> 2) * NT + (i >> 3)) * 32 + (i & 7) * 4 + (lane & 3)] = make_uint4(h[0], h[1], h[2], h[3]);
+                // sums of the groups: 4 * BPG lanes each, or all
+                constexpr int LANES = NG == 1 ? 32 : 4 * BPG;
+#pragma unroll
+                for (int s = 1; s < LANES; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+                if (lane % LANES == 0 && lane / LANES < NG) start[lane / LANES * R + i] = -kKeyOffset<BITS> * sum;
+                if (lane == 0) factor[i] = p.scale_log2 * __int_as_float((127 - sh) << 23);
             }
-            if (lane == 0) factor[i] = p.scale_log2 * __int_as_float((127 - sh) << 23);
         }
         __syncthreads();
 
         float acc[NB][2][NT][4], m[NT][2], l[NT][2], f[NT][2];
-        uint32_t ev[NB];  // exponent field (bf16 bits) of the unit that acc is in, per 32 channels
+        // sums of values are kept in units of a power of two for each scale
+        // group, near its largest scale so far: bf16 scales reach beyond fp16
+        float inv[NG];  // 1 / unit
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            ev[b] = 4u << 7;
+        for (int q = 0; q < NG; ++q) inv[q] = __uint_as_float(250u << 23);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[b][h][t][e] = 0.0f;
-        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -265,45 +357,11 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                 f[t][e] = factor[t * 8 + 2 * j + e];
             }
 
-        const int sub0 = blk0 * (kBlock / kSub), sub1 = min(blk1 * (kBlock / kSub), (len + kSub - 1) / kSub);
-        const int stage_bytes = S::stage(g.ng);
-        uint8_t* mine = ring + warp * p.stages * stage_bytes;
-        const int32_t* row_table = p.table + (int64_t)grp * p.width;
-        const int bpg = g.ng == 1 ? 8 : g.group / 32;  // 32-blocks a scale covers, a power of two
-
-        // copies of one 16-token block into a stage; its page
-        const auto fetch = [&](int sub, uint8_t* to) -> int {
-            const int pos = sub * kSub, page = kv_page(g, row_table, p.width, pos);
-            if (page < 0) return -1;
-            const int tok = pos & (g.pt - 1);
-            const int64_t at = kv_row(g, page, head, tok);
-            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
-            static_assert(S::CODES % 512 == 0, "whole pieces for every lane");
-#pragma unroll
-            for (int c = 0; c < S::CODES / 512; ++c) {
-                const int o = (c * 32 + lane) * 16;
-                cp16(dst + swz<ROW>(o), p.kc + at + o);
-                cp16(dst + S::CODES + swz<ROW>(o), p.vc + at + o);
-            }
-            if (lane < 4 * g.ng) {
-                const int of = lane >= 2 * g.ng, c = of ? lane - 2 * g.ng : lane;
-                const uint16_t* src = (of ? p.vs : p.ks) + kv_scale(g, page, head, c >> 1, tok) + 8 * (c & 1);
-                cp16(dst + 2 * S::CODES + (of * g.ng * kSub + (c >> 1) * kSub + 8 * (c & 1)) * 2, src);
-            }
-            return page;
-        };
-        // pages of the blocks in flight, one bit each: there or not
-        uint32_t there = 0;
-        int ahead = sub0 + warp;
-        for (int s = 0; s < p.stages - 1; ++s, ahead += kWarps) {
-            if (ahead < sub1 && fetch(ahead, mine + s * stage_bytes) >= 0) there |= 1u << s;
-            cp_commit();
-        }
         int st = 0, st_in = p.stages - 1;
         for (int sub = sub0 + warp; sub < sub1; sub += kWarps) {
             // the stage read a round ago is free: all lanes passed the barrier below
             there &= ~(1u << st_in);
-            if (ahead < sub1 && fetch(ahead, mine + st_in * stage_bytes) >= 0) there |= 1u << st_in;
+            if (ahead < sub1 && fetch(ahead, mine + st_in * at.stage) >= 0) there |= 1u << st_in;
             ahead += kWarps;
             cp_commit();
             st_in = st_in + 1 == p.stages ? 0 : st_in + 1;
@@ -315,56 +373,64 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                 default: cp_wait<5>(); break;
             }
             __syncwarp();
-            const uint8_t* kb = mine + st * stage_bytes;
+            const uint8_t* kb = mine + st * at.stage;
             const bool page_there = there >> st & 1u;
             st = st + 1 == p.stages ? 0 : st + 1;
             if (page_there) {
-                const uint8_t* vb = kb + S::CODES;
-                const uint16_t* ksc = reinterpret_cast<const uint16_t*>(kb + 2 * S::CODES);
-                const uint16_t* vsc = ksc + g.ng * kSub;
+                const uint8_t* vb = kb + CODES;
+                const uint16_t* sc = reinterpret_cast<const uint16_t*>(kb + 2 * CODES);  // [keys, values][token][NGP]
                 // scores: tokens r and r + 8 in rows, query rows in columns
-                float s[NT][4] = {};
+                float s[NT][4];
                 {
                     uint32_t k0[KP / 4], k1[KP / 4];
                     lds_part<ROW, KP>(k0, kb, r * ROW + j * KP);
                     lds_part<ROW, KP>(k1, kb, (r + 8) * ROW + j * KP);
-                    float c[NT][4] = {};
+                    float s0[NGP], s1[NGP];
+                    load_scales<NGP>(s0, sc + r * NGP);
+                    load_scales<NGP>(s1, sc + (r + 8) * NGP);
+                    float c[NT][4];
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
+                        if (b % BPG == 0)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                const float2 z = *reinterpret_cast<const float2*>(start + b / BPG * R + t * 8 + 2 * j);
+                                c[t][0] = c[t][2] = z.x, c[t][1] = c[t][3] = z.y;
+                            }
                         uint4 qv[NT];
 #pragma unroll
                         for (int t = 0; t < NT; ++t) qv[t] = qf[(b * NT + t) * 32 + lane];
+                        uint32_t n0[4], n1[4];
+                        if constexpr (BITS == 4) nibbles4(n0, k0[b]), nibbles4(n1, k1[b]);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             uint32_t a[4];
                             if constexpr (BITS == 8) {
-                                a[0] = pair8<0>(k0[2 * b + h]), a[1] = pair8<0>(k1[2 * b + h]);
-                                a[2] = pair8<2>(k0[2 * b + h]), a[3] = pair8<2>(k1[2 * b + h]);
+                                a[0] = bytes2<0>(k0[2 * b + h]), a[1] = bytes2<0>(k1[2 * b + h]);
+                                a[2] = bytes2<2>(k0[2 * b + h]), a[3] = bytes2<2>(k1[2 * b + h]);
                             } else {
-                                a[0] = pair4(k0[b], 2 * h), a[1] = pair4(k1[b], 2 * h);
-                                a[2] = pair4(k0[b], 2 * h + 1), a[3] = pair4(k1[b], 2 * h + 1);
+                                a[0] = n0[2 * h], a[1] = n1[2 * h], a[2] = n0[2 * h + 1], a[3] = n1[2 * h + 1];
                             }
 #pragma unroll
                             for (int t = 0; t < NT; ++t) Fp16::mma(c[t], a, h ? qv[t].z : qv[t].x, h ? qv[t].w : qv[t].y);
                         }
-                        if (b == NB - 1 || ((b + 1) & (bpg - 1)) == 0) {
-                            // the group's scale, on its sum of products
-                            const int grp_at = min(b / bpg, g.ng - 1) * kSub;
-                            const float s0 = bf16_float(ksc[grp_at + r]), s1 = bf16_float(ksc[grp_at + r + 8]);
+                        if (b == NB - 1 || b % BPG == BPG - 1) {  // the group's scale, on its sum of products
+                            const float g0 = s0[b / BPG], g1 = s1[b / BPG];
 #pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                s[t][0] = fmaf(s0, c[t][0], s[t][0]), s[t][1] = fmaf(s0, c[t][1], s[t][1]);
-                                s[t][2] = fmaf(s1, c[t][2], s[t][2]), s[t][3] = fmaf(s1, c[t][3], s[t][3]);
-                                c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0.0f;
-                            }
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[t][e] = b < BPG ? (e < 2 ? g0 : g1) * c[t][e] : fmaf(e < 2 ? g0 : g1, c[t][e], s[t][e]);
                         }
                     }
                 }
                 const bool in0 = sub * kSub + r < len, in1 = sub * kSub + r + 8 < len;
-                // The running maximum is one that was the maximum when it was
-                // last raised: it is raised when a score is 2^8 above it, so
-                // most blocks need no reduction over the lanes. exp2 of at
-                // most 8 stays in fp16 and the ratio to the sum is the same.
+                float v0[NGP], v1[NGP];
+                load_scales<NGP>(v0, sc + (kSub + r) * NGP);
+                load_scales<NGP>(v1, sc + (kSub + r + 8) * NGP);
+                // The running maximum and the units are lazy: raised when a
+                // score is 2^8 above the maximum, or a scale 2^6 above its
+                // unit, so most blocks need no reduction over the lanes.
+                // weight * scale / unit stays below 2^14, in fp16.
                 bool raise = false;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -374,6 +440,11 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                         s[t][2 + e] = in1 ? s[t][2 + e] * f[t][e] : -INFINITY;
                         raise |= fmaxf(s[t][e], s[t][2 + e]) > m[t][e] + 8.0f;
                     }
+#pragma unroll
+                for (int q = 0; q < NG; ++q) {
+                    v0[q] = in0 ? v0[q] : 0.0f, v1[q] = in1 ? v1[q] : 0.0f;
+                    raise |= fmaxf(v0[q], v1[q]) * inv[q] > 64.0f;
+                }
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
@@ -392,6 +463,23 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) acc[b][h][t][e] *= corr, acc[b][h][t][2 + e] *= corr;
                         }
+#pragma unroll
+                    for (int q = 0; q < NG; ++q) {
+                        const uint32_t u0 = __float_as_uint(v0[q]), u1 = __float_as_uint(v1[q]);  // NaN: bits above infinity's
+                        const uint32_t big = __reduce_max_sync(0xffffffffu, max(u0 < 0x7f800000u ? u0 : 0u, u1 < 0x7f800000u ? u1 : 0u));
+                        const uint32_t unit = (254u << 23) - __float_as_uint(inv[q]), now = max(unit, min(big & 0x7f800000u, 253u << 23));
+                        const int down = (int)((now - unit) >> 23);
+                        const float corr = down > 126 ? 0.0f : __int_as_float((127 - down) << 23);
+                        inv[q] = __uint_as_float((254u << 23) - now);
+#pragma unroll
+                        for (int b = q * BPG; b < (q + 1) * BPG && b < NB; ++b)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) acc[b][h][t][e] *= corr;
+                    }
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -403,41 +491,22 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                         l[t][e] += s[t][e] + s[t][2 + e];
                     }
                 // output: channels in rows, query rows in columns, the tokens
-                // summed. The values' scales go with the weights: weight *
-                // scale in units of a power of two near the largest scale so
-                // far (bf16 scales reach beyond fp16), rounded once to fp16.
-                // Error: 2^-12 of each term, independent of one another, next
-                // to a result of 8 or 11 bits.
+                // summed. The values' scales go with the weights, rounded
+                // once to fp16: 2^-12 of each term, independent of one
+                // another, next to a result of 8 or 11 bits.
                 uint32_t vw[4][(VP + 3) / 4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) lds_part<ROW, VP>(vw[t], vb, (2 * j + (t & 1) + 8 * (t >> 1)) * ROW + r * VP);
-                uint32_t e_new = 0;
                 uint32_t wb[NT][2];
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    if ((b & (bpg - 1)) == 0 || b == 0) {
-                        const int grp_at = min(b / bpg, g.ng - 1) * kSub;
-                        const uint32_t u0 = in0 ? vsc[grp_at + r] : 0u, u1 = in1 ? vsc[grp_at + r + 8] : 0u;
-                        const uint32_t big = max(u0 < 0x7f80u ? u0 : 0u, u1 < 0x7f80u ? u1 : 0u);
-                        e_new = max(ev[b], min(__reduce_max_sync(0xffffffffu, big) & 0x7f80u, 253u << 7));
-                        const float inv = __uint_as_float((254u << 23) - (e_new << 16));
-                        const float w0 = bf16_float((uint16_t)u0) * inv, w1 = bf16_float((uint16_t)u1) * inv;
+                    if (b % BPG == 0) {
+                        const float w0 = v0[b / BPG] * inv[b / BPG], w1 = v1[b / BPG] * inv[b / BPG];
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
                             wb[t][0] = movm_t(pack2(s[t][0] * w0, s[t][1] * w0, true));
                             wb[t][1] = movm_t(pack2(s[t][2] * w1, s[t][3] * w1, true));
                         }
-                    }
-                    if (e_new != ev[b]) {
-                        const int down = (int)((e_new - ev[b]) >> 7);
-                        const float corr = down > 126 ? 0.0f : __int_as_float((127 - down) << 23);
-                        ev[b] = e_new;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[b][h][t][e] *= corr;
                     }
                     uint32_t a[2][4];
                     if constexpr (BITS == 8) {
@@ -445,15 +514,16 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                         for (int x = 0; x < 2; ++x) {  // tokens 2j, 2j + 1; then 8 behind
                             const uint32_t lo = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x5140);
                             const uint32_t hi = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x7362);
-                            a[0][2 * x] = pair8<0>(lo), a[0][2 * x + 1] = pair8<2>(lo);
-                            a[1][2 * x] = pair8<0>(hi), a[1][2 * x + 1] = pair8<2>(hi);
+                            a[0][2 * x] = Fp16::sub2(bytes2<0>(lo), 0x64806480u), a[0][2 * x + 1] = Fp16::sub2(bytes2<2>(lo), 0x64806480u);
+                            a[1][2 * x] = Fp16::sub2(bytes2<0>(hi), 0x64806480u), a[1][2 * x + 1] = Fp16::sub2(bytes2<2>(hi), 0x64806480u);
                         }
                     } else {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const uint32_t v = __byte_perm(vw[2 * x][b >> 1], vw[2 * x + 1][b >> 1], b & 1 ? 0x7632 : 0x5410);
-                            a[0][2 * x] = pair4(v, 0), a[0][2 * x + 1] = pair4(v, 1);
-                            a[1][2 * x] = pair4(v, 2), a[1][2 * x + 1] = pair4(v, 3);
+                            uint32_t n[4];
+                            nibbles4(n, __byte_perm(vw[2 * x][b >> 1], vw[2 * x + 1][b >> 1], b & 1 ? 0x7632 : 0x5410));
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) a[h >> 1][2 * x + (h & 1)] = Fp16::sub2(n[h], 0x54805480u);  // 72
                         }
                     }
 #pragma unroll
@@ -482,7 +552,7 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                 if (r == 0) wml[warp * R + row] = make_float2(m[t][e], l[t][e]);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const float unit = __uint_as_float(ev[b] << 16);
+                    const float unit = __uint_as_float((254u << 23) - __float_as_uint(inv[b / BPG]));
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                         *reinterpret_cast<float2*>(sums + (warp * R + row) * (DP + 8) + 32 * b + 4 * r + 2 * h) =
@@ -504,8 +574,8 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                 c[w] = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
                 sum += ml.x == -INFINITY ? 0.0f : c[w] * ml.y;
             }
-            const int64_t at = row0 + i, seq = at / p.share;
-            const int qh = head * p.share + (int)(at % p.share);
+            const int64_t row = row0 + i, seq = row / p.share;
+            const int qh = head * p.share + (int)(row % p.share);
             const float norm = direct ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
             for (int d = 2 * lane; d < DP; d += 64) {
                 float2 v = make_float2(0.0f, 0.0f);
@@ -534,95 +604,108 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
         __syncthreads();
         u += blk1 - blk0;
     }
+    // The kernel for the sequences' own positions runs beside the prefix's,
+    // and ends behind it, so that the join follows both.
+    if (p.second) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // ---------------------------------------------------------------- join
 // One CTA a query row: the parts of its items, of its own positions (and of
 // the prefix), each a sum with its maximum, joined with their weights.
 struct JoinSide {
-    const int32_t* pre;  // nullptr: this side has nothing
+    const int2* owners;  // nullptr: this side has nothing
     const float* pacc;
     const float2* pml;
-    int n_grp, rg, rt, R, ctas;
+    const int32_t* lengths;
+    int length;
+    int rg, rt, R, ctas;
 };
 struct JoinParams {
     JoinSide side[2];  // own positions, prefix
     int heads, share, dim, dp;
+    int width[2];  // pages of the tables
     uint16_t* out;
     int64_t o_seq, o_head;
     float* lse;
     bool fp16, partial;
 };
 
-__global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
-    __shared__ float sums[4][256];
-    __shared__ float2 wml[4];
+constexpr int kJoinWarps = 4;
+
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams p) {
+    __shared__ __align__(16) float sums[kJoinWarps][256];
+    __shared__ float2 wml[kJoinWarps];
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int q_heads = p.heads * p.share;
-    const int64_t seq = blockIdx.x / q_heads;
-    const int qh = blockIdx.x % q_heads, head = qh / p.share;
+    const int seq = blockIdx.x / q_heads, qh = blockIdx.x % q_heads, head = qh / p.share;
+    const int row = seq * p.share + qh % p.share;  // of the kv head's query rows
     float m = -INFINITY, l = 0.0f, acc[8] = {};
     for (int w = 0; w < 2; ++w) {
-        const JoinSide s = p.side[w];
-        if (!s.pre) continue;
-        // this row in that side's items
-        const int64_t row = seq * p.share + qh % p.share, grp = row / s.rg;
-        const int in = (int)(row % s.rg), tile = in / s.R, i = in % s.R;
-        const int items = p.heads * s.rt, item = head * s.rt + tile;
-        const int nb = s.pre[grp + 1] - s.pre[grp];
-        if (nb == 0) continue;
-        const int64_t units = (int64_t)s.pre[s.n_grp] * items, u0 = (int64_t)s.pre[grp] * items + (int64_t)item * nb;
-        const int n = split_ctas(units, s.ctas), c0 = split_owner(units, u0, n), c1 = split_owner(units, u0 + nb - 1, n);
-        if (c0 == c1 && !p.partial) continue;
-        for (int c = c0 + warp; c <= c1; c += 4) {
-            const int64_t slot = c0 == c1 ? 2 * (int64_t)s.ctas + grp * items + item : 2 * (int64_t)c + (c == c0);
-            const float2 ml = s.pml[slot * s.R + i];
-            if (ml.x == -INFINITY) continue;  // this part saw nothing
-            const float top = fmaxf(m, ml.x), a = m == -INFINITY ? 0.0f : exp2_fast(m - top), b = exp2_fast(ml.x - top);
+        const JoinSide& s = p.side[w];
+        if (!s.owners) continue;
+        // the item that the row is in, and the CTAs that have its parts
+        const int grp = row / s.rg, in = row % s.rg, i = in % s.R, item = (grp * p.heads + head) * s.rt + in / s.R;
+        const int2 own = (s.lengths ? s.lengths[grp] : s.length) > 0 && p.width[w] > 0 ? s.owners[item] : make_int2(0, -1);
+        if (!p.partial && own.x >= own.y) return;  // the attention kernel has finished this row itself
+        // a lane reads the maximum and sum of a part, then all read its values
+        for (int c = own.x + warp; c <= own.y; c += 32 * kJoinWarps) {
+            const int mine = c + lane * kJoinWarps;
+            const int64_t slot = own.x == own.y ? 2 * (int64_t)s.ctas + item : 2 * (int64_t)mine + (mine == own.x);
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (mine <= own.y) ml = s.pml[slot * s.R + i];
+            float top = ml.x;
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, m);
+            const float a = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+            const float b = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);  // 0: this part saw nothing
+            float sum = ml.x == -INFINITY ? 0.0f : b * ml.y;
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             m = top;
-            l = l * a + ml.y * b;
-            const float* x = s.pacc + (slot * s.R + i) * p.dp;
+            l = l * a + sum;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k * 32 < p.dp) acc[k] = acc[k] * a + b * x[k * 32 + lane];
+            for (int k = 0; k < 8; ++k) acc[k] *= a;
+            // (a part that saw nothing has left zeros)
+            const int parts = min(32, (own.y - c) / kJoinWarps + 1);
+#pragma unroll 8
+            for (int q = 0; q < parts; ++q) {
+                const float f = __shfl_sync(0xffffffffu, b, q);
+                const int64_t from = __shfl_sync(0xffffffffu, slot, q);
+                const float* x = s.pacc + (from * s.R + i) * p.dp + 4 * lane;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (128 * k + 4 * lane < p.dp) {
+                        const float4 v = *reinterpret_cast<const float4*>(x + 128 * k);
+                        acc[4 * k] = fmaf(f, v.x, acc[4 * k]), acc[4 * k + 1] = fmaf(f, v.y, acc[4 * k + 1]);
+                        acc[4 * k + 2] = fmaf(f, v.z, acc[4 * k + 2]), acc[4 * k + 3] = fmaf(f, v.w, acc[4 * k + 3]);
+                    }
+            }
         }
-        if (c0 == c1) continue;
-    }
-    // a row that the attention kernel has finished itself
-    if (!p.partial) {
-        const JoinSide s = p.side[0];
-        const int64_t row = seq * p.share + qh % p.share, grp = row / s.rg;
-        const int tile = (int)(row % s.rg) / s.R, items = p.heads * s.rt, item = head * s.rt + tile;
-        const int nb = s.pre[grp + 1] - s.pre[grp];
-        if (nb == 0) return;
-        const int64_t units = (int64_t)s.pre[s.n_grp] * items, u0 = (int64_t)s.pre[grp] * items + (int64_t)item * nb;
-        const int n = split_ctas(units, s.ctas);
-        if (split_owner(units, u0, n) == split_owner(units, u0 + nb - 1, n)) return;
     }
     if (lane == 0) wml[warp] = make_float2(m, l);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (k * 32 < p.dp) sums[warp][k * 32 + lane] = acc[k];
+    for (int k = 0; k < 2; ++k)
+        if (128 * k + 4 * lane < p.dp)
+            *reinterpret_cast<float4*>(&sums[warp][128 * k + 4 * lane]) = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
     __syncthreads();
-    float top = -INFINITY, c[4], sum = 0.0f;
+    float top = -INFINITY, c[kJoinWarps], sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, wml[w].x);
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, wml[w].x);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kJoinWarps; ++w) {
         c[w] = wml[w].x == -INFINITY ? 0.0f : exp2_fast(wml[w].x - top);
         sum += wml[w].x == -INFINITY ? 0.0f : c[w] * wml[w].y;
     }
     const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int d = threadIdx.x; d < p.dim; d += 128) {
+    for (int d = threadIdx.x; d < p.dim; d += 32 * kJoinWarps) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < kJoinWarps; ++w)
             if (c[w] != 0.0f) v = fmaf(c[w], sums[w][d], v);
         p.out[seq * p.o_seq + qh * p.o_head + d] = (uint16_t)pack2(v * norm, 0.0f, p.fp16);
     }
     if (p.lse && threadIdx.x == 0)
-        p.lse[seq * q_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+        p.lse[(int64_t)seq * q_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
 // ---------------------------------------------------------------- host
@@ -631,8 +714,8 @@ __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
 struct Plan {
     int n_grp, rg, nt, rt, ctas, stages, smem;
     int64_t slots;
-    size_t pre_bytes, acc_bytes, ml_bytes;
-    size_t bytes() const { return pre_bytes + acc_bytes + ml_bytes; }
+    size_t own_bytes, acc_bytes, ml_bytes;
+    size_t bytes() const { return own_bytes + acc_bytes + ml_bytes; }
 };
 
 Plan attend_plan(const bnn_kv_cache* c, int n_grp, int rg, bool partial) {
@@ -645,66 +728,60 @@ Plan attend_plan(const bnn_kv_cache* c, int n_grp, int rg, bool partial) {
     s.rt = (int)cdiv64(rg, 8 * s.nt);
     const int per_sm = g.dp <= 128 && s.nt == 1 ? 3 : 2;
     s.ctas = (c->sms > 0 ? c->sms : 148) * per_sm;
-    const int R = 8 * s.nt, row = g.row;
-    const int stage = 2 * kSub * row + ((2 * g.ng * kSub * 2 + 127) & ~127);
-    const int head = (((n_grp + 1) * 4 + 127) & ~127) + 128 * ((R * 4 + 127) / 128) + kWarps * R * 8 + g.dp / 32 * s.nt * 512;
-    const int merge = kWarps * R * (g.dp + 8) * 4;
-    const int budget = 224 * 1024 / per_sm - 1024;
-    int n = (budget - head) / (kWarps * stage);
-    s.stages = n < 2 ? 2 : n > 6 ? 6 : n;
-    const int ring = kWarps * s.stages * stage;
-    s.smem = head + (ring > merge ? ring : merge);
+    const int R = 8 * s.nt;
+    s.stages = 2;
+    while (s.stages < 6 && attend_smem(g, n_grp, s.nt, s.stages + 1).bytes <= 224 * 1024 / per_sm - 1024) ++s.stages;
+    s.smem = attend_smem(g, n_grp, s.nt, s.stages).bytes;
     s.slots = 2 * (int64_t)s.ctas + (partial ? (int64_t)n_grp * g.heads * s.rt : 0);
     const auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-    s.pre_bytes = up((size_t)(n_grp + 1) * 4);
+    s.own_bytes = up((size_t)n_grp * g.heads * s.rt * 8);
     s.acc_bytes = up((size_t)s.slots * R * g.dp * 4);
     s.ml_bytes = up((size_t)s.slots * R * 8);
     return s;
 }
 
-template <int DP, int BITS, int NT>
-cudaError_t attend_launch(const AttendParams& p, const Plan& s, cudaStream_t st) {
-    attend_kernel<DP, BITS, NT><<<s.ctas, 32 * kWarps, s.smem, st>>>(p);
-    return cudaGetLastError();
-}
-template <int DP, int BITS>
-cudaError_t attend_rows(const AttendParams& p, const Plan& s, cudaStream_t st) {
-    if (s.nt == 1) return attend_launch<DP, BITS, 1>(p, s, st);
-    if (s.nt == 2) return attend_launch<DP, BITS, 2>(p, s, st);
-    if constexpr (DP <= 128) return attend_launch<DP, BITS, 4>(p, s, st);
+// f(kernel) of a cache's kernel for nt row tiles
+template <int DP, int BITS, int BPG, class F>
+cudaError_t attend_rows(int nt, F&& f) {
+    if (nt == 1) return f(attend_kernel<DP, BITS, 1, BPG>);
+    if (nt == 2) return f(attend_kernel<DP, BITS, 2, BPG>);
+    if constexpr (DP <= 128) return f(attend_kernel<DP, BITS, 4, BPG>);
     return cudaErrorInvalidValue;
 }
-template <int BITS>
-cudaError_t attend_dim(const AttendParams& p, const Plan& s, cudaStream_t st) {
-    switch (p.g.dp) {
-        case 64: return attend_rows<64, BITS>(p, s, st);
-        case 128: return attend_rows<128, BITS>(p, s, st);
-        case 192: return attend_rows<192, BITS>(p, s, st);
-        default: return attend_rows<256, BITS>(p, s, st);
+template <int DP, int BITS, class F>
+cudaError_t attend_group(const KvGeo& g, int nt, F&& f) {
+    if (g.ng == 1) return attend_rows<DP, BITS, 8>(nt, f);
+    if (g.group == 32) return attend_rows<DP, BITS, 1>(nt, f);
+    if constexpr (DP > 64)
+        if (g.group == 64) return attend_rows<DP, BITS, 2>(nt, f);
+    if constexpr (DP > 128)
+        if (g.group == 128) return attend_rows<DP, BITS, 4>(nt, f);
+    return cudaErrorInvalidValue;
+}
+template <int BITS, class F>
+cudaError_t attend_dim(const KvGeo& g, int nt, F&& f) {
+    switch (g.dp) {
+        case 64: return attend_group<64, BITS>(g, nt, f);
+        case 128: return attend_group<128, BITS>(g, nt, f);
+        case 192: return attend_group<192, BITS>(g, nt, f);
+        default: return attend_group<256, BITS>(g, nt, f);
     }
 }
-cudaError_t attend_one(const AttendParams& p, const Plan& s, cudaStream_t st) {
-    return p.g.bits == 8 ? attend_dim<8>(p, s, st) : attend_dim<4>(p, s, st);
+template <class F>
+cudaError_t attend_any(const KvGeo& g, int nt, F&& f) {
+    return g.bits == 8 ? attend_dim<8>(g, nt, f) : attend_dim<4>(g, nt, f);
 }
 
-// the kernels of a cache may use all of an SM's shared memory: set once, when the cache is made
-template <int DP, int BITS>
-cudaError_t attend_setup_rows() {
-    constexpr int all = 226 * 1024;
-    cudaError_t e = cudaFuncSetAttribute(attend_kernel<DP, BITS, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, all);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<DP, BITS, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, all);
-    if constexpr (DP <= 128)
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<DP, BITS, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, all);
-    return e;
-}
-template <int BITS>
-cudaError_t attend_setup_dim(int dp) {
-    switch (dp) {
-        case 64: return attend_setup_rows<64, BITS>();
-        case 128: return attend_setup_rows<128, BITS>();
-        case 192: return attend_setup_rows<192, BITS>();
-        default: return attend_setup_rows<256, BITS>();
-    }
+cudaLaunchConfig_t launch_config(dim3 grid, int threads, int smem, cudaStream_t st, cudaLaunchAttribute* beside) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    beside->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    beside->val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = beside;
+    return cfg;
 }
 
 constexpr int kMaxSeqs = 16384;
@@ -719,7 +796,13 @@ int attend_check(const bnn_kv_cache* c, int n_seqs, int q_heads, int prefix_toke
 
 }  // namespace
 
-cudaError_t attend_setup(const KvGeo& g) { return g.bits == 8 ? attend_setup_dim<8>(g.dp) : attend_setup_dim<4>(g.dp); }
+cudaError_t attend_setup(const KvGeo& g) {
+    // the kernels may use all of an SM's shared memory
+    cudaError_t e = cudaSuccess;
+    for (int nt = 1; nt <= (g.dp <= 128 ? 4 : 2) && e == cudaSuccess; nt *= 2)
+        e = attend_any(g, nt, [](auto k) { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024); });
+    return e;
+}
 
 }  // namespace lowbit
 }  // namespace bnn
@@ -796,22 +879,23 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
         p.length = side ? prefix_tokens : 0;
         p.table = side ? d_prefix : d_table;
         p.width = side ? prefix_pages : table_pages;
-        p.pre = (int32_t*)work;
-        p.pacc = (float*)(work + s.pre_bytes);
-        p.pml = (float2*)(work + s.pre_bytes + s.acc_bytes);
+        p.owners = (int2*)work;
+        p.pacc = (float*)(work + s.own_bytes);
+        p.pml = (float2*)(work + s.own_bytes + s.acc_bytes);
         work += s.bytes();
-        const cudaError_t e = attend_one(p, s, st);
+        p.second = prefix && side == 0;
+        cudaLaunchAttribute beside[1];
+        cudaLaunchConfig_t cfg = launch_config(dim3(s.ctas), 32 * kWarps, s.smem, st, beside);
+        cfg.numAttrs = p.second;
+        const cudaError_t e = attend_any(g, s.nt, [&](auto k) { return cudaLaunchKernelEx(&cfg, k, (const AttendParams)p); });
         if (e != cudaSuccess) return cuda_error("bnn_kv_attend", e);
-        jp.side[side] = JoinSide{p.pre, p.pacc, p.pml, s.n_grp, s.rg, s.rt, 8 * s.nt, s.ctas};
+        jp.side[side] = JoinSide{p.owners, p.pacc, p.pml, p.lengths, p.length, s.rg, s.rt, 8 * s.nt, s.ctas};
+        jp.width[side] = p.width;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((int64_t)n_seqs * q_heads));
-    cfg.blockDim = dim3(128);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
+    // no sequence can be longer than a block: none is cut
+    if (!prefix && (int64_t)table_pages * g.pt <= kShort) return BNN_OK;
+    cudaLaunchAttribute beside[1];
+    cudaLaunchConfig_t cfg = launch_config(dim3((unsigned)((int64_t)n_seqs * q_heads)), 32 * kJoinWarps, 0, st, beside);
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel, (const JoinParams)jp);
     return e == cudaSuccess ? BNN_OK : cuda_error("bnn_kv_attend", e);

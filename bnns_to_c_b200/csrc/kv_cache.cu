@@ -18,133 +18,253 @@ struct KvRows {
     int64_t token[2], head[2];
     int n_tokens, n_seqs, width;
     const int32_t *table, *start, *off;
-    bool vec[2], fp16;
+    bool vec[2];
+    int tpc;              // tokens a CTA
+    uint32_t head_magic;  // unit / heads = unit * head_magic >> 32 (heads > 1)
 };
 
-// page and place in it of row t; false: the row has none
-__device__ __forceinline__ bool kv_place(const KvRows& p, int t, int& page, int& tok) {
-    const int b = p.off ? kv_seq(p.off, p.n_seqs, t) : t;
-    if (b < 0) return false;
-    const int64_t pos = (int64_t)p.start[b] + (p.off ? (int64_t)t - p.off[b] : 0);
-    if (pos < 0 || pos > 0x7fffffff) return false;
-    page = kv_page(p.g, p.table + (int64_t)b * p.width, p.width, (int)pos);
-    tok = (int)pos & (p.g.pt - 1);
-    return page >= 0;
+constexpr int kRowThreads = 256, kMaxTpc = 32;
+
+// pages and places of the CTA's tokens, a warp each; page -1: none
+__device__ __forceinline__ void kv_places(const KvRows& p, int2* place) {
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < p.tpc; i += kRowThreads / 32) {
+        const int t = blockIdx.x * p.tpc + i;
+        int2 at = make_int2(-1, 0);
+        if (t < p.n_tokens) {
+            const int b = p.off ? kv_seq(p.off, p.n_seqs, t,
+                                         [&](int lo, int step, int len) {
+                                             return __popc(__ballot_sync(0xffffffffu, lane * step < len && p.off[lo + lane * step] <= t));
+                                         })
+                                : t;
+            if (b >= 0) {
+                const int64_t pos = (int64_t)p.start[b] + (p.off ? (int64_t)t - p.off[b] : 0);
+                if (pos >= 0 && pos <= 0x7fffffff) {
+                    at.x = kv_page(p.g, p.table + (int64_t)b * p.width, p.width, (int)pos);
+                    at.y = (int)pos & (p.g.pt - 1);
+                }
+            }
+        }
+        if (lane == 0) place[i] = at;
+    }
+    __syncthreads();
 }
 
-// Both kernels: W = dp / 8 neighbouring lanes (32 for dp = 192) have one
-// head of one token's keys or values, 8 numbers each: 16 bytes of the
-// caller's row. Bound by those rows' bytes.
-//
-// The codes. x has at most 11 significant bits (24-bit sums are not at work
-// here) and the scale 8, so x / scale is at least 2^-12 away from a border
-// k + 1/2 that it does not hit exactly, far more than the rounding of the
-// 32-bit quotient (2^-17 at 127): rounding that quotient to even gives the
-// code of the exact quotient. The scale: max / top in 32 bits, then to 8
-// bits; the exact quotient is, by the same argument with top for the scale,
-// not within 2^-17 of a border of bf16 that it does not hit, so the two
-// roundings give the one rounding of the definition.
-template <int W>
-__global__ void __launch_bounds__(256) kv_write_kernel(const KvRows p) {
-    const KvGeo g = p.g;
-    const int i = threadIdx.x % W;  // numbers 8 * i .. of the head
-    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / W;
-    const int which = blockIdx.y;
-    const bool in = unit < (int64_t)p.n_tokens * g.heads;
-    const int t = in ? (int)(unit / g.heads) : 0, head = in ? (int)(unit % g.heads) : 0;
-    int page = 0, tok = 0;
-    const bool there = in && kv_place(p, t, page, tok);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (there && 8 * i < g.dim) v = load8(p.x[which] + t * p.token[which] + head * p.head[which] + 8 * i, g.dim - 8 * i, p.vec[which]);
-    float x[8];
+// Both kernels: W = dp / 8 neighbouring lanes (32 for dp = 192) have one head
+// of one token, 8 numbers each: 16 bytes of the caller's row of keys and as
+// many of values, for two heads at a time. Bound by those rows' bytes: they
+// are on their way while the tokens' places are looked up.
+template <int W, int BITS>
+struct KvLane {
+    int i, dim_left;      // numbers 8 * i .. of a head; how many of them there are from there on
+    int grp, k_at, v_at;  // its scale; bytes of a row
+    bool owner;           // stores the group's scale
+    int lanes;            // of a group
+    __device__ __forceinline__ explicit KvLane(const KvGeo& g) {
+        i = threadIdx.x % W;
+        dim_left = g.dim - 8 * i;
+        const int per = g.ng == 1 ? W : g.group / 8;  // a power of two
+        lanes = per;
+        grp = i / per;
+        owner = i % per == 0 && grp < g.ng;
+        k_at = kv_k_at(g, i), v_at = kv_v_at(g, 2 * i);
+    }
+};
+// numbers 8 * i + 4 .. of a value lie this far behind 8 * i ..
+template <int BITS>
+__device__ __forceinline__ int kv_v_next(const KvGeo& g) { return g.dp / 32 * (BITS / 2); }
+
+// unit n of the CTA: token and head
+__device__ __forceinline__ bool kv_unit(const KvRows& p, int unit, int& local, int& head) {
+    local = p.g.heads == 1 ? unit : (int)__umulhi((uint32_t)unit, p.head_magic);
+    head = unit - local * p.g.heads;
+    return local < p.tpc && (int64_t)blockIdx.x * p.tpc + local < p.n_tokens;
+}
+
+// Codes and scale of a group, of which this lane has the 8 numbers of v. x
+// has at most 11 significant bits and the scale s has 8, so x / s is at
+// least 2^-12 away from a border k + 1/2 of two codes that it does not hit
+// exactly. x * (1 / s) is within 2^-15 of it: rounded to a grid of 2^-12 it
+// is on its own side, or on the border where x / s is, and rounding that to
+// even gives the code of the exact quotient. The scale: max * (1 / top) is
+// within 2^-23 of max / top, which is at least 2^-16 away from any border of
+// bf16 (none can be hit: 127 or 7 times an odd number of 9 bits has more than
+// 11), so it rounds as the exact quotient does.
+template <int BITS, bool FP16>
+__device__ __forceinline__ void kv_quantise(uint4 v, int lanes, uint32_t* code, uint16_t& scale) {
+    constexpr int most = BITS == 8 ? 127 : 7;
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t top = 0;  // |x| as bits: an order that puts NaN above infinity above all numbers
+    // |x| as bits, two at a time: an order that puts NaN above infinity above all numbers
+    uint32_t big = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    for (int s = 1; s < lanes; s <<= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, s));
+    big = max(big & 0xffffu, big >> 16);
+    const bool bad = big >= (FP16 ? 0x7c00u : 0x7f80u);
+    const float top = bad ? 0.0f : unpack2(big, FP16).x;
+    float x[8];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-        const float2 f = unpack2(w[c], p.fp16);
-        x[2 * c] = f.x;
-        x[2 * c + 1] = f.y;
-        top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+        const float2 f = unpack2(w[c], FP16);
+        x[2 * c] = f.x, x[2 * c + 1] = f.y;
     }
-    // lanes of a group: group / 8 (a power of two), or all W of one group
-    const int lanes = g.ng == 1 ? W : g.group / 8;
-    for (int s = 1; s < lanes; s <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
-    const int most = g.bits == 8 ? 127 : 7;
-    const bool bad = top >= 0x7f800000u;
-    const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(bad ? 0.0f : __uint_as_float(top), (float)most));
-    const float s = __bfloat162float(sb);
-    uint32_t code[8];
+    const float grid = 0x1.8p11f, whole = 0x1.8p23f + (float)(most + 1);  // steps of 2^-12; of 1, and the stored offset
+    __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(top, 1.0f / (float)most));
+    float s = __bfloat162float(sb);
+    if (s >= 0x1p-100f) {
+        float inv;
+        asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        const float q = s > 0.0f && !bad ? rintf(__fdiv_rn(x[c], s)) : 0.0f;
-        code[c] = (uint32_t)((int)fminf(fmaxf(q, -(float)most), (float)most) + most + 1);
-    }
-    if (!there || 8 * i >= g.dp) return;
-    const int grp = g.ng == 1 ? 0 : 8 * i / g.group;
-    if (grp < g.ng && (g.ng == 1 ? i == 0 : 8 * i % g.group == 0))
-        p.scales[which][kv_scale(g, page, head, grp, tok)] = bad ? (uint16_t)0x7fff : *reinterpret_cast<const uint16_t*>(&sb);
-    uint8_t* row = p.codes[which] + kv_row(g, page, head, tok);
-    if (g.bits == 8) {
-        const uint32_t a = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
-        const uint32_t b = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
-        if (which == 0) {
-            *reinterpret_cast<uint2*>(row + kv_k_at(g, i)) = make_uint2(a, b);
-        } else {
-            *reinterpret_cast<uint32_t*>(row + kv_v_at(g, 2 * i)) = a;
-            *reinterpret_cast<uint32_t*>(row + kv_v_at(g, 2 * i + 1)) = b;
+        for (int c = 0; c < 8; ++c) code[c] = __float_as_uint(__fadd_rn(__fadd_rn(__fmaf_rn(x[c], inv, grid), -grid), whole));
+    } else {  // 1 / s may be out of range, and a subnormal scale far from max / top
+        sb = __float2bfloat16_rn(__fdiv_rn(top, (float)most));
+        s = __bfloat162float(sb);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float q = s > 0.0f && !bad ? rintf(__fdiv_rn(x[c], s)) : 0.0f;
+            code[c] = (uint32_t)((int)fminf(fmaxf(q, -(float)most), (float)most) + most + 1);
         }
-    } else if (which == 0) {
-        uint32_t a = 0;
+    }
+    scale = bad ? (uint16_t)0x7fff : *reinterpret_cast<const uint16_t*>(&sb);
+}
+// the low bytes of four words
+__device__ __forceinline__ uint32_t bytes4(const uint32_t* c) {
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+
+template <int W, int BITS, bool FP16>
+__global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
+    __shared__ int2 place[kMaxTpc];
+    constexpr int U = 2;
+    const KvGeo& g = p.g;
+    const KvLane<W, BITS> me(g);
+    const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
+    bool looked = false;
+    for (int n0 = 0; n0 < units; n0 += U * kRowThreads / W) {
+        uint4 v[U][2];
+        int local[U], head[U];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) a |= code[c] << (4 * (c >> 1) + 16 * (c & 1));
-        *reinterpret_cast<uint32_t*>(row + kv_k_at(g, i)) = a;
-    } else {
-        *reinterpret_cast<uint16_t*>(row + kv_v_at(g, 2 * i)) = (uint16_t)(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
-        *reinterpret_cast<uint16_t*>(row + kv_v_at(g, 2 * i + 1)) = (uint16_t)(code[4] | code[5] << 4 | code[6] << 8 | code[7] << 12);
+        for (int u = 0; u < U; ++u) {
+            const bool in = kv_unit(p, n0 + (u * kRowThreads + threadIdx.x) / W, local[u], head[u]) && me.dim_left > 0;
+            const int64_t t = (int64_t)blockIdx.x * p.tpc + local[u];
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                v[u][which] = make_uint4(0, 0, 0, 0);
+                if (in) v[u][which] = load8(p.x[which] + t * p.token[which] + head[u] * p.head[which] + 8 * me.i, me.dim_left, p.vec[which]);
+            }
+        }
+        if (!looked) kv_places(p, place);
+        looked = true;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int2 at = local[u] < p.tpc ? place[local[u]] : make_int2(-1, 0);
+            const bool store = at.x >= 0 && 8 * me.i < g.dp;
+            const int64_t slot = ((int64_t)at.x * g.heads + head[u]) * g.pt + at.y;
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                uint32_t code[8];
+                uint16_t scale;
+                kv_quantise<BITS, FP16>(v[u][which], me.lanes, code, scale);
+                if (!store) continue;
+                if (me.owner) p.scales[which][slot * g.ngp + me.grp] = scale;
+                uint8_t* row = p.codes[which] + slot * g.row;
+                if (BITS == 8) {
+                    const uint32_t a = bytes4(code), b = bytes4(code + 4);
+                    if (which == 0) {
+                        *reinterpret_cast<uint2*>(row + me.k_at) = make_uint2(a, b);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(row + me.v_at) = a;
+                        *reinterpret_cast<uint32_t*>(row + me.v_at + next) = b;
+                    }
+                } else {
+                    // bytes 0..3 and 4..7 to nibbles: keys pair (c, c + 1) in both halves, values in order
+                    const uint32_t a = bytes4(code) & 0x0f0f0f0fu, b = bytes4(code + 4) & 0x0f0f0f0fu;
+                    if (which == 0) {
+                        const uint32_t lo = __byte_perm(a, b, 0x6420), hi = __byte_perm(a, b, 0x7531);  // even, odd numbers
+                        *reinterpret_cast<uint32_t*>(row + me.k_at) =
+                            __byte_perm((lo | lo >> 4) & 0x00ff00ffu, (hi | hi >> 4) & 0x00ff00ffu, 0x6420);
+                    } else {
+                        const uint32_t c = (a | a >> 4) & 0x00ff00ffu, d = (b | b >> 4) & 0x00ff00ffu;
+                        *reinterpret_cast<uint16_t*>(row + me.v_at) = (uint16_t)__byte_perm(c, 0, 0x4420);
+                        *reinterpret_cast<uint16_t*>(row + me.v_at + next) = (uint16_t)__byte_perm(d, 0, 0x4420);
+                    }
+                }
+            }
+        }
     }
 }
 
-template <int W>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvRows p) {
-    const KvGeo g = p.g;
-    const int i = threadIdx.x % W;
-    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / W;
-    const int which = blockIdx.y;
-    if (unit >= (int64_t)p.n_tokens * g.heads || 8 * i >= g.dim) return;
-    const int t = (int)(unit / g.heads), head = (int)(unit % g.heads);
-    int page, tok;
-    if (!kv_place(p, t, page, tok)) return;
-    const int grp = g.ng == 1 ? 0 : 8 * i / g.group;
-    const float s = bf16_float(p.scales[which][kv_scale(g, page, head, grp, tok)]);
-    const uint8_t* row = p.codes[which] + kv_row(g, page, head, tok);
-    uint32_t code[8];
-    if (g.bits == 8) {
-        uint2 v;
-        if (which == 0) {
-            v = *reinterpret_cast<const uint2*>(row + kv_k_at(g, i));
-        } else {
-            v.x = *reinterpret_cast<const uint32_t*>(row + kv_v_at(g, 2 * i));
-            v.y = *reinterpret_cast<const uint32_t*>(row + kv_v_at(g, 2 * i + 1));
+template <int W, int BITS, bool FP16>
+__global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
+    __shared__ int2 place[kMaxTpc];
+    constexpr int U = 2;
+    const KvGeo& g = p.g;
+    const KvLane<W, BITS> me(g);
+    const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
+    kv_places(p, place);
+    for (int n0 = 0; n0 < units; n0 += U * kRowThreads / W) {
+        uint2 v[U][2];
+        uint16_t sc[U][2];
+        int local[U], head[U];
+        bool in[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            in[u] = kv_unit(p, n0 + (u * kRowThreads + threadIdx.x) / W, local[u], head[u]) && me.dim_left > 0;
+            const int2 at = in[u] ? place[local[u]] : make_int2(-1, 0);
+            in[u] = at.x >= 0;
+            const int64_t slot = ((int64_t)at.x * g.heads + head[u]) * g.pt + at.y;
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                v[u][which] = make_uint2(0, 0);
+                sc[u][which] = 0;
+                if (!in[u]) continue;
+                const uint8_t* row = p.codes[which] + slot * g.row;
+                sc[u][which] = p.scales[which][slot * g.ngp + me.grp];
+                if (BITS == 8) {
+                    if (which == 0) {
+                        v[u][0] = *reinterpret_cast<const uint2*>(row + me.k_at);
+                    } else {
+                        v[u][1].x = *reinterpret_cast<const uint32_t*>(row + me.v_at);
+                        v[u][1].y = *reinterpret_cast<const uint32_t*>(row + me.v_at + next);
+                    }
+                } else if (which == 0) {
+                    v[u][0].x = *reinterpret_cast<const uint32_t*>(row + me.k_at);
+                } else {
+                    v[u][1].x = *reinterpret_cast<const uint16_t*>(row + me.v_at) |
+                                (uint32_t)*reinterpret_cast<const uint16_t*>(row + me.v_at + next) << 16;
+                }
+            }
         }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) code[c] = ((c < 4 ? v.x : v.y) >> (8 * (c & 3))) & 255u;
-    } else if (which == 0) {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(row + kv_k_at(g, i));
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) code[c] = (v >> (4 * (c >> 1) + 16 * (c & 1))) & 15u;
-    } else {
-        const uint32_t v = *reinterpret_cast<const uint16_t*>(row + kv_v_at(g, 2 * i)) |
-                           (uint32_t)*reinterpret_cast<const uint16_t*>(row + kv_v_at(g, 2 * i + 1)) << 16;
+            for (int which = 0; which < 2; ++which) {
+                if (!in[u]) continue;
+                const float s = bf16_float(sc[u][which]);
+                float x[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) code[c] = (v >> (4 * c)) & 15u;
+                for (int c = 0; c < 8; ++c) {
+                    // on 2^23 as a float; then 7 bits times 8: exact, rounded once below
+                    uint32_t b;
+                    if (BITS == 8) b = __byte_perm(c < 4 ? v[u][which].x : v[u][which].y, 0x4b000000u, 0x7440 + (c & 3));
+                    else b = and_or(v[u][which].x >> (which ? 4 * c : 4 * (c >> 1) + 16 * (c & 1)), 15u, 0x4b000000u);
+                    x[c] = (__uint_as_float(b) - (8388608.0f + (BITS == 8 ? 128.0f : 8.0f))) * s;
+                }
+                const uint4 o = make_uint4(pack2(x[0], x[1], FP16), pack2(x[2], x[3], FP16), pack2(x[4], x[5], FP16),
+                                           pack2(x[6], x[7], FP16));
+                const int64_t t = (int64_t)blockIdx.x * p.tpc + local[u];
+                store8(p.x[which] + t * p.token[which] + head[u] * p.head[which] + 8 * me.i, o, me.dim_left, p.vec[which]);
+            }
     }
-    const int zero = g.bits == 8 ? 128 : 8;
-    float x[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) x[c] = (float)((int)code[c] - zero) * s;  // 7 bits times 8: exact, rounded once below
-    const uint4 o = make_uint4(pack2(x[0], x[1], p.fp16), pack2(x[2], x[3], p.fp16), pack2(x[4], x[5], p.fp16),
-                               pack2(x[6], x[7], p.fp16));
-    store8(p.x[which] + t * p.token[which] + head * p.head[which] + 8 * i, o, g.dim - 8 * i, p.vec[which]);
+}
+
+template <int W, int BITS, bool FP16, bool WRITE>
+void kv_launch(const KvRows& p, dim3 grid, cudaStream_t st) {
+    if (WRITE) kv_write_kernel<W, BITS, FP16><<<grid, kRowThreads, 0, st>>>(p);
+    else kv_read_kernel<W, BITS, FP16><<<grid, kRowThreads, 0, st>>>(p);
+}
+template <int W, bool WRITE>
+void kv_width(const KvRows& p, bool fp16, dim3 grid, cudaStream_t st) {
+    if (p.g.bits == 8) fp16 ? kv_launch<W, 8, true, WRITE>(p, grid, st) : kv_launch<W, 8, false, WRITE>(p, grid, st);
+    else fp16 ? kv_launch<W, 4, true, WRITE>(p, grid, st) : kv_launch<W, 4, false, WRITE>(p, grid, st);
 }
 
 template <bool WRITE>
@@ -177,23 +297,19 @@ int kv_rows(const char* what, const bnn_kv_cache* c, const void* k, int64_t k_to
     p.token[0] = k_token, p.head[0] = k_head, p.token[1] = v_token, p.head[1] = v_head;
     p.n_tokens = n_tokens, p.n_seqs = n_seqs, p.width = width;
     p.table = table, p.start = start, p.off = off;
-    p.fp16 = c->type == BNN_FP16;
     for (int w = 0; w < 2; ++w)
         p.vec[w] = aligned(p.x[w], 16) && (n_tokens == 1 || p.token[w] % 8 == 0) && (g.heads == 1 || p.head[w] % 8 == 0);
     const int W = g.dp == 64 ? 8 : g.dp == 128 ? 16 : 32;
-    const int64_t blocks = cdiv64((int64_t)n_tokens * g.heads * W, 256);
-    if (blocks > 0x7fffffff) return set_error(BNN_ERR_ARG, "%s: %d tokens are too many for one call", what, n_tokens);
-    const dim3 grid((unsigned)blocks, 2);
+    // a CTA's two heads at a time: more tokens a CTA only where every SM has several CTAs
+    p.tpc = 1;
+    while (p.tpc < kMaxTpc && p.tpc * g.heads * W < 4 * kRowThreads && n_tokens / (2 * p.tpc) >= 8 * c->sms) p.tpc *= 2;
+    p.head_magic = (uint32_t)((0x100000000ull + g.heads - 1) / g.heads);
+    const dim3 grid((unsigned)cdiv64(n_tokens, p.tpc));
     const cudaStream_t st = (cudaStream_t)stream;
-    if (WRITE) {
-        if (W == 8) kv_write_kernel<8><<<grid, 256, 0, st>>>(p);
-        else if (W == 16) kv_write_kernel<16><<<grid, 256, 0, st>>>(p);
-        else kv_write_kernel<32><<<grid, 256, 0, st>>>(p);
-    } else {
-        if (W == 8) kv_read_kernel<8><<<grid, 256, 0, st>>>(p);
-        else if (W == 16) kv_read_kernel<16><<<grid, 256, 0, st>>>(p);
-        else kv_read_kernel<32><<<grid, 256, 0, st>>>(p);
-    }
+    const bool fp16 = c->type == BNN_FP16;
+    if (W == 8) kv_width<8, WRITE>(p, fp16, grid, st);
+    else if (W == 16) kv_width<16, WRITE>(p, fp16, grid, st);
+    else kv_width<32, WRITE>(p, fp16, grid, st);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? BNN_OK : cuda_error(what, e);
 }

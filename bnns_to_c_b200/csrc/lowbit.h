@@ -53,15 +53,15 @@ LB_HD int64_t q4_scales(const Q4Geo& g) { return (int64_t)g.tiles * g.ng * 16; }
 
 // ---------------------------------------------------------------- key/value cache
 // Codes: [page][kv head][token][row bytes], keys and values apart; scales
-// (bf16): [page][kv head][group][token], so that a block of tokens has a
-// group's scales side by side. A row holds dp >= head_dim numbers (head_dim
+// (bf16): [page][kv head][token][ngp], a token's groups side by side, their
+// number rounded up to a power of two. A row holds dp >= head_dim numbers (head_dim
 // rounded up to 64, 128, 192 or 256; code 0 in the padding) in the order in
 // which the attention's lanes take them: of each 32 numbers, lane quarter
 // j = 0..3 takes 8 neighbouring keys, and lane eighth r = 0..7 takes 4
 // neighbouring values; a lane's numbers of all the 32-blocks lie together.
 // Codes are stored as code + 128 (a byte) or code + 8 (a nibble).
 struct KvGeo {
-    int pages, pt, heads, dim, dp, bits, group, ng;
+    int pages, pt, heads, dim, dp, bits, group, ng, ngp;
     int row;  // bytes of a row of codes
     int sh;   // pt = 1 << sh
 };
@@ -75,16 +75,17 @@ LB_HD KvGeo kv_geo(int pages, int pt, int heads, int dim, int bits, int group) {
     g.bits = bits;
     g.group = group;
     g.ng = (dim + group - 1) / group;
+    g.ngp = g.ng <= 1 ? 1 : g.ng <= 2 ? 2 : g.ng <= 4 ? 4 : 8;
     g.row = g.dp * bits / 8;
     g.sh = 0;
     while ((1 << g.sh) < pt) ++g.sh;
     return g;
 }
 LB_HD int64_t kv_code_bytes(const KvGeo& g) { return (int64_t)g.pages * g.heads * g.pt * g.row; }
-LB_HD int64_t kv_scales(const KvGeo& g) { return (int64_t)g.pages * g.heads * g.ng * g.pt; }
+LB_HD int64_t kv_scales(const KvGeo& g) { return (int64_t)g.pages * g.heads * g.pt * g.ngp; }
 LB_HD int64_t kv_row(const KvGeo& g, int page, int head, int tok) { return (((int64_t)page * g.heads + head) * g.pt + tok) * g.row; }
 LB_HD int64_t kv_scale(const KvGeo& g, int page, int head, int grp, int tok) {
-    return (((int64_t)page * g.heads + head) * g.ng + grp) * g.pt + tok;
+    return (((int64_t)page * g.heads + head) * g.pt + tok) * g.ngp + grp;
 }
 // byte of the row where the 8 numbers 8 * i .. 8 * i + 7 of a key lie
 // (8 bytes, or 4 with 4 bits: number c in nibble c / 2 + 4 * (c % 2))
@@ -101,25 +102,30 @@ LB_HD int kv_page(const KvGeo& g, const int32_t* table, int width, int p) {
     return page >= 0 && page < g.pages ? page : -1;
 }
 // sequence of row t: the last b in [0, n) with off[b] <= t; -1 where t is
-// before the first or behind the last
-LB_HD int kv_seq(const int32_t* off, int n, int t) {
+// before the first or behind the last. 32 places are looked at together:
+// below(lo, step, len) counts the l in 0 .. 31 with l * step < len and
+// off[lo + l * step] <= t. Offsets that do not ascend give some b in [0, n).
+template <class F>
+LB_HD int kv_seq(const int32_t* off, int n, int t, F&& below) {
     if (t < off[0] || t >= off[n]) return -1;
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (off[mid] <= t) lo = mid;
-        else hi = mid;
+    int lo = 0, len = n;
+    while (len > 1) {
+        const int step = (len + 31) / 32, k = below(lo, step, len);
+        const int skip = (k > 0 ? k - 1 : 0) * step;
+        lo += skip;
+        len = len - skip < step ? len - skip : step;
     }
     return lo;
 }
 
 // ---------------------------------------------------------------- attention's split
-// All the work is one line of blocks of kBlock tokens: sequence by sequence,
+// All the work is one line of blocks of kBlock tokens (or of kShort, where
+// no sequence is longer than that, so that none is cut): sequence by sequence,
 // within it item by item (kv head, tile of query rows), within that block by
 // block; `cta` of n takes the blocks [u * cta / n, u * (cta + 1) / n). So
 // every CTA has the same share whatever the lengths, and an item is cut at
 // most where a CTA's share ends.
-constexpr int kBlock = 64;
+constexpr int kBlock = 64, kShort = 256;
 // CTAs with a share: no more than blocks, so that none of them is empty
 LB_HD int split_ctas(int64_t units, int ctas) { return units < ctas ? (int)units : ctas; }
 LB_HD int64_t split_begin(int64_t units, int cta, int n) { return units * cta / n; }
