@@ -107,36 +107,32 @@ __device__ __forceinline__ void lds_part(uint32_t* w, const uint8_t* base, int o
 }
 
 // Codes as fp16 pairs. A byte or a nibble put into the mantissa of a power
-// of two is that power plus the code and its offset, exactly. Keys stay so:
-// a sum of products starts at -(power + offset) * (sum of q) instead of 0.
-// (That sum is at most 18 times as large as the sum of |q code|, so it costs
-// 4 of the 24 bits of a 32-bit sum.) Values have it subtracted: their weights
-// are all positive, and the sum over thousands of tokens would grow with it.
-template <int BITS>
-constexpr float kKeyOffset = BITS == 8 ? 1024.0f + 128.0f : 64.0f + 8.0f;
+// of two is that power plus the code and its offset, exactly; the subtraction
+// leaves the code. (Sums of products could start at -(power + offset) *
+// sum(q) instead, for the keys; that saves the subtraction, which is not what
+// bounds this, and costs 4 of the 24 bits of the scores' sums.)
 template <int LO>
-__device__ __forceinline__ uint32_t bytes2(uint32_t w) {  // bytes LO and LO + 1 of w on 1024
-    return __byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140);
+__device__ __forceinline__ uint32_t bytes2(uint32_t w) {  // bytes LO and LO + 1 of w
+    return Fp16::sub2(__byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140), 0x64806480u);
 }
-// the four nibble pairs of a word on 64: bits 4-7 of a half are worth 1 there
+// the four nibble pairs of a word; bits 4-7 of a half are worth 1 on 64
 __device__ __forceinline__ void nibbles4(uint32_t* a, uint32_t w) {
-    a[0] = and_or(w << 4, 0x00f000f0u, 0x54005400u);
-    a[1] = and_or(w, 0x00f000f0u, 0x54005400u);
-    a[2] = and_or(w >> 4, 0x00f000f0u, 0x54005400u);
-    a[3] = and_or(w >> 8, 0x00f000f0u, 0x54005400u);
+    a[0] = Fp16::sub2(and_or(w << 4, 0x00f000f0u, 0x54005400u), 0x54805480u);
+    a[1] = Fp16::sub2(and_or(w, 0x00f000f0u, 0x54005400u), 0x54805480u);
+    a[2] = Fp16::sub2(and_or(w >> 4, 0x00f000f0u, 0x54005400u), 0x54805480u);
+    a[3] = Fp16::sub2(and_or(w >> 8, 0x00f000f0u, 0x54005400u), 0x54805480u);
 }
 
-// Shared memory: prefix sums | row factors | start values of the score sums |
-// (m, l) of the warps | q fragments | stages, later the warps' sums.
+// Shared memory: prefix sums | row factors | (m, l) of the warps | q fragments
+// | stages, later the warps' sums.
 struct AttendSmem {
-    int factor, start, ml, q, ring, stage, bytes;
+    int factor, ml, q, ring, stage, bytes;
 };
 __host__ __device__ inline AttendSmem attend_smem(const KvGeo& g, int n_grp, int nt, int stages) {
     const int rows = 8 * nt;
     AttendSmem s;
     s.factor = ((n_grp + 1) * 4 + 127) & ~127;
-    s.start = s.factor + 128 * ((rows * 4 + 127) / 128);
-    s.ml = s.start + g.ngp * rows * 4;
+    s.ml = s.factor + 128 * ((rows * 4 + 127) / 128);
     s.q = s.ml + kWarps * rows * 8;
     s.ring = s.q + g.dp / 32 * nt * 512;
     s.stage = 2 * kSub * g.row + ((2 * g.ngp * kSub * 2 + 127) & ~127);
@@ -181,7 +177,6 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
     const AttendSmem at = attend_smem(g, p.n_grp, NT, p.stages);
     int* pre = reinterpret_cast<int*>(smem);
     float* factor = reinterpret_cast<float*>(smem + at.factor);
-    float* start = reinterpret_cast<float*>(smem + at.start);  // [group][row]
     float2* wml = reinterpret_cast<float2*>(smem + at.ml);
     uint4* qf = reinterpret_cast<uint4*>(smem + at.q);
     uint8_t* ring = smem + at.ring;
@@ -317,19 +312,9 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                 const int sh = top == 0 || e == 255 ? 0 : max(-126, min(126, 9 + 127 - e));
                 const float up = __int_as_float((127 + sh) << 23);
                 uint32_t h[4];
-                float sum = 0.0f;  // of the values as they are multiplied
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    h[c] = pack2(x[2 * c] * up, x[2 * c + 1] * up, true);
-                    const float2 f = unpack2(h[c], true);
-                    sum += f.x + f.y;
-                }
+                for (int c = 0; c < 4; ++c) h[c] = pack2(x[2 * c] * up, x[2 * c + 1] * up, true);
                 if (lane < DP / 8) qf[((lane >> 2) * NT + (i >> 3)) * 32 + (i & 7) * 4 + (lane & 3)] = make_uint4(h[0], h[1], h[2], h[3]);
-                // sums of the groups: 4 * BPG lanes each, or all
-                constexpr int LANES = NG == 1 ? 32 : 4 * BPG;
-#pragma unroll
-                for (int s = 1; s < LANES; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-                if (lane % LANES == 0 && lane / LANES < NG) start[lane / LANES * R + i] = -kKeyOffset<BITS> * sum;
                 if (lane == 0) factor[i] = p.scale_log2 * __int_as_float((127 - sh) << 23);
             }
         }
@@ -391,12 +376,6 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                     float c[NT][4];
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        if (b % BPG == 0)
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                const float2 z = *reinterpret_cast<const float2*>(start + b / BPG * R + t * 8 + 2 * j);
-                                c[t][0] = c[t][2] = z.x, c[t][1] = c[t][3] = z.y;
-                            }
                         uint4 qv[NT];
 #pragma unroll
                         for (int t = 0; t < NT; ++t) qv[t] = qf[(b * NT + t) * 32 + lane];
@@ -412,7 +391,10 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                                 a[0] = n0[2 * h], a[1] = n1[2 * h], a[2] = n0[2 * h + 1], a[3] = n1[2 * h + 1];
                             }
 #pragma unroll
-                            for (int t = 0; t < NT; ++t) Fp16::mma(c[t], a, h ? qv[t].z : qv[t].x, h ? qv[t].w : qv[t].y);
+                            for (int t = 0; t < NT; ++t) {
+                                if (b % BPG == 0 && h == 0) Fp16::mma0(c[t], a, qv[t].x, qv[t].y);
+                                else Fp16::mma(c[t], a, h ? qv[t].z : qv[t].x, h ? qv[t].w : qv[t].y);
+                            }
                         }
                         if (b == NB - 1 || b % BPG == BPG - 1) {  // the group's scale, on its sum of products
                             const float g0 = s0[b / BPG], g1 = s1[b / BPG];
@@ -445,7 +427,7 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                     v0[q] = in0 ? v0[q] : 0.0f, v1[q] = in1 ? v1[q] : 0.0f;
                     raise |= fmaxf(v0[q], v1[q]) * inv[q] > 64.0f;
                 }
-                if (__any_sync(0xffffffffu, raise)) {
+                if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -514,8 +496,8 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                         for (int x = 0; x < 2; ++x) {  // tokens 2j, 2j + 1; then 8 behind
                             const uint32_t lo = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x5140);
                             const uint32_t hi = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x7362);
-                            a[0][2 * x] = Fp16::sub2(bytes2<0>(lo), 0x64806480u), a[0][2 * x + 1] = Fp16::sub2(bytes2<2>(lo), 0x64806480u);
-                            a[1][2 * x] = Fp16::sub2(bytes2<0>(hi), 0x64806480u), a[1][2 * x + 1] = Fp16::sub2(bytes2<2>(hi), 0x64806480u);
+                            a[0][2 * x] = bytes2<0>(lo), a[0][2 * x + 1] = bytes2<2>(lo);
+                            a[1][2 * x] = bytes2<0>(hi), a[1][2 * x + 1] = bytes2<2>(hi);
                         }
                     } else {
 #pragma unroll
@@ -523,7 +505,7 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
                             uint32_t n[4];
                             nibbles4(n, __byte_perm(vw[2 * x][b >> 1], vw[2 * x + 1][b >> 1], b & 1 ? 0x7632 : 0x5410));
 #pragma unroll
-                            for (int h = 0; h < 4; ++h) a[h >> 1][2 * x + (h & 1)] = Fp16::sub2(n[h], 0x54805480u);  // 72
+                            for (int h = 0; h < 4; ++h) a[h >> 1][2 * x + (h & 1)] = n[h];
                         }
                     }
 #pragma unroll

@@ -19,14 +19,17 @@ namespace lowbit {
 // makes a device current, and the caller's again at the end of the scope
 struct DeviceScope {
     int prev = -1;
+    bool changed = false;
     cudaError_t err;
     explicit DeviceScope(int device) {
         err = cudaGetDevice(&prev);
-        if (err == cudaSuccess && prev != device) err = cudaSetDevice(device);
+        if (err == cudaSuccess && prev != device) {
+            err = cudaSetDevice(device);
+            changed = true;
+        }
     }
     ~DeviceScope() {
-        int now = -1;
-        if (prev >= 0 && cudaGetDevice(&now) == cudaSuccess && now != prev) cudaSetDevice(prev);
+        if (changed) cudaSetDevice(prev);
     }
 };
 

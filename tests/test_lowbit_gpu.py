@@ -321,11 +321,8 @@ def filled(seed, lengths, heads, dim, bits, group, kind, page, prefix=0, spare=2
 
 
 def attend_ref(q, held, scale, kind):
-    """Results, log-sums and bounds. A score is a sum of q * (code + offset),
-    minus offset * sum(q): offset * scale is 1152 / 127 or 72 / 7, at most
-    10.3, times the group's largest |key| (a scale's own rounding: 2^-8 of
-    it), so 10.4 times that joins each |term|. exp(s) has the relative error
-    of s's absolute one; weights are rounded to fp16 (2^-12, or 2^-25 of a unit that
+    """Results, log-sums and bounds. exp(s) has the relative error of s's
+    absolute one; weights are rounded to fp16 (2^-12, or 2^-25 of a unit that
     is at most twice the largest scale: |value| <= 127 scales, so at most
     2^-23 of the largest |value| a token); 2^-21 for exp2 and the joins."""
     b, heads, dim = q.shape
@@ -340,7 +337,7 @@ def attend_ref(q, held, scale, kind):
             kk, vv = k[:, h // share], v[:, h // share]
             x = q[i, h].double()
             s = kk @ x * scale
-            size = (kk.abs() + 10.4 * kk.abs().amax(-1, keepdim=True)) @ x.abs() * abs(scale)
+            size = kk.abs() @ x.abs() * abs(scale)
             ds = (2 * (dim + 16) * U * size).max() + 8 * U * s.abs().max()
             p = torch.softmax(s, 0)
             n = k.shape[0]
