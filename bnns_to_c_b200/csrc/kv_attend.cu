@@ -23,6 +23,17 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kSub = 16;  // tokens a warp takes at a time
 
+// CTAs of an attention kernel on an SM: as many as the registers allow, dp * nt
+// sums over a CTA's warps among them
+#ifndef OCC1
+#define OCC1 4
+#define OCC2 2
+#define OCC3 2
+#endif
+__host__ __device__ constexpr int attend_ctas(int dp, int nt) {
+    return dp * nt <= 128 ? OCC1 : dp * nt <= 256 ? OCC2 : OCC3;
+}
+
 struct AttendParams {
     KvGeo g;
     const uint8_t *kc, *vc;
@@ -32,7 +43,7 @@ struct AttendParams {
     uint16_t* out;
     int64_t o_seq, o_head;
     float* lse;
-    bool fp16, q_vec;
+    bool fp16, q_vec, o_vec;  // rows of q are 16-byte, of out 8-byte aligned
     int n_grp;               // sequences; 1 for the prefix
     const int32_t* lengths;  // [n_grp], or nullptr: `length`
     int length;
@@ -167,12 +178,12 @@ __device__ __forceinline__ void load_scales(float* f, const uint16_t* at) {  // 
 // DP: head_dim rounded up; NT: tiles of 8 query rows; BPG: 32-blocks of
 // channels that share a scale (8: all).
 template <int DP, int BITS, int NT, int BPG>
-__global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) attend_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kernel(const AttendParams p) {
     constexpr int NB = DP / 32, R = 8 * NT, ROW = DP * BITS / 8, CODES = kSub * ROW;
     constexpr int NG = (NB + BPG - 1) / BPG, NGP = NG <= 1 ? 1 : NG <= 2 ? 2 : NG <= 4 ? 4 : 8;
     constexpr int KP = ROW / 4, VP = ROW / 8;  // a lane's bytes of a key's, a value's row
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int warp_sum[kWarps];
+    __shared__ int2 warp_sum[kWarps];
     const KvGeo g = p.g;
     const AttendSmem at = attend_smem(g, p.n_grp, NT, p.stages);
     int* pre = reinterpret_cast<int*>(smem);
@@ -184,48 +195,61 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
     const int r = lane >> 2, j = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-    // blocks before each group, and the size of a block
-    int block = kBlock;
+    // blocks before each group, counted in both sizes at once
+    const int items = g.heads * p.rt;  // of a group
+    int block;
     {
         const int per = (p.n_grp + 32 * kWarps - 1) / (32 * kWarps), b0 = tid * per, b1 = min(p.n_grp, b0 + per);
-        bool longer = false;
-        for (int b = b0; b < b1; ++b) longer |= grp_len(p, b) > kShort;
-        if (!__syncthreads_or(longer)) block = kShort;
-        int sum = 0;
-        for (int b = b0; b < b1; ++b) sum += (grp_len(p, b) + block - 1) / block;
-        int inc = sum;
+        const auto blocks = [&](int b) {
+            const int n = grp_len(p, b);
+            return make_int2((n + kBlock - 1) / kBlock, (n + kLong - 1) / kLong);
+        };
+        int2 sum = make_int2(0, 0);
+        int most = 0;
+        for (int b = b0; b < b1; ++b) {
+            const int2 n = blocks(b);
+            sum.x += n.x, sum.y += n.y;
+            most = max(most, n.y);
+        }
+        int2 inc = sum;
         for (int s = 1; s < 32; s <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, inc, s);
-            if (lane >= s) inc += o;
+            const int x = __shfl_up_sync(0xffffffffu, inc.x, s), y = __shfl_up_sync(0xffffffffu, inc.y, s);
+            if (lane >= s) inc.x += x, inc.y += y;
         }
         if (lane == 31) warp_sum[warp] = inc;
-        __syncthreads();
-        int to = inc - sum;
-        for (int w = 0; w < warp; ++w) to += warp_sum[w];
-        for (int b = b0; b < b1; ++b) {
-            pre[b] = to;
-            to += (grp_len(p, b) + block - 1) / block;
+        const bool cut = __syncthreads_or(most > 1);
+        int2 to = make_int2(inc.x - sum.x, inc.y - sum.y), all = make_int2(0, 0);
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) to.x += warp_sum[w].x, to.y += warp_sum[w].y;
+            all.x += warp_sum[w].x, all.y += warp_sum[w].y;
         }
-        if (b0 < p.n_grp && b1 == p.n_grp) pre[p.n_grp] = to;
+        const bool lng = !cut || split_long((int64_t)all.x * items, gridDim.x);
+        block = lng ? kLong : kBlock;
+        int at = lng ? to.y : to.x;
+        for (int b = b0; b < b1; ++b) {
+            pre[b] = at;
+            const int2 n = blocks(b);
+            at += lng ? n.y : n.x;
+        }
+        if (tid == 0) pre[p.n_grp] = lng ? all.y : all.x;
         __syncthreads();
     }
-    const int items = g.heads * p.rt;  // of a group
-    const int64_t units = (int64_t)pre[p.n_grp] * items;
+    const uint32_t units = (uint32_t)pre[p.n_grp] * (uint32_t)items;  // below 2^31: the host's check
     const int ctas = split_ctas(units, gridDim.x);
     const bool has = (int)blockIdx.x < ctas;
-    const int64_t u_end = has ? split_begin(units, blockIdx.x + 1, ctas) : 0;
-    int64_t u = has ? split_begin(units, blockIdx.x, ctas) : 0;
+    const uint32_t u_end = has ? split_begin(units, blockIdx.x + 1, ctas) : 0;
+    uint32_t u = has ? split_begin(units, blockIdx.x, ctas) : 0;
 
-    // groups with nothing in them
-    if (!p.partial)
-        for (int b = blockIdx.x; b < p.n_grp; b += gridDim.x) {
+    // rows of groups with nothing in them, a warp each
+    if (!p.partial) {
+        const int q_heads = g.heads * p.share;
+        for (int64_t row = (int64_t)blockIdx.x * kWarps + warp; row < (int64_t)p.n_grp * q_heads; row += gridDim.x * kWarps) {
+            const int b = (int)((uint32_t)row / (uint32_t)q_heads), qh = (int)((uint32_t)row % (uint32_t)q_heads);
             if (pre[b + 1] != pre[b]) continue;
-            for (int i = tid; i < g.heads * p.share * g.dim; i += 32 * kWarps) {
-                const int head = i / g.dim, d = i % g.dim;
-                p.out[b * p.o_seq + head * p.o_head + d] = 0;
-                if (p.lse && d == 0) p.lse[(int64_t)b * g.heads * p.share + head] = -INFINITY;
-            }
+            for (int d = lane; d < g.dim; d += 32) p.out[b * p.o_seq + qh * p.o_head + d] = 0;
+            if (p.lse && lane == 0) p.lse[row] = -INFINITY;
         }
+    }
 
     int grp = 0;
     while (u < u_end) {
@@ -234,19 +258,19 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
             int lo = grp, hi = p.n_grp;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if ((int64_t)pre[mid] * items <= u) lo = mid;
+                if ((uint32_t)pre[mid] * (uint32_t)items <= u) lo = mid;
                 else hi = mid;
             }
             grp = lo;
         }
         const int nb = pre[grp + 1] - pre[grp];
-        const int64_t in_grp = u - (int64_t)pre[grp] * items;
-        const int item = (int)(in_grp / nb), blk0 = (int)(in_grp % nb);
-        const int blk1 = (int)min((int64_t)nb, blk0 + (u_end - u));
+        const uint32_t in_grp = u - (uint32_t)pre[grp] * (uint32_t)items;
+        const int item = (int)(in_grp / (uint32_t)nb), blk0 = (int)(in_grp % (uint32_t)nb);
+        const int blk1 = (int)min((uint32_t)nb, blk0 + (u_end - u));
         const int head = item / p.rt, tile = item % p.rt;
         const int len = grp_len(p, grp);
         const int rows = min(R, p.rg - tile * R);
-        const int64_t row0 = (int64_t)grp * p.rg + tile * R;  // row i of the item: query row (row0 + i)
+        const int row0 = grp * p.rg + tile * R;  // row i of the item: query row (row0 + i)
         if (blk0 == 0 && tid == 0)
             p.owners[(int64_t)grp * items + item] = make_int2(blockIdx.x, split_owner(units, u + nb - 1, ctas));
 
@@ -289,10 +313,10 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
 #pragma unroll
             for (int k = 0; k < R / kWarps; ++k) {
                 const int i = warp + k * kWarps;
-                const int64_t row = row0 + i;
+                const int row = row0 + i, seq = row / p.share;
                 v[k] = make_uint4(0, 0, 0, 0);
                 if (i < rows && 8 * lane < g.dim)
-                    v[k] = load8(p.q + row / p.share * p.q_seq + (head * p.share + row % p.share) * p.q_head + 8 * lane,
+                    v[k] = load8(p.q + seq * p.q_seq + (head * p.share + row - seq * p.share) * p.q_head + 8 * lane,
                                  g.dim - 8 * lane, p.q_vec);
             }
 #pragma unroll
@@ -545,42 +569,47 @@ __global__ void __launch_bounds__(32 * kWarps, DP <= 128 && NT == 1 ? 3 : 2) att
         const bool whole = blk0 == 0 && blk1 == nb;
         const int64_t slot = whole ? 2 * (int64_t)gridDim.x + (int64_t)grp * items + item : 2 * (int64_t)blockIdx.x + (blk0 == 0);
         const bool direct = whole && !p.partial;
-        for (int i = warp; i < rows; i += kWarps) {
-            float top = -INFINITY;
+        // a thread a row: the warps' weights, in the place of their maxima
+        if (tid < rows) {
+            float top = -INFINITY, c[kWarps], sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, wml[w * R + i].x);
-            float c[kWarps], sum = 0.0f;
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, wml[w * R + tid].x);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float2 ml = wml[w * R + i];
+                const float2 ml = wml[w * R + tid];
                 c[w] = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
                 sum += ml.x == -INFINITY ? 0.0f : c[w] * ml.y;
             }
-            const int64_t row = row0 + i, seq = row / p.share;
-            const int qh = head * p.share + (int)(row % p.share);
             const float norm = direct ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
-            for (int d = 2 * lane; d < DP; d += 64) {
-                float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w)
-                    if (c[w] != 0.0f) {
-                        const float2 x = *reinterpret_cast<const float2*>(sums + (w * R + i) * (DP + 8) + d);
-                        v.x = fmaf(c[w], x.x, v.x), v.y = fmaf(c[w], x.y, v.y);
-                    }
-                v.x *= norm, v.y *= norm;
-                if (direct) {
-                    if (d < g.dim) {
-                        const uint32_t o = pack2(v.x, v.y, p.fp16);
-                        uint16_t* to = p.out + seq * p.o_seq + qh * p.o_head + d;
-                        to[0] = (uint16_t)o, to[1] = (uint16_t)(o >> 16);
-                    }
-                } else {
-                    *reinterpret_cast<float2*>(p.pacc + (slot * R + i) * DP + d) = v;
-                }
+            for (int w = 0; w < kWarps; ++w) wml[w * R + tid].x = c[w] * norm;
+            const int row = row0 + tid;
+            if (!direct) p.pml[slot * R + tid] = make_float2(top, sum);
+            else if (p.lse)
+                p.lse[(int64_t)(row / p.share) * g.heads * p.share + head * p.share + row % p.share] =
+                    sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+        }
+        __syncthreads();
+        for (int n = tid; n < rows * (DP / 4); n += 32 * kWarps) {
+            const int i = n / (DP / 4), d = n % (DP / 4) * 4;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float c = wml[w * R + i].x;
+                const float4 x = *reinterpret_cast<const float4*>(sums + (w * R + i) * (DP + 8) + d);
+                v.x = fmaf(c, x.x, v.x), v.y = fmaf(c, x.y, v.y), v.z = fmaf(c, x.z, v.z), v.w = fmaf(c, x.w, v.w);
             }
-            if (lane == 0) {
-                if (!direct) p.pml[slot * R + i] = make_float2(top, sum);
-                else if (p.lse) p.lse[seq * g.heads * p.share + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+            if (!direct) {
+                *reinterpret_cast<float4*>(p.pacc + (slot * R + i) * DP + d) = v;
+            } else if (d < g.dim) {
+                const int row = row0 + i, seq = row / p.share;
+                uint16_t* to = p.out + seq * p.o_seq + (head * p.share + row - seq * p.share) * p.o_head + d;
+                const uint32_t lo = pack2(v.x, v.y, p.fp16), hi = pack2(v.z, v.w, p.fp16);
+                if (p.o_vec) {
+                    *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+                } else {
+                    to[0] = (uint16_t)lo, to[1] = (uint16_t)(lo >> 16), to[2] = (uint16_t)hi, to[3] = (uint16_t)(hi >> 16);
+                }
             }
         }
         __syncthreads();
@@ -604,6 +633,7 @@ struct JoinSide {
 };
 struct JoinParams {
     JoinSide side[2];  // own positions, prefix
+    int rows;  // query rows
     int heads, share, dim, dp;
     int width[2];  // pages of the tables
     uint16_t* out;
@@ -620,74 +650,80 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int q_heads = p.heads * p.share;
-    const int seq = blockIdx.x / q_heads, qh = blockIdx.x % q_heads, head = qh / p.share;
-    const int row = seq * p.share + qh % p.share;  // of the kv head's query rows
-    float m = -INFINITY, l = 0.0f, acc[8] = {};
-    for (int w = 0; w < 2; ++w) {
-        const JoinSide& s = p.side[w];
-        if (!s.owners) continue;
-        // the item that the row is in, and the CTAs that have its parts
-        const int grp = row / s.rg, in = row % s.rg, i = in % s.R, item = (grp * p.heads + head) * s.rt + in / s.R;
-        const int2 own = (s.lengths ? s.lengths[grp] : s.length) > 0 && p.width[w] > 0 ? s.owners[item] : make_int2(0, -1);
-        if (!p.partial && own.x >= own.y) return;  // the attention kernel has finished this row itself
-        // a lane reads the maximum and sum of a part, then all read its values
-        for (int c = own.x + warp; c <= own.y; c += 32 * kJoinWarps) {
-            const int mine = c + lane * kJoinWarps;
-            const int64_t slot = own.x == own.y ? 2 * (int64_t)s.ctas + item : 2 * (int64_t)mine + (mine == own.x);
-            float2 ml = make_float2(-INFINITY, 0.0f);
-            if (mine <= own.y) ml = s.pml[slot * s.R + i];
-            float top = ml.x;
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top = fmaxf(top, m);
-            const float a = m == -INFINITY ? 0.0f : exp2_fast(m - top);
-            const float b = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);  // 0: this part saw nothing
-            float sum = ml.x == -INFINITY ? 0.0f : b * ml.y;
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            m = top;
-            l = l * a + sum;
+    for (int n = blockIdx.x; n < p.rows; n += gridDim.x) {
+        const int seq = n / q_heads, qh = n % q_heads, head = qh / p.share;
+        const int row = seq * p.share + qh % p.share;  // of the kv head's query rows
+        float m = -INFINITY, l = 0.0f, acc[8] = {};
+        bool todo = true;
+        for (int w = 0; w < 2; ++w) {
+            const JoinSide& s = p.side[w];
+            if (!s.owners) continue;
+            // the item that the row is in, and the CTAs that have its parts
+            const int grp = row / s.rg, in = row % s.rg, i = in % s.R, item = (grp * p.heads + head) * s.rt + in / s.R;
+            const int2 own = (s.lengths ? s.lengths[grp] : s.length) > 0 && p.width[w] > 0 ? s.owners[item] : make_int2(0, -1);
+            todo = p.partial || own.x < own.y;  // else the attention kernel has finished this row itself
+            if (!todo) break;
+            // a lane reads the maximum and sum of a part, then all read its values
+            for (int c = own.x + warp; c <= own.y; c += 32 * kJoinWarps) {
+                const int mine = c + lane * kJoinWarps;
+                const int64_t slot = own.x == own.y ? 2 * (int64_t)s.ctas + item : 2 * (int64_t)mine + (mine == own.x);
+                float2 ml = make_float2(-INFINITY, 0.0f);
+                if (mine <= own.y) ml = s.pml[slot * s.R + i];
+                float top = ml.x;
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = fmaxf(top, m);
+                const float a = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+                const float b = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);  // 0: this part saw nothing
+                float sum = ml.x == -INFINITY ? 0.0f : b * ml.y;
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                m = top;
+                l = l * a + sum;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] *= a;
-            // (a part that saw nothing has left zeros)
-            const int parts = min(32, (own.y - c) / kJoinWarps + 1);
+                for (int k = 0; k < 8; ++k) acc[k] *= a;
+                // (a part that saw nothing has left zeros)
+                const int parts = min(32, (own.y - c) / kJoinWarps + 1);
 #pragma unroll 8
-            for (int q = 0; q < parts; ++q) {
-                const float f = __shfl_sync(0xffffffffu, b, q);
-                const int64_t from = __shfl_sync(0xffffffffu, slot, q);
-                const float* x = s.pacc + (from * s.R + i) * p.dp + 4 * lane;
+                for (int q = 0; q < parts; ++q) {
+                    const float f = __shfl_sync(0xffffffffu, b, q);
+                    const int64_t from = __shfl_sync(0xffffffffu, slot, q);
+                    const float* x = s.pacc + (from * s.R + i) * p.dp + 4 * lane;
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    if (128 * k + 4 * lane < p.dp) {
-                        const float4 v = *reinterpret_cast<const float4*>(x + 128 * k);
-                        acc[4 * k] = fmaf(f, v.x, acc[4 * k]), acc[4 * k + 1] = fmaf(f, v.y, acc[4 * k + 1]);
-                        acc[4 * k + 2] = fmaf(f, v.z, acc[4 * k + 2]), acc[4 * k + 3] = fmaf(f, v.w, acc[4 * k + 3]);
-                    }
+                    for (int k = 0; k < 2; ++k)
+                        if (128 * k + 4 * lane < p.dp) {
+                            const float4 v = *reinterpret_cast<const float4*>(x + 128 * k);
+                            acc[4 * k] = fmaf(f, v.x, acc[4 * k]), acc[4 * k + 1] = fmaf(f, v.y, acc[4 * k + 1]);
+                            acc[4 * k + 2] = fmaf(f, v.z, acc[4 * k + 2]), acc[4 * k + 3] = fmaf(f, v.w, acc[4 * k + 3]);
+                        }
+                }
             }
         }
+        if (!todo) continue;
+        if (lane == 0) wml[warp] = make_float2(m, l);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (128 * k + 4 * lane < p.dp)
+                *reinterpret_cast<float4*>(&sums[warp][128 * k + 4 * lane]) = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
+        __syncthreads();
+        float top = -INFINITY, c[kJoinWarps], sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, wml[w].x);
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            c[w] = wml[w].x == -INFINITY ? 0.0f : exp2_fast(wml[w].x - top);
+            sum += wml[w].x == -INFINITY ? 0.0f : c[w] * wml[w].y;
+        }
+        const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int d = threadIdx.x; d < p.dim; d += 32 * kJoinWarps) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w)
+                if (c[w] != 0.0f) v = fmaf(c[w], sums[w][d], v);
+            p.out[seq * p.o_seq + qh * p.o_head + d] = (uint16_t)pack2(v * norm, 0.0f, p.fp16);
+        }
+        if (p.lse && threadIdx.x == 0)
+            p.lse[(int64_t)seq * q_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+        __syncthreads();
     }
-    if (lane == 0) wml[warp] = make_float2(m, l);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-        if (128 * k + 4 * lane < p.dp)
-            *reinterpret_cast<float4*>(&sums[warp][128 * k + 4 * lane]) = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
-    __syncthreads();
-    float top = -INFINITY, c[kJoinWarps], sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, wml[w].x);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-        c[w] = wml[w].x == -INFINITY ? 0.0f : exp2_fast(wml[w].x - top);
-        sum += wml[w].x == -INFINITY ? 0.0f : c[w] * wml[w].y;
-    }
-    const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int d = threadIdx.x; d < p.dim; d += 32 * kJoinWarps) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w)
-            if (c[w] != 0.0f) v = fmaf(c[w], sums[w][d], v);
-        p.out[seq * p.o_seq + qh * p.o_head + d] = (uint16_t)pack2(v * norm, 0.0f, p.fp16);
-    }
-    if (p.lse && threadIdx.x == 0)
-        p.lse[(int64_t)seq * q_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
 // ---------------------------------------------------------------- host
@@ -708,7 +744,7 @@ Plan attend_plan(const bnn_kv_cache* c, int n_grp, int rg, bool partial) {
     const int most = g.dp <= 128 ? 4 : 2;  // registers: dp * nt sums over a warp's lanes
     s.nt = rg <= 8 ? 1 : rg <= 16 || most == 2 ? 2 : 4;
     s.rt = (int)cdiv64(rg, 8 * s.nt);
-    const int per_sm = g.dp <= 128 && s.nt == 1 ? 3 : 2;
+    const int per_sm = attend_ctas(g.dp, s.nt);
     s.ctas = (c->sms > 0 ? c->sms : 148) * per_sm;
     const int R = 8 * s.nt;
     s.stages = 2;
@@ -812,7 +848,8 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
         return set_error(BNN_ERR_ARG, "bnn_kv_attend: negative table width, or a scale that is not finite");
     if ((int64_t)table_pages * g.pt > INT_MAX - 256 || (int64_t)prefix_pages * g.pt > INT_MAX - 256)
         return set_error(BNN_ERR_ARG, "bnn_kv_attend: a table of 2^31 tokens or more");
-    if ((int64_t)n_seqs * cdiv64((int64_t)table_pages * g.pt, kBlock) > INT_MAX)
+    if (n_seqs > 0 && q_heads > INT_MAX / n_seqs) return set_error(BNN_ERR_ARG, "bnn_kv_attend: %d sequences of %d heads", n_seqs, q_heads);
+    if (((int64_t)n_seqs * table_pages + (prefix ? (int64_t)n_seqs * prefix_pages : 0)) * cdiv64(g.pt, kBlock) > INT_MAX / q_heads)
         return set_error(BNN_ERR_ARG, "bnn_kv_attend: %d sequences of up to %lld tokens are too many for one call", n_seqs,
                          (long long)table_pages * g.pt);
     if (prefix && (!d_prefix || (int64_t)prefix_pages * g.pt < prefix_tokens))
@@ -846,10 +883,12 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
     p.out = (uint16_t*)d_out, p.o_seq = o_seq, p.o_head = o_head, p.lse = d_lse;
     p.fp16 = c->type == BNN_FP16;
     p.q_vec = aligned(d_q, 16) && (n_seqs == 1 || q_seq % 8 == 0) && (q_heads == 1 || q_head % 8 == 0);
+    p.o_vec = aligned(d_out, 8) && (n_seqs == 1 || o_seq % 4 == 0) && (q_heads == 1 || o_head % 4 == 0);
     p.share = share;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.partial = prefix;
     JoinParams jp{};
+    jp.rows = n_seqs * q_heads;
     jp.heads = g.heads, jp.share = share, jp.dim = g.dim, jp.dp = g.dp;
     jp.out = p.out, jp.o_seq = o_seq, jp.o_head = o_head, jp.lse = d_lse;
     jp.fp16 = p.fp16, jp.partial = prefix;
@@ -875,9 +914,9 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
         jp.width[side] = p.width;
     }
     // no sequence can be longer than a block: none is cut
-    if (!prefix && (int64_t)table_pages * g.pt <= kShort) return BNN_OK;
+    if (!prefix && (int64_t)table_pages * g.pt <= kLong) return BNN_OK;
     cudaLaunchAttribute beside[1];
-    cudaLaunchConfig_t cfg = launch_config(dim3((unsigned)((int64_t)n_seqs * q_heads)), 32 * kJoinWarps, 0, st, beside);
+    cudaLaunchConfig_t cfg = launch_config(dim3((unsigned)min(jp.rows, c->sms * 12)), 32 * kJoinWarps, 0, st, beside);
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel, (const JoinParams)jp);
     return e == cudaSuccess ? BNN_OK : cuda_error("bnn_kv_attend", e);

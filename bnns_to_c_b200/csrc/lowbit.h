@@ -119,18 +119,26 @@ LB_HD int kv_seq(const int32_t* off, int n, int t, F&& below) {
 }
 
 // ---------------------------------------------------------------- attention's split
-// All the work is one line of blocks of kBlock tokens (or of kShort, where
-// no sequence is longer than that, so that none is cut): sequence by sequence,
-// within it item by item (kv head, tile of query rows), within that block by
-// block; `cta` of n takes the blocks [u * cta / n, u * (cta + 1) / n). So
-// every CTA has the same share whatever the lengths, and an item is cut at
-// most where a CTA's share ends.
-constexpr int kBlock = 64, kShort = 256;
+// All the work is one line of blocks of tokens: sequence by sequence, within
+// it item by item (kv head, tile of query rows), within that block by block;
+// n CTAs take equal shares of it, the first ones a block more. So every CTA
+// has the same work whatever the lengths, and an item is cut only where a
+// share ends. A cut costs a CTA about what 256 tokens do, so blocks have as
+// many, unless the shares are so long that 64 balance them better. They have
+// as many, too, where no sequence is longer: then no item is cut.
+constexpr int kBlock = 64, kLong = 256;
+LB_HD bool split_long(int64_t blocks, int ctas) { return blocks < (int64_t)ctas * (2 * kLong / kBlock); }
 // CTAs with a share: no more than blocks, so that none of them is empty
-LB_HD int split_ctas(int64_t units, int ctas) { return units < ctas ? (int)units : ctas; }
-LB_HD int64_t split_begin(int64_t units, int cta, int n) { return units * cta / n; }
+LB_HD int split_ctas(uint32_t units, int ctas) { return units < (uint32_t)ctas ? (int)units : ctas; }
+LB_HD uint32_t split_begin(uint32_t units, int cta, int n) {
+    const uint32_t q = units / (uint32_t)n, r = units % (uint32_t)n;
+    return cta * q + ((uint32_t)cta < r ? (uint32_t)cta : r);
+}
 // the CTA that has block u (0 <= u < units)
-LB_HD int split_owner(int64_t units, int64_t u, int n) { return (int)(((u + 1) * n - 1) / units); }
+LB_HD int split_owner(uint32_t units, uint32_t u, int n) {
+    const uint32_t q = units / (uint32_t)n, r = units % (uint32_t)n, more = r * (q + 1);
+    return (int)(u < more ? u / (q + 1) : r + (u - more) / q);
+}
 
 }  // namespace lowbit
 }  // namespace bnn

@@ -109,16 +109,16 @@ static void pages() {
 static void split() {
     std::mt19937 rng(2);
     for (int n = 0; n < 3000; ++n) {
-        const int64_t units = 1 + (int64_t)(rng() % 3000);
+        const uint32_t units = 1 + rng() % 3000;
         const int ctas = split_ctas(units, 1 + (int)(rng() % 500));
-        CHECK(ctas >= 1 && ctas <= units);
+        CHECK(ctas >= 1 && (uint32_t)ctas <= units);
         for (int c = 0; c < ctas; ++c) CHECK(split_begin(units, c, ctas) < split_begin(units, c + 1, ctas));
         for (int c = 0; c < ctas; ++c)
-            for (int64_t u = split_begin(units, c, ctas); u < split_begin(units, c + 1, ctas); ++u) CHECK(split_owner(units, u, ctas) == c);
+            for (uint32_t u = split_begin(units, c, ctas); u < split_begin(units, c + 1, ctas); ++u) CHECK(split_owner(units, u, ctas) == c);
         CHECK(split_begin(units, 0, ctas) == 0 && split_begin(units, ctas, ctas) == units);
     }
-    const int64_t many = (int64_t)1 << 44;  // 2^31 blocks of a batch, 4096 kv heads and tiles of them
-    CHECK(split_owner(many, many - 1, 592) == 591 && split_begin(many, 592, 592) == many);
+    const uint32_t many = 0x7fffffff;  // the most that a call takes
+    CHECK(split_owner(many, many - 1, 592) == 591 && split_begin(many, 592, 592) == many && split_owner(many, 0, 592) == 0);
 }
 
 int main() {
