@@ -21,7 +21,12 @@ namespace lowbit {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kSub = 16;  // tokens a warp takes at a time
+constexpr int kSub = 16;  // tokens of an instruction
+// 16-token blocks that a warp takes at a time: two where the sums leave it the
+// registers and a row is short (of `row` bytes), so that shared memory holds
+// enough steps: 64 ragged sequences in 4 bits 82 us against 90 of one at a
+// time, but 100003 tokens in 8 bits, 128-byte rows, 58 against 47.
+__host__ __device__ constexpr int attend_halves(int nt, int row) { return nt == 1 && row <= 64 ? 2 : 1; }
 
 // CTAs of an attention kernel on an SM: as many as the registers allow, dp * nt
 // sums over a CTA's warps among them
@@ -126,12 +131,14 @@ template <int LO>
 __device__ __forceinline__ uint32_t bytes2(uint32_t w) {  // bytes LO and LO + 1 of w
     return Fp16::sub2(__byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140), 0x64806480u);
 }
-// the four nibble pairs of a word; bits 4-7 of a half are worth 1 on 64
+// the four nibble pairs of a word: bits 0-3 of a half on 1024, bits 4-7, which
+// are worth 1 there, on 64
 __device__ __forceinline__ void nibbles4(uint32_t* a, uint32_t w) {
-    a[0] = Fp16::sub2(and_or(w << 4, 0x00f000f0u, 0x54005400u), 0x54805480u);
+    const uint32_t v = w >> 8;
+    a[0] = Fp16::sub2(and_or(w, 0x000f000fu, 0x64006400u), 0x64086408u);
     a[1] = Fp16::sub2(and_or(w, 0x00f000f0u, 0x54005400u), 0x54805480u);
-    a[2] = Fp16::sub2(and_or(w >> 4, 0x00f000f0u, 0x54005400u), 0x54805480u);
-    a[3] = Fp16::sub2(and_or(w >> 8, 0x00f000f0u, 0x54005400u), 0x54805480u);
+    a[2] = Fp16::sub2(and_or(v, 0x000f000fu, 0x64006400u), 0x64086408u);
+    a[3] = Fp16::sub2(and_or(v, 0x00f000f0u, 0x54005400u), 0x54805480u);
 }
 
 // Shared memory: prefix sums | row factors | (m, l) of the warps | q fragments
@@ -146,7 +153,7 @@ __host__ __device__ inline AttendSmem attend_smem(const KvGeo& g, int n_grp, int
     s.ml = s.factor + 128 * ((rows * 4 + 127) / 128);
     s.q = s.ml + kWarps * rows * 8;
     s.ring = s.q + g.dp / 32 * nt * 512;
-    s.stage = 2 * kSub * g.row + ((2 * g.ngp * kSub * 2 + 127) & ~127);
+    s.stage = attend_halves(nt, g.row) * (2 * kSub * g.row + ((2 * g.ngp * kSub * 2 + 127) & ~127));
     const int ring = kWarps * stages * s.stage, merge = kWarps * rows * (g.dp + 8) * 4;
     s.bytes = s.ring + (ring > merge ? ring : merge);
     return s;
@@ -182,6 +189,8 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
     constexpr int NB = DP / 32, R = 8 * NT, ROW = DP * BITS / 8, CODES = kSub * ROW;
     constexpr int NG = (NB + BPG - 1) / BPG, NGP = NG <= 1 ? 1 : NG <= 2 ? 2 : NG <= 4 ? 4 : 8;
     constexpr int KP = ROW / 4, VP = ROW / 8;  // a lane's bytes of a key's, a value's row
+    constexpr int HV = attend_halves(NT, ROW), KS = kSub * HV;  // 16-token blocks, tokens of a step
+    constexpr int HALF = 2 * CODES + ((2 * NGP * kSub * 2 + 127) & ~127);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int2 warp_sum[kWarps];
     const KvGeo g = p.g;
@@ -274,34 +283,41 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
         if (blk0 == 0 && tid == 0)
             p.owners[(int64_t)grp * items + item] = make_int2(blockIdx.x, split_owner(units, u + nb - 1, ctas));
 
-        const int sub0 = blk0 * (block / kSub), sub1 = min(blk1 * (block / kSub), (len + kSub - 1) / kSub);
+        // steps of KS tokens; the warps take them in turn
+        const int end = min(blk1 * block, len), sub0 = blk0 * (block / KS), sub1 = (end + KS - 1) / KS;
         uint8_t* mine = ring + warp * p.stages * at.stage;
         const int32_t* row_table = p.table + (int64_t)grp * p.width;
-        // copies of one 16-token block into a stage; its page
-        const auto fetch = [&](int sub, uint8_t* to) -> int {
-            const int pos = sub * kSub, page = kv_page(g, row_table, p.width, pos);
-            if (page < 0) return -1;
-            const int tok = pos & (g.pt - 1);
-            const int64_t from = kv_row(g, page, head, tok);
-            const uint32_t dst = smem_addr(to);
-            static_assert(CODES % 512 == 0, "whole pieces for every lane");
+        // copies of a step's tokens into a stage; bit h: its h-th 16 tokens have a page
+        const auto fetch = [&](int sub, uint8_t* to) -> uint32_t {
+            uint32_t got = 0;
 #pragma unroll
-            for (int c = 0; c < CODES / 512; ++c) {
-                const int o = (c * 32 + lane) * 16;
-                cp16(dst + swz<ROW>(o), p.kc + from + o);
-                cp16(dst + CODES + swz<ROW>(o), p.vc + from + o);
+            for (int h = 0; h < HV; ++h) {
+                const int pos = sub * KS + h * kSub;
+                const int page = pos < end ? kv_page(g, row_table, p.width, pos) : -1;
+                if (page < 0) continue;
+                got |= 1u << h;
+                const int tok = pos & (g.pt - 1);
+                const int64_t slot = ((int64_t)page * g.heads + head) * g.pt + tok, from = slot * ROW;
+                const uint32_t dst = smem_addr(to) + h * HALF;
+                static_assert(CODES % 512 == 0, "whole pieces for every lane");
+#pragma unroll
+                for (int c = 0; c < CODES / 512; ++c) {
+                    const int o = (c * 32 + lane) * 16;
+                    cp16(dst + swz<ROW>(o), p.kc + from + o);
+                    cp16(dst + CODES + swz<ROW>(o), p.vc + from + o);
+                }
+                if (lane < 4 * NGP) {  // 32 * NGP bytes of scales of each
+                    const int of = lane >= 2 * NGP, c = of ? lane - 2 * NGP : lane;
+                    cp16(dst + 2 * CODES + lane * 16, (of ? p.vs : p.ks) + slot * NGP + 8 * c);
+                }
             }
-            if (lane < 4 * NGP) {  // 32 * NGP bytes of scales of each
-                const int of = lane >= 2 * NGP, c = of ? lane - 2 * NGP : lane;
-                cp16(dst + 2 * CODES + lane * 16, (of ? p.vs : p.ks) + kv_scale(g, page, head, 0, tok) + 8 * c);
-            }
-            return page;
+            return got;
         };
-        // the first blocks are on their way while q is made ready
-        uint32_t there = 0;  // of the stages: whether their block has a page
+        // the first steps are on their way while q is made ready
+        uint32_t there = 0;  // HV bits a stage
         int ahead = sub0 + warp;
         for (int s = 0; s < p.stages - 1; ++s, ahead += kWarps) {
-            if (ahead < sub1 && fetch(ahead, mine + s * at.stage) >= 0) there |= 1u << s;
+            if (ahead < sub1) there |= fetch(ahead, mine + s * at.stage) << (HV * s);
             cp_commit();
         }
 
@@ -369,8 +385,8 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
         int st = 0, st_in = p.stages - 1;
         for (int sub = sub0 + warp; sub < sub1; sub += kWarps) {
             // the stage read a round ago is free: all lanes passed the barrier below
-            there &= ~(1u << st_in);
-            if (ahead < sub1 && fetch(ahead, mine + st_in * at.stage) >= 0) there |= 1u << st_in;
+            there &= ~(((1u << HV) - 1) << (HV * st_in));
+            if (ahead < sub1) there |= fetch(ahead, mine + st_in * at.stage) << (HV * st_in);
             ahead += kWarps;
             cp_commit();
             st_in = st_in + 1 == p.stages ? 0 : st_in + 1;
@@ -382,21 +398,24 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                 default: cp_wait<5>(); break;
             }
             __syncwarp();
-            const uint8_t* kb = mine + st * at.stage;
-            const bool page_there = there >> st & 1u;
+            const uint8_t* step = mine + st * at.stage;
+            const uint32_t have = there >> (HV * st) & ((1u << HV) - 1);
             st = st + 1 == p.stages ? 0 : st + 1;
-            if (page_there) {
-                const uint8_t* vb = kb + CODES;
-                const uint16_t* sc = reinterpret_cast<const uint16_t*>(kb + 2 * CODES);  // [keys, values][token][NGP]
+            if (have) {
                 // scores: tokens r and r + 8 in rows, query rows in columns
-                float s[NT][4];
-                {
+                float s[HV][NT][4], v0[HV][NGP], v1[HV][NGP];  // v0, v1: scales of the two tokens' values
+#pragma unroll
+                for (int h = 0; h < HV; ++h) {
+                    const uint8_t* kb = step + h * HALF;
+                    const uint16_t* sc = reinterpret_cast<const uint16_t*>(kb + 2 * CODES);  // [keys, values][token][NGP]
                     uint32_t k0[KP / 4], k1[KP / 4];
                     lds_part<ROW, KP>(k0, kb, r * ROW + j * KP);
                     lds_part<ROW, KP>(k1, kb, (r + 8) * ROW + j * KP);
                     float s0[NGP], s1[NGP];
                     load_scales<NGP>(s0, sc + r * NGP);
                     load_scales<NGP>(s1, sc + (r + 8) * NGP);
+                    load_scales<NGP>(v0[h], sc + (kSub + r) * NGP);
+                    load_scales<NGP>(v1[h], sc + (kSub + r + 8) * NGP);
                     float c[NT][4];
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
@@ -406,18 +425,18 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                         uint32_t n0[4], n1[4];
                         if constexpr (BITS == 4) nibbles4(n0, k0[b]), nibbles4(n1, k1[b]);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
+                        for (int x = 0; x < 2; ++x) {
                             uint32_t a[4];
                             if constexpr (BITS == 8) {
-                                a[0] = bytes2<0>(k0[2 * b + h]), a[1] = bytes2<0>(k1[2 * b + h]);
-                                a[2] = bytes2<2>(k0[2 * b + h]), a[3] = bytes2<2>(k1[2 * b + h]);
+                                a[0] = bytes2<0>(k0[2 * b + x]), a[1] = bytes2<0>(k1[2 * b + x]);
+                                a[2] = bytes2<2>(k0[2 * b + x]), a[3] = bytes2<2>(k1[2 * b + x]);
                             } else {
-                                a[0] = n0[2 * h], a[1] = n1[2 * h], a[2] = n0[2 * h + 1], a[3] = n1[2 * h + 1];
+                                a[0] = n0[2 * x], a[1] = n1[2 * x], a[2] = n0[2 * x + 1], a[3] = n1[2 * x + 1];
                             }
 #pragma unroll
                             for (int t = 0; t < NT; ++t) {
-                                if (b % BPG == 0 && h == 0) Fp16::mma0(c[t], a, qv[t].x, qv[t].y);
-                                else Fp16::mma(c[t], a, h ? qv[t].z : qv[t].x, h ? qv[t].w : qv[t].y);
+                                if (b % BPG == 0 && x == 0) Fp16::mma0(c[t], a, qv[t].x, qv[t].y);
+                                else Fp16::mma(c[t], a, x ? qv[t].z : qv[t].x, x ? qv[t].w : qv[t].y);
                             }
                         }
                         if (b == NB - 1 || b % BPG == BPG - 1) {  // the group's scale, on its sum of products
@@ -425,38 +444,57 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 #pragma unroll
                             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) s[t][e] = b < BPG ? (e < 2 ? g0 : g1) * c[t][e] : fmaf(e < 2 ? g0 : g1, c[t][e], s[t][e]);
+                                for (int e = 0; e < 4; ++e)
+                                    s[h][t][e] = b < BPG ? (e < 2 ? g0 : g1) * c[t][e] : fmaf(e < 2 ? g0 : g1, c[t][e], s[h][t][e]);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[h][t][e] *= f[t][e & 1];
+                }
+                // tokens that are not there: behind the end, or without a page
+                if (__builtin_expect(have != (1u << HV) - 1 || (sub + 1) * KS > len, 0)) {
+#pragma unroll
+                    for (int h = 0; h < HV; ++h) {
+                        const int left = have >> h & 1u ? len - (sub * KS + h * kSub) : 0;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[h][t][e] = r + (e < 2 ? 0 : 8) < left ? s[h][t][e] : -INFINITY;
+#pragma unroll
+                        for (int q = 0; q < NG; ++q) {
+                            v0[h][q] = r < left ? v0[h][q] : 0.0f;
+                            v1[h][q] = r + 8 < left ? v1[h][q] : 0.0f;
                         }
                     }
                 }
-                const bool in0 = sub * kSub + r < len, in1 = sub * kSub + r + 8 < len;
-                float v0[NGP], v1[NGP];
-                load_scales<NGP>(v0, sc + (kSub + r) * NGP);
-                load_scales<NGP>(v1, sc + (kSub + r + 8) * NGP);
                 // The running maximum and the units are lazy: raised when a
                 // score is 2^8 above the maximum, or a scale 2^6 above its
-                // unit, so most blocks need no reduction over the lanes.
+                // unit, so most steps need no reduction over the lanes.
                 // weight * scale / unit stays below 2^14, in fp16.
                 bool raise = false;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        s[t][e] = in0 ? s[t][e] * f[t][e] : -INFINITY;
-                        s[t][2 + e] = in1 ? s[t][2 + e] * f[t][e] : -INFINITY;
-                        raise |= fmaxf(s[t][e], s[t][2 + e]) > m[t][e] + 8.0f;
+                        float x = fmaxf(s[0][t][e], s[0][t][2 + e]);
+                        if constexpr (HV == 2) x = fmaxf(x, fmaxf(s[1][t][e], s[1][t][2 + e]));
+                        raise |= x > m[t][e] + 8.0f;
                     }
 #pragma unroll
                 for (int q = 0; q < NG; ++q) {
-                    v0[q] = in0 ? v0[q] : 0.0f, v1[q] = in1 ? v1[q] : 0.0f;
-                    raise |= fmaxf(v0[q], v1[q]) * inv[q] > 64.0f;
+                    float x = fmaxf(v0[0][q], v1[0][q]);
+                    if constexpr (HV == 2) x = fmaxf(x, fmaxf(v0[1][q], v1[1][q]));
+                    raise |= x * inv[q] > 64.0f;
                 }
                 if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float x = fmaxf(s[t][e], s[t][2 + e]);
+                            float x = fmaxf(s[0][t][e], s[0][t][2 + e]);
+                            if constexpr (HV == 2) x = fmaxf(x, fmaxf(s[1][t][e], s[1][t][2 + e]));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -471,8 +509,13 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                         }
 #pragma unroll
                     for (int q = 0; q < NG; ++q) {
-                        const uint32_t u0 = __float_as_uint(v0[q]), u1 = __float_as_uint(v1[q]);  // NaN: bits above infinity's
-                        const uint32_t big = __reduce_max_sync(0xffffffffu, max(u0 < 0x7f800000u ? u0 : 0u, u1 < 0x7f800000u ? u1 : 0u));
+                        uint32_t big = 0;
+#pragma unroll
+                        for (int h = 0; h < HV; ++h) {
+                            const uint32_t u0 = __float_as_uint(v0[h][q]), u1 = __float_as_uint(v1[h][q]);  // NaN: bits above infinity's
+                            big = max(big, max(u0 < 0x7f800000u ? u0 : 0u, u1 < 0x7f800000u ? u1 : 0u));
+                        }
+                        big = __reduce_max_sync(0xffffffffu, big);
                         const uint32_t unit = (254u << 23) - __float_as_uint(inv[q]), now = max(unit, min(big & 0x7f800000u, 253u << 23));
                         const int down = (int)((now - unit) >> 23);
                         const float corr = down > 126 ? 0.0f : __int_as_float((127 - down) << 23);
@@ -492,50 +535,57 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float base = m[t][e] == -INFINITY ? 0.0f : m[t][e];
-                        s[t][e] = exp2_fast(s[t][e] - base);
-                        s[t][2 + e] = exp2_fast(s[t][2 + e] - base);
-                        l[t][e] += s[t][e] + s[t][2 + e];
+#pragma unroll
+                        for (int h = 0; h < HV; ++h) {
+                            s[h][t][e] = exp2_fast(s[h][t][e] - base);
+                            s[h][t][2 + e] = exp2_fast(s[h][t][2 + e] - base);
+                            l[t][e] += s[h][t][e] + s[h][t][2 + e];
+                        }
                     }
                 // output: channels in rows, query rows in columns, the tokens
                 // summed. The values' scales go with the weights, rounded
                 // once to fp16: 2^-12 of each term, independent of one
                 // another, next to a result of 8 or 11 bits.
-                uint32_t vw[4][(VP + 3) / 4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) lds_part<ROW, VP>(vw[t], vb, (2 * j + (t & 1) + 8 * (t >> 1)) * ROW + r * VP);
-                uint32_t wb[NT][2];
+                for (int h = 0; h < HV; ++h) {
+                    const uint8_t* vb = step + h * HALF + CODES;
+                    uint32_t vw[4][(VP + 3) / 4];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if (b % BPG == 0) {
-                        const float w0 = v0[b / BPG] * inv[b / BPG], w1 = v1[b / BPG] * inv[b / BPG];
+                    for (int t = 0; t < 4; ++t) lds_part<ROW, VP>(vw[t], vb, (2 * j + (t & 1) + 8 * (t >> 1)) * ROW + r * VP);
+                    uint32_t wb[NT][2];
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            wb[t][0] = movm_t(pack2(s[t][0] * w0, s[t][1] * w0, true));
-                            wb[t][1] = movm_t(pack2(s[t][2] * w1, s[t][3] * w1, true));
+                    for (int b = 0; b < NB; ++b) {
+                        if (b % BPG == 0) {
+                            const float w0 = v0[h][b / BPG] * inv[b / BPG], w1 = v1[h][b / BPG] * inv[b / BPG];
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                wb[t][0] = movm_t(pack2(s[h][t][0] * w0, s[h][t][1] * w0, true));
+                                wb[t][1] = movm_t(pack2(s[h][t][2] * w1, s[h][t][3] * w1, true));
+                            }
                         }
+                        uint32_t a[2][4];
+                        if constexpr (BITS == 8) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {  // tokens 2j, 2j + 1; then 8 behind
+                                const uint32_t lo = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x5140);
+                                const uint32_t hi = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x7362);
+                                a[0][2 * x] = bytes2<0>(lo), a[0][2 * x + 1] = bytes2<2>(lo);
+                                a[1][2 * x] = bytes2<0>(hi), a[1][2 * x + 1] = bytes2<2>(hi);
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                uint32_t n[4];
+                                nibbles4(n, __byte_perm(vw[2 * x][b >> 1], vw[2 * x + 1][b >> 1], b & 1 ? 0x7632 : 0x5410));
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) a[c >> 1][2 * x + (c & 1)] = n[c];
+                            }
+                        }
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) Fp16::mma(acc[b][c][t], a[c], wb[t][0], wb[t][1]);
                     }
-                    uint32_t a[2][4];
-                    if constexpr (BITS == 8) {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {  // tokens 2j, 2j + 1; then 8 behind
-                            const uint32_t lo = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x5140);
-                            const uint32_t hi = __byte_perm(vw[2 * x][b], vw[2 * x + 1][b], 0x7362);
-                            a[0][2 * x] = bytes2<0>(lo), a[0][2 * x + 1] = bytes2<2>(lo);
-                            a[1][2 * x] = bytes2<0>(hi), a[1][2 * x + 1] = bytes2<2>(hi);
-                        }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            uint32_t n[4];
-                            nibbles4(n, __byte_perm(vw[2 * x][b >> 1], vw[2 * x + 1][b >> 1], b & 1 ? 0x7632 : 0x5410));
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) a[h >> 1][2 * x + (h & 1)] = n[h];
-                        }
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) Fp16::mma(acc[b][h][t], a[h], wb[t][0], wb[t][1]);
                 }
             }
             __syncwarp();
