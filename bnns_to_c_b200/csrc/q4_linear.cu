@@ -250,11 +250,14 @@ cudaError_t q4_forms(const Q4Params& p, cudaStream_t st) {
 // 256 (128 clocks a product) two threads take the stages in turn, with sums
 // of their own that are added at the end.
 constexpr int kGroups = 2, kWWarps = 8 * kGroups;
-constexpr int kAhead = 4;   // stages of a group whose codes are on their way
-constexpr int kXWarps = 8;  // that load x where TMA cannot
+constexpr int kAhead = 4;   // 64-input blocks of a group whose codes are on their way
+constexpr int kXWarps = 8;  // that load x where TMA cannot: kXWarps / S of them a stage
 constexpr int q4_issuers(int ntok) { return ntok == 256 ? 1 : 2; }
 constexpr int q4_tile_threads(int ntok) { return 32 * (kWWarps + q4_issuers(ntok) + kXWarps); }
-constexpr int q4_stages(int ntok) { return ntok == 256 ? 6 : 8; }
+// 64-input blocks a stage: handing one over costs about 300 clocks, more than
+// the products of 64 inputs where NTOK is small
+constexpr int q4_blocks(int ntok) { return ntok == 256 ? 1 : 2; }
+constexpr int q4_stages(int ntok) { return ntok == 256 ? 6 : 4; }
 __device__ unsigned int g_q4_wait_timeouts = 0;
 
 struct Q4TileParams {
@@ -263,10 +266,10 @@ struct Q4TileParams {
     bool tma;
 };
 
-constexpr int kTileCols = 512;  // of tensor memory: NTOK sums an issuer, 32 a stage of weights
+constexpr int kTileCols = 512;  // of tensor memory: NTOK sums an issuer, 32 a block of weights
 // one CTA an SM: two would want the same columns
 constexpr int q4_tile_smem(int ntok) {
-    const int ring = q4_stages(ntok) * ntok * 128;
+    const int ring = q4_stages(ntok) * q4_blocks(ntok) * ntok * 128;
     return ring < 116 * 1024 ? 116 * 1024 : ring;
 }
 
@@ -304,10 +307,10 @@ __device__ __forceinline__ void tile_sums(float* v, uint32_t at, int nk) {
 template <class A, int NTOK, bool G32>
 __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     q4_tiles_kernel(const Q4TileParams tp, const __grid_constant__ CUtensorMap map) {
-    constexpr int S = q4_stages(NTOK), STAGE = NTOK * 128;
+    constexpr int S = q4_stages(NTOK), KB = q4_blocks(NTOK), BLOCK = NTOK * 128, STAGE = KB * BLOCK;
     constexpr int ISS = q4_issuers(NTOK), WW = kWWarps, XW = WW + ISS;  // warps: weights 0 ..; products WW ..; x XW ..
     constexpr int WCOL = NTOK * ISS;                                     // first column of the weights
-    static_assert(WCOL + 32 * S <= kTileCols && S % kGroups == 0 && S % ISS == 0, "stages");
+    static_assert(WCOL + 32 * KB * S <= kTileCols && S % kGroups == 0 && S % ISS == 0, "stages");
     extern __shared__ __align__(1024) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[3 * S + 1];
     __shared__ uint32_t tmem_s;
@@ -317,13 +320,14 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int tile0 = blockIdx.x * 8, m0 = blockIdx.y * NTOK;
     const int share = tp.shares > 1 ? (int)cluster_rank() : 0;
-    const int kb0 = (int)((int64_t)g.kb * share / tp.shares), nk = (int)((int64_t)g.kb * (share + 1) / tp.shares) - kb0;
+    const int kb0 = (int)((int64_t)g.kb * share / tp.shares), nkb = (int)((int64_t)g.kb * (share + 1) / tp.shares) - kb0;
+    const int nk = (nkb + KB - 1) / KB;  // stages; the last one may have fewer blocks
     const uint32_t full_w = smem_addr(bars), full_x = full_w + 8 * S, empty = full_x + 8 * S, done = empty + 8 * S;
     if (warp == WW) t5_alloc(smem_addr(&tmem_s), kTileCols);
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
             bar_init(full_w + 8 * s, 8);
-            bar_init(full_x + 8 * s, 1);
+            bar_init(full_x + 8 * s, tp.tma ? 1 : kXWarps / S);
             bar_init(empty + 8 * s, 1);
         }
         bar_init(done, ISS);
@@ -342,17 +346,23 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
         const uint2* sp = p.sz + (int64_t)tile * g.ng * 8 + (lane >> 2);
         const uint32_t to = tmem + WCOL + ((uint32_t)(32 * (warp & 3) + 16 * (warp >> 2 & 1)) << 16);
         const int first = warp >> 3;
+        constexpr int AHEAD = kAhead / KB;  // stages
         uint4 w[kAhead];
         uint2 sz[kAhead][G32 ? 2 : 1];
-        const auto fetch = [&](int slot, int it) {
-            w[slot] = __ldcs(wp + it * 32);
+        const auto fetch_block = [&](int slot, int kb) {
+            w[slot] = __ldcs(wp + kb * 32);
 #pragma unroll
             for (int h = 0; h < (G32 ? 2 : 1); ++h) {
-                const int b = 2 * (kb0 + it) + h;
+                const int b = 2 * (kb0 + kb) + h;
                 int grp = p.gshift >= 0 ? b >> p.gshift : b / (g.group >> 5);
                 if (G32) grp = min(grp, g.ng - 1);
                 sz[slot][h] = __ldg(sp + grp * 8);
             }
+        };
+        const auto fetch = [&](int slot, int it) {
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+                if (it * KB + k < nkb) fetch_block(slot * KB + k, it * KB + k);
         };
         const auto weights = [&](uint32_t* v, int slot) {
             const uint32_t ww[4] = {w[slot].x, w[slot].y, w[slot].z, w[slot].w};
@@ -368,21 +378,25 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
         };
         int it = first, s = first, ph = 1;  // ph: parity of the wait for a free stage; the first round passes
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
+        for (int a = 0; a < AHEAD; ++a)
             if (it + a * kGroups < nk) fetch(a, it + a * kGroups);
         while (it < nk) {
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
+            for (int a = 0; a < AHEAD; ++a) {
                 if (it >= nk) break;
                 uint32_t v[16];
-                weights(v, a);
-                if (it + kAhead * kGroups < nk) fetch(a, it + kAhead * kGroups);
+                weights(v, a * KB);
                 if (!__all_sync(0xffffffffu, bar_wait(empty + 8 * s, ph, &gave_up))) {
                     it = nk;
                     break;
                 }
                 t5_after();
-                t5_st_16x256b_x4(to + 32 * s, v);
+                t5_st_16x256b_x4(to + 32 * KB * s, v);
+                if (KB == 2 && it * KB + 1 < nkb) {
+                    weights(v, a * KB + KB - 1);
+                    t5_st_16x256b_x4(to + 32 * KB * s + 32, v);
+                }
+                if (it + AHEAD * kGroups < nk) fetch(a, it + AHEAD * kGroups);
                 t5_wait_st();
                 t5_before();
                 __syncwarp();
@@ -408,7 +422,11 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
                 // K-major, 128-byte swizzle: 8 rows of 128 bytes 1024 bytes apart
                 const uint64_t b = (uint64_t)((smem_addr(ring) + s * STAGE) >> 4 & 0x3fffu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t5_mma_ts(d, tmem + WCOL + 32 * s + 8 * e, b + 2 * e, idesc, it >= ISS || e > 0);
+                for (int k = 0; k < KB; ++k)
+                    if (k == 0 || it * KB + k < nkb)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            t5_mma_ts(d, tmem + WCOL + 32 * (KB * s + k) + 8 * e, b + k * (BLOCK >> 4) + 2 * e, idesc, it >= ISS || k > 0 || e > 0);
                 t5_commit(empty + 8 * s);
             }
             __syncwarp();
@@ -421,8 +439,9 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
             int it = 0, s = 0, ph = 1;
             for (; it < nk; ++it) {
                 if (!bar_wait(empty + 8 * s, ph, &gave_up)) break;
-                bar_arrive_tx(full_x + 8 * s, STAGE);
-                tma_2d(smem_addr(ring) + s * STAGE, &map, (kb0 + it) * 64, m0, full_x + 8 * s);
+                const int n = min(KB, nkb - it * KB);
+                bar_arrive_tx(full_x + 8 * s, n * BLOCK);
+                for (int k = 0; k < n; ++k) tma_2d(smem_addr(ring) + s * STAGE + k * BLOCK, &map, (kb0 + it * KB + k) * 64, m0, full_x + 8 * s);
                 if (++s == S) s = 0, ph ^= 1;
             }
             // copies that nothing waits for any more still have to land before the CTA ends
@@ -433,18 +452,21 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
                 }
         }
     } else {
-        // a stage a warp: 8 values of a row a lane, in pieces of what x is aligned to
-        for (int it = warp - XW; it < nk; it += kXWarps) {
-            const int s = it % S;
+        // 8 values of a row a lane, in pieces of what x is aligned to. A warp
+        // has a stage of its own, so that it never waits for a round of it
+        // further ahead than the next: a barrier tells only two rounds apart.
+        const int s = (warp - XW) % S, part = (warp - XW) / S;
+        constexpr int PARTS = kXWarps / S;
+        for (int it = s; it < nk && part < PARTS; it += S) {
             if (!__all_sync(0xffffffffu, bar_wait(empty + 8 * s, (it / S & 1) ^ 1, &gave_up))) break;
             uint8_t* st = ring + s * STAGE;
-            const int k0 = (kb0 + it) * 64;
+            const int k0 = (kb0 + it * KB) * 64, values = min(KB, nkb - it * KB) * NTOK * 8;
 #pragma unroll 1
-            for (int i0 = lane; i0 < NTOK * 8; i0 += 32 * 4) {
+            for (int i0 = lane + 32 * 4 * part; i0 < values; i0 += 32 * 4 * PARTS) {
                 uint4 v[4];
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
-                    const int i = i0 + 32 * a, m = m0 + (i >> 3), k = k0 + 8 * (i & 7);
+                    const int i = i0 + 32 * a, m = m0 + (i >> 3) % NTOK, k = k0 + 64 * (i / (NTOK * 8)) + 8 * (i & 7);
                     v[a] = make_uint4(0, 0, 0, 0);
                     if (m < p.M && k < g.K) {
                         const uint16_t* x = p.x + m * p.xs + k;
@@ -576,8 +598,8 @@ cudaError_t q4_tiles_launch(const Q4TileParams& p, const CUtensorMap& map, cudaS
 }
 
 // Rows a tile and shares of K: the pair with the least estimated clocks of
-// the busiest SM: a 64-input stage costs 560 (NTOK = 256) or 300 (fewer), and
-// more where x is loaded by hand; a CTA 4000 to start and end, a joined one
+// the busiest SM: a 64-input block costs 560 (NTOK = 256), 290 or 220, and more
+// where x is loaded by hand; a CTA 4000 to start and end, a joined one
 // 1500 more.
 void q4_tiles_choose(const Q4Params& p, int* ntok, int* shares) {
     double best = 1e30;
@@ -586,7 +608,7 @@ void q4_tiles_choose(const Q4Params& p, int* ntok, int* shares) {
         for (int c = 1; c <= 8; c *= 2) {
             if (c > 1 && p.g.kb < 8 * c) break;
             const int64_t ctas = cdiv64(p.g.tiles, 8) * cdiv64(p.M, t) * c;
-            const double stage = (t <= 128 ? 300 : 560) * (p.vec8 ? 1.0 : p.vec2 ? 1 + t / 128.0 : 1 + t / 64.0);
+            const double stage = (t <= 64 ? 220 : t == 128 ? 290 : 560) * (p.vec8 ? 1.0 : p.vec2 ? 1 + t / 128.0 : 1 + t / 64.0);
             // clusters of one CTA an SM do not fill every GPC
             const double clocks = (double)cdiv64(ctas, c == 1 ? 148 : c == 2 ? 144 : c == 4 ? 136 : 128) * ((double)p.g.kb / c * stage + 4000 + (c > 1 ? 1500 : 0));
             if (clocks < best) best = clocks, *ntok = t, *shares = c;

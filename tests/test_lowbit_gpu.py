@@ -87,7 +87,10 @@ def linear_ref(d, x, k, group, kind):
     (5, 96, 48, 96, True, False), (8, 200, 130, 64, False, False), (9, 130, 70, 128, True, True), (16, 512, 512, 128, False, False),
     (17, 1000, 77, 32, True, True), (33, 257, 129, 128, True, False), (64, 640, 300, 64, False, True), (65, 64, 64, 32, True, False),
     (100, 1030, 257, 128, True, True), (129, 448, 128, 64, True, True), (300, 777, 511, 32, True, True), (513, 256, 1000, 128, False, False),
-    (1, 16384, 64, 128, True, False), (1, 120, 4096, 32, False, True)])
+    (1, 16384, 64, 128, True, False), (1, 120, 4096, 32, False, True),
+    # long rows that TMA cannot load, at every width of a tile: many rounds of its stages
+    (40, 4099, 200, 32, False, False), (60, 6002, 140, 128, True, False), (128, 5001, 130, 64, False, True), (260, 4098, 300, 128, True, True),
+    (1000, 3001, 1111, 64, False, False)])
 def test_linear(m, k, n, group, zeros, bias, kind):
     layer, d = linear_case(m * 7 + k, m, k, n, group, kind, zeros, bias)
     y = torch.full((m + 1, n), 7.0, device="cuda", dtype=TYPES[kind])
