@@ -137,6 +137,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
+    grid_wait();
+    grid_launch();
     bool looked = false;
     for (int n0 = 0; n0 < units; n0 += U * kRowThreads / W) {
         uint4 v[U][2];
@@ -199,6 +201,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
+    grid_wait();
+    grid_launch();
     kv_places(p, place);
     for (int n0 = 0; n0 < units; n0 += U * kRowThreads / W) {
         uint2 v[U][2];
@@ -257,14 +261,14 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
 }
 
 template <int W, int BITS, bool FP16, bool WRITE>
-void kv_launch(const KvRows& p, dim3 grid, cudaStream_t st) {
-    if (WRITE) kv_write_kernel<W, BITS, FP16><<<grid, kRowThreads, 0, st>>>(p);
-    else kv_read_kernel<W, BITS, FP16><<<grid, kRowThreads, 0, st>>>(p);
+cudaError_t kv_launch(const KvRows& p, dim3 grid, cudaStream_t st) {
+    if constexpr (WRITE) return launch(kv_write_kernel<W, BITS, FP16>, grid, kRowThreads, 0, st, true, p);
+    else return launch(kv_read_kernel<W, BITS, FP16>, grid, kRowThreads, 0, st, true, p);
 }
 template <int W, bool WRITE>
-void kv_width(const KvRows& p, bool fp16, dim3 grid, cudaStream_t st) {
-    if (p.g.bits == 8) fp16 ? kv_launch<W, 8, true, WRITE>(p, grid, st) : kv_launch<W, 8, false, WRITE>(p, grid, st);
-    else fp16 ? kv_launch<W, 4, true, WRITE>(p, grid, st) : kv_launch<W, 4, false, WRITE>(p, grid, st);
+cudaError_t kv_width(const KvRows& p, bool fp16, dim3 grid, cudaStream_t st) {
+    if (p.g.bits == 8) return fp16 ? kv_launch<W, 8, true, WRITE>(p, grid, st) : kv_launch<W, 8, false, WRITE>(p, grid, st);
+    return fp16 ? kv_launch<W, 4, true, WRITE>(p, grid, st) : kv_launch<W, 4, false, WRITE>(p, grid, st);
 }
 
 template <bool WRITE>
@@ -307,10 +311,8 @@ int kv_rows(const char* what, const bnn_kv_cache* c, const void* k, int64_t k_to
     const dim3 grid((unsigned)cdiv64(n_tokens, p.tpc));
     const cudaStream_t st = (cudaStream_t)stream;
     const bool fp16 = c->type == BNN_FP16;
-    if (W == 8) kv_width<8, WRITE>(p, fp16, grid, st);
-    else if (W == 16) kv_width<16, WRITE>(p, fp16, grid, st);
-    else kv_width<32, WRITE>(p, fp16, grid, st);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = W == 8 ? kv_width<8, WRITE>(p, fp16, grid, st) : W == 16 ? kv_width<16, WRITE>(p, fp16, grid, st)
+                                                                                   : kv_width<32, WRITE>(p, fp16, grid, st);
     return e == cudaSuccess ? BNN_OK : cuda_error(what, e);
 }
 

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstdlib>
 
 #include "../../include/bnn_lowbit.h"
 #include "common.h"
@@ -41,9 +42,50 @@ inline int no_device(const char* what) {
     return set_error(BNN_ERR_CUDA, "%s: the handle was made without a device", what);
 }
 inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// Kernels here are launched as programmatic dependents of what is before them
+// in the stream: they may start while it ends, and wait for it (grid_wait)
+// before they touch anything that another kernel can have written or still
+// reads. Every CTA waits, so that a kernel that has ended stands for all
+// before it. BNN_PDL=0 in the environment turns this off, as for the engine.
+inline bool pdl_on() {
+    static const bool on = [] {
+        const char* e = getenv("BNN_PDL");
+        return !(e && e[0] == '0');
+    }();
+    return on;
+}
+template <class K, class... Args>
+cudaError_t launch_cluster(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, bool early, int cluster_z, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (early && pdl_on()) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster_z > 0) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = at[n].val.clusterDim.y = 1;
+        at[n++].val.clusterDim.z = (unsigned)cluster_z;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <class K, class... Args>
+cudaError_t launch(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, bool early, const Args&... args) {
+    return launch_cluster(kernel, grid, threads, smem, st, early, 0, args...);
+}
 inline int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---------------------------------------------------------------- device side
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
 // (a & b) | c in one instruction (the compiler makes two of two constants)
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;

@@ -81,22 +81,24 @@ struct Q4Params {
 // at a time; 0 = value by value.
 constexpr int kQ4Warps = 8;
 
-template <int MT, int U, int SZ>
+// GM: what a scale covers: 0 = 32 inputs (or another odd multiple of 32), 1 = a
+// block of 64, 2 = a chunk of U blocks.
+template <int MT, int U, int GM>
 struct Q4Chunk {
     uint4 w[U][MT];
-    uint2 sz[U][MT][SZ];
+    uint2 sz[GM == 0 ? 2 * U : GM == 1 ? U : 1][MT];
 };
 
-template <class A, int NT, int MT, int U, bool G32, int X>
+template <class A, int NT, int MT, int U, int GM, int X>
 __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Params p) {
     extern __shared__ float red[];  // [warp][8 * NT][16 * MT + 1]
     constexpr int PITCH = 16 * MT + 1;
-    constexpr int SZ = G32 ? 2 : 1;  // scales a block
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be one number a warp
     const int r = lane >> 2, j = lane & 3;
     const int tile0 = blockIdx.x * MT, m0 = blockIdx.y * 8 * NT;
     const Q4Geo g = p.g;
+    grid_launch();
     // Whole chunks first, U blocks at a time, the warps in turn; the blocks
     // that are left over one at a time. A few blocks go one at a time, too.
     const int whole = g.kb >= U * warps ? g.kb / U : 0;
@@ -120,58 +122,64 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
         sr[i] = p.sz + (int64_t)tile * g.ng * 8 + r;
     }
     float acc[MT][NT][4] = {};
-    using Chunk = Q4Chunk<MT, U, SZ>;
+    using Chunk = Q4Chunk<MT, U, GM>;
     const auto fetch = [&](Chunk& c, int at, int count) {
 #pragma unroll
-        for (int u = 0; u < count; ++u) {
+        for (int i = 0; i < MT; ++i) {
+            const uint4* w = wr[i] + (int64_t)at * 32;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) c.w[u][i] = __ldcs(wr[i] + (at + u) * 32);
+            for (int u = 0; u < count; ++u) c.w[u][i] = __ldcs(w + u * 32);
+        }
 #pragma unroll
-            for (int h = 0; h < SZ; ++h) {
-                int grp = p.gshift >= 0 ? (2 * (at + u) + h) >> p.gshift : (2 * (at + u) + h) / (g.group >> 5);
-                if (G32) grp = min(grp, g.ng - 1);  // the second half of the last block may be padding alone
+        for (int h = 0; h < (GM == 0 ? 2 * count : GM == 1 ? count : 1); ++h) {
+            const int b = GM == 0 ? 2 * at + h : 2 * (at + h);  // 32-input block
+            int grp = p.gshift >= 0 ? b >> p.gshift : b / (g.group >> 5);
+            if (GM == 0) grp = min(grp, g.ng - 1);  // the second half of the last block may be padding alone
 #pragma unroll
-                for (int i = 0; i < MT; ++i) c.sz[u][i][h] = __ldg(sr[i] + grp * 8);
-            }
+            for (int i = 0; i < MT; ++i) c.sz[h][i] = __ldg(sr[i] + grp * 8);
         }
     };
     const auto multiply = [&](const Chunk& q, int at, int count) {
+        float c[MT][NT][4];
+        const uint16_t* xp[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) xp[t] = xr[t] + (int64_t)at * 64;
 #pragma unroll
         for (int u = 0; u < count; ++u) {
             uint2 xv[4][NT];
+            const int left = g.K - (at + u) * 64 - 4 * j;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint16_t* xp = xr[t] + (at + u) * 64;
-                const int left = g.K - (at + u) * 64 - 4 * j;
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (X == 2 || (X == 1 && e * 16 < left)) xv[e][t] = __ldg(reinterpret_cast<const uint2*>(xp + e * 16));
-                    else xv[e][t] = X == 0 ? load4(xp + e * 16, left - e * 16) : make_uint2(0, 0);
+                    const uint16_t* x = xp[t] + u * 64 + e * 16;
+                    if (X == 2 || (X == 1 && e * 16 < left)) xv[e][t] = __ldg(reinterpret_cast<const uint2*>(x));
+                    else xv[e][t] = X == 0 ? load4(x, left - e * 16) : make_uint2(0, 0);
                 }
-            }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const uint32_t w[4] = {q.w[u][i].x, q.w[u][i].y, q.w[u][i].z, q.w[u][i].w};
-                float c[NT][4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint2 sz = q.sz[u][i][G32 ? e >> 1 : 0];
+                    const uint2 sz = q.sz[GM == 0 ? 2 * u + (e >> 1) : GM == 1 ? u : 0][i];
                     const uint32_t z0 = __byte_perm(sz.y, 0, 0x1010), z1 = __byte_perm(sz.y, 0, 0x3232);
                     uint32_t a[4];
                     A::weights(a, w[e], z0, z1);
+                    const bool first = GM == 0 ? e % 2 == 0 : GM == 1 ? e == 0 : u == 0 && e == 0;
+                    const bool last = GM == 0 ? e % 2 == 1 : GM == 1 ? e == 3 : u == count - 1 && e == 3;
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        if (e == 0 || (G32 && e == 2)) A::mma0(c[t], a, xv[e][t].x, xv[e][t].y);
-                        else A::mma(c[t], a, xv[e][t].x, xv[e][t].y);
+                        if (first) A::mma0(c[i][t], a, xv[e][t].x, xv[e][t].y);
+                        else A::mma(c[i][t], a, xv[e][t].x, xv[e][t].y);
                     }
-                    if (e == 3 || (G32 && e == 1)) {
+                    if (last) {
                         const float2 s = A::unpack(sz.x);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            acc[i][t][0] = fmaf(s.x, c[t][0], acc[i][t][0]);
-                            acc[i][t][1] = fmaf(s.x, c[t][1], acc[i][t][1]);
-                            acc[i][t][2] = fmaf(s.y, c[t][2], acc[i][t][2]);
-                            acc[i][t][3] = fmaf(s.y, c[t][3], acc[i][t][3]);
+                            acc[i][t][0] = fmaf(s.x, c[i][t][0], acc[i][t][0]);
+                            acc[i][t][1] = fmaf(s.x, c[i][t][1], acc[i][t][1]);
+                            acc[i][t][2] = fmaf(s.y, c[i][t][2], acc[i][t][2]);
+                            acc[i][t][3] = fmaf(s.y, c[i][t][3], acc[i][t][3]);
                         }
                     }
                 }
@@ -181,7 +189,8 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     {
         Chunk c0, c1;
         const int step = warps * U;
-        if (n > 0) fetch(c0, kb, U);
+        if (n > 0) fetch(c0, kb, U);  // the weights are nobody's output: they need not wait
+        grid_wait();
         while (n > 0) {
             if (n > 1) fetch(c1, kb + step, U);
             multiply(c0, kb, U);
@@ -216,22 +225,26 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     }
 }
 
-template <class A, int NT, int MT, int U, bool G32, int X>
+template <class A, int NT, int MT, int U, int GM, int X>
 cudaError_t q4_launch(const Q4Params& p, cudaStream_t st) {
     const dim3 grid((unsigned)cdiv64(p.g.tiles, MT), (unsigned)cdiv64(p.M, 8 * NT));
     // warps of a CTA: as many as there are chunks, 4 where the tiles alone
     // give every SM several CTAs
     const int warps = p.g.kb < kQ4Warps ? p.g.kb : kQ4Warps;
-    q4_rows_kernel<A, NT, MT, U, G32, X><<<grid, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st>>>(p);
-    return cudaGetLastError();
+    return launch(q4_rows_kernel<A, NT, MT, U, GM, X>, grid, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st, true, p);
+}
+template <class A, int NT, int MT, int U, int GM>
+cudaError_t q4_forms(const Q4Params& p, cudaStream_t st) {
+    if (!p.vec4 || p.g.K % 4) return q4_launch<A, NT, MT, U, GM, 0>(p, st);
+    return p.g.K % 64 ? q4_launch<A, NT, MT, U, GM, 1>(p, st) : q4_launch<A, NT, MT, U, GM, 2>(p, st);
 }
 template <class A, int NT, int MT, int U>
-cudaError_t q4_forms(const Q4Params& p, cudaStream_t st) {
-    const int x = !p.vec4 || p.g.K % 4 ? 0 : p.g.K % 64 ? 1 : 2;
-    if (p.g.group % 64)
-        return x == 2 ? q4_launch<A, NT, MT, U, true, 2>(p, st) : x == 1 ? q4_launch<A, NT, MT, U, true, 1>(p, st) : q4_launch<A, NT, MT, U, true, 0>(p, st);
-    return x == 2 ? q4_launch<A, NT, MT, U, false, 2>(p, st) : x == 1 ? q4_launch<A, NT, MT, U, false, 1>(p, st) : q4_launch<A, NT, MT, U, false, 0>(p, st);
+cudaError_t q4_rows(const Q4Params& p, cudaStream_t st) {
+    if (p.g.group % 64) return q4_forms<A, NT, MT, U, 0>(p, st);
+    if (U == 1 || p.g.group % (64 * U)) return q4_forms<A, NT, MT, U, 1>(p, st);
+    return q4_forms<A, NT, MT, U, U == 1 ? 1 : 2>(p, st);
 }
+
 // ---------------------------------------------------------------- tiles on tcgen05
 // More rows: bound by the products. A CTA makes 128 outputs x NTOK rows of x
 // (of K, or of a cluster's share of K): D[output][row] in tensor memory. The
@@ -323,6 +336,7 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     const int kb0 = (int)((int64_t)g.kb * share / tp.shares), nkb = (int)((int64_t)g.kb * (share + 1) / tp.shares) - kb0;
     const int nk = (nkb + KB - 1) / KB;  // stages; the last one may have fewer blocks
     const uint32_t full_w = smem_addr(bars), full_x = full_w + 8 * S, empty = full_x + 8 * S, done = empty + 8 * S;
+    grid_launch();
     if (warp == WW) t5_alloc(smem_addr(&tmem_s), kTileCols);
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
@@ -338,6 +352,7 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     __syncthreads();
     t5_after();
     const uint32_t tmem = tmem_s;
+    if (warp >= WW) grid_wait();  // the weights need not wait for the kernels before
 
     if (warp < WW) {
         // 16 outputs a warp: lanes 32 * (warp % 4) + 16 * (warp / 4 % 2) of tensor memory
@@ -583,18 +598,8 @@ EncodeTiledFn encode_tiled() {
 
 template <class A, int NTOK, bool G32>
 cudaError_t q4_tiles_launch(const Q4TileParams& p, const CUtensorMap& map, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)cdiv64(p.q.g.tiles, 8), (unsigned)cdiv64(p.q.M, NTOK), (unsigned)p.shares);
-    cfg.blockDim = dim3(q4_tile_threads(NTOK));
-    cfg.dynamicSmemBytes = q4_tile_smem(NTOK);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = (unsigned)p.shares;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, q4_tiles_kernel<A, NTOK, G32>, p, map);
+    const dim3 grid((unsigned)cdiv64(p.q.g.tiles, 8), (unsigned)cdiv64(p.q.M, NTOK), (unsigned)p.shares);
+    return launch_cluster(q4_tiles_kernel<A, NTOK, G32>, grid, q4_tile_threads(NTOK), q4_tile_smem(NTOK), st, true, p.shares, p, map);
 }
 
 // Rows a tile and shares of K: the pair with the least estimated clocks of
@@ -652,8 +657,8 @@ cudaError_t q4_run(const Q4Params& p, cudaStream_t st) {
     // Two tiles a CTA share their loads of x, where there are tiles enough
     // for every SM. 8192 x 8192, one row: 11.6 us against 13.4 of one tile a
     // CTA; 4096 x 4096: 5.9 against 5.0.
-    if (p.M <= 8) return p.g.tiles >= 3 * 148 ? q4_forms<A, 1, 2, 2>(p, st) : q4_forms<A, 1, 1, 4>(p, st);
-    if (p.M <= 16) return q4_forms<A, 2, 2, 1>(p, st);
+    if (p.M <= 8) return p.g.tiles >= 3 * 148 ? q4_rows<A, 1, 2, 2>(p, st) : q4_rows<A, 1, 1, 4>(p, st);
+    if (p.M <= 16) return q4_rows<A, 2, 2, 1>(p, st);
     return p.g.group % 64 ? q4_tiles<A, true>(p, st) : q4_tiles<A, false>(p, st);
 }
 
