@@ -1,5 +1,6 @@
 // kv_cache.cu - the block-scaled key/value cache of include/bnn_lowbit.h:
 // create, write (quantise as it is stored) and read.
+#include <climits>
 #include <new>
 #include <utility>
 
@@ -15,7 +16,7 @@ struct KvRows {
     uint8_t* codes[2];    // keys, values
     uint16_t* scales[2];
     uint16_t* x[2];       // the caller's rows
-    int64_t token[2], head[2];
+    int token[2], head[2];  // strides
     int n_tokens, n_seqs, width;
     const int32_t *table, *start, *off;
     bool vec[2];
@@ -25,12 +26,16 @@ struct KvRows {
 
 constexpr int kRowThreads = 256, kMaxTpc = 32;
 
-// pages and places of the CTA's tokens, a warp each; page -1: none
-__device__ __forceinline__ void kv_places(const KvRows& p, int2* place) {
+// where head 0 of a token lies: bytes into the codes, scales; row -1: nowhere
+struct KvPlace {
+    int64_t row, scale;
+};
+// places of the CTA's tokens, a warp each
+__device__ __forceinline__ void kv_places(const KvRows& p, KvPlace* place) {
     const int lane = threadIdx.x & 31;
     for (int i = threadIdx.x >> 5; i < p.tpc; i += kRowThreads / 32) {
         const int t = blockIdx.x * p.tpc + i;
-        int2 at = make_int2(-1, 0);
+        KvPlace at = {-1, 0};
         if (t < p.n_tokens) {
             const int b = p.off ? kv_seq(p.off, p.n_seqs, t,
                                          [&](int lo, int step, int len) {
@@ -40,8 +45,11 @@ __device__ __forceinline__ void kv_places(const KvRows& p, int2* place) {
             if (b >= 0) {
                 const int64_t pos = (int64_t)p.start[b] + (p.off ? (int64_t)t - p.off[b] : 0);
                 if (pos >= 0 && pos <= 0x7fffffff) {
-                    at.x = kv_page(p.g, p.table + (int64_t)b * p.width, p.width, (int)pos);
-                    at.y = (int)pos & (p.g.pt - 1);
+                    const int page = kv_page(p.g, p.table + (int64_t)b * p.width, p.width, (int)pos);
+                    if (page >= 0) {
+                        at.row = kv_row(p.g, page, 0, (int)pos & (p.g.pt - 1));
+                        at.scale = kv_scale(p.g, page, 0, 0, (int)pos & (p.g.pt - 1));
+                    }
                 }
             }
         }
@@ -90,6 +98,7 @@ __device__ __forceinline__ bool kv_unit(const KvRows& p, int unit, int& local, i
 // within 2^-23 of max / top, which is at least 2^-16 away from any border of
 // bf16 (none can be hit: 127 or 7 times an odd number of 9 bits has more than
 // 11), so it rounds as the exact quotient does.
+constexpr uint32_t kWhole = 0x4b400000u;  // 0x1.8p23f: on it, a whole number is in the low bits of a float
 template <int BITS, bool FP16>
 __device__ __forceinline__ void kv_quantise(uint4 v, int lanes, uint32_t* code, uint16_t& scale) {
     constexpr int most = BITS == 8 ? 127 : 7;
@@ -111,7 +120,7 @@ __device__ __forceinline__ void kv_quantise(uint4 v, int lanes, uint32_t* code, 
     float s = __bfloat162float(sb);
     if (s >= 0x1p-100f) {
         float inv;
-        asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
 #pragma unroll
         for (int c = 0; c < 8; ++c) code[c] = __float_as_uint(__fadd_rn(__fadd_rn(__fmaf_rn(x[c], inv, grid), -grid), whole));
     } else {  // 1 / s may be out of range, and a subnormal scale far from max / top
@@ -120,23 +129,44 @@ __device__ __forceinline__ void kv_quantise(uint4 v, int lanes, uint32_t* code, 
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const float q = s > 0.0f && !bad ? rintf(__fdiv_rn(x[c], s)) : 0.0f;
-            code[c] = (uint32_t)((int)fminf(fmaxf(q, -(float)most), (float)most) + most + 1);
+            code[c] = kWhole + (uint32_t)((int)fminf(fmaxf(q, -(float)most), (float)most) + most + 1);
         }
     }
     scale = bad ? (uint16_t)0x7fff : *reinterpret_cast<const uint16_t*>(&sb);
 }
-// the low bytes of four words
-__device__ __forceinline__ uint32_t bytes4(const uint32_t* c) {
-    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+// N codes side by side, code c at bit c * log2(base). Each one stands on
+// kWhole, whose multiples drop out; multiply-adds, since the pipe of shifts
+// and masks is what bounds the write.
+template <int N, int STEP>
+__device__ __forceinline__ uint32_t side_by_side(const uint32_t* code, uint32_t base, uint32_t off) {
+    uint32_t w = code[(N - 1) * STEP];
+#pragma unroll
+    for (int c = N - 2; c >= 0; --c) asm("mad.lo.u32 %0, %0, %1, %2;" : "+r"(w) : "r"(base), "r"(code[c * STEP]));
+    return w - off;
+}
+constexpr uint32_t whole_sum(int n, int bits) {  // kWhole * (1 + 2^bits + ...), n terms
+    uint32_t s = 0;
+    for (int i = 0; i < n; ++i) s = (s << bits) + kWhole;
+    return s;
+}
+// a number that the compiler does not know, so that it does not make shifts of multiplications
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+    asm("mov.b32 %0, %0;" : "+r"(v));
+    return v;
 }
 
 template <int W, int BITS, bool FP16>
 __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
-    __shared__ int2 place[kMaxTpc];
+    __shared__ KvPlace place[kMaxTpc];
     constexpr int U = 2;
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
+    const int head_row = g.pt * g.row, head_scale = g.pt * g.ngp;  // from one head to the next
+    uint16_t* x0[2];  // this lane's numbers of head 0 of the CTA's first token
+#pragma unroll
+    for (int which = 0; which < 2; ++which) x0[which] = p.x[which] + (int64_t)blockIdx.x * p.tpc * p.token[which] + 8 * me.i;
+    const uint32_t base = opaque(BITS == 8 ? 256u : 16u);
     grid_wait();
     grid_launch();
     bool looked = false;
@@ -146,48 +176,42 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool in = kv_unit(p, n0 + (u * kRowThreads + threadIdx.x) / W, local[u], head[u]) && me.dim_left > 0;
-            const int64_t t = (int64_t)blockIdx.x * p.tpc + local[u];
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
                 v[u][which] = make_uint4(0, 0, 0, 0);
-                if (in) v[u][which] = load8(p.x[which] + t * p.token[which] + head[u] * p.head[which] + 8 * me.i, me.dim_left, p.vec[which]);
+                if (in) v[u][which] = load8(x0[which] + (int64_t)local[u] * p.token[which] + (int64_t)head[u] * p.head[which], me.dim_left, p.vec[which]);
             }
         }
         if (!looked) kv_places(p, place);
         looked = true;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int2 at = local[u] < p.tpc ? place[local[u]] : make_int2(-1, 0);
-            const bool store = at.x >= 0 && 8 * me.i < g.dp;
-            const int64_t slot = ((int64_t)at.x * g.heads + head[u]) * g.pt + at.y;
+            const KvPlace at = local[u] < p.tpc ? place[local[u]] : KvPlace{-1, 0};
+            const bool store = at.row >= 0 && 8 * me.i < g.dp;
+            const int64_t row_at = at.row + (int64_t)head[u] * head_row, scale_at = at.scale + (int64_t)head[u] * head_scale + me.grp;
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
                 uint32_t code[8];
                 uint16_t scale;
                 kv_quantise<BITS, FP16>(v[u][which], me.lanes, code, scale);
                 if (!store) continue;
-                if (me.owner) p.scales[which][slot * g.ngp + me.grp] = scale;
-                uint8_t* row = p.codes[which] + slot * g.row;
+                if (me.owner) p.scales[which][scale_at] = scale;
+                uint8_t* row = p.codes[which] + row_at;
                 if (BITS == 8) {
-                    const uint32_t a = bytes4(code), b = bytes4(code + 4);
+                    const uint32_t a = side_by_side<4, 1>(code, base, whole_sum(4, 8)), b = side_by_side<4, 1>(code + 4, base, whole_sum(4, 8));
                     if (which == 0) {
                         *reinterpret_cast<uint2*>(row + me.k_at) = make_uint2(a, b);
                     } else {
                         *reinterpret_cast<uint32_t*>(row + me.v_at) = a;
                         *reinterpret_cast<uint32_t*>(row + me.v_at + next) = b;
                     }
+                } else if (which == 0) {  // even numbers in the low half, odd ones in the high
+                    const uint32_t a = side_by_side<4, 2>(code, base, whole_sum(4, 4)), b = side_by_side<4, 2>(code + 1, base, whole_sum(4, 4));
+                    *reinterpret_cast<uint32_t*>(row + me.k_at) = __byte_perm(a, b, 0x5410);
                 } else {
-                    // bytes 0..3 and 4..7 to nibbles: keys pair (c, c + 1) in both halves, values in order
-                    const uint32_t a = bytes4(code) & 0x0f0f0f0fu, b = bytes4(code + 4) & 0x0f0f0f0fu;
-                    if (which == 0) {
-                        const uint32_t lo = __byte_perm(a, b, 0x6420), hi = __byte_perm(a, b, 0x7531);  // even, odd numbers
-                        *reinterpret_cast<uint32_t*>(row + me.k_at) =
-                            __byte_perm((lo | lo >> 4) & 0x00ff00ffu, (hi | hi >> 4) & 0x00ff00ffu, 0x6420);
-                    } else {
-                        const uint32_t c = (a | a >> 4) & 0x00ff00ffu, d = (b | b >> 4) & 0x00ff00ffu;
-                        *reinterpret_cast<uint16_t*>(row + me.v_at) = (uint16_t)__byte_perm(c, 0, 0x4420);
-                        *reinterpret_cast<uint16_t*>(row + me.v_at + next) = (uint16_t)__byte_perm(d, 0, 0x4420);
-                    }
+                    const uint32_t a = side_by_side<8, 1>(code, base, whole_sum(8, 4));
+                    *reinterpret_cast<uint16_t*>(row + me.v_at) = (uint16_t)a;
+                    *reinterpret_cast<uint16_t*>(row + me.v_at + next) = (uint16_t)(a >> 16);
                 }
             }
         }
@@ -196,11 +220,15 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
 
 template <int W, int BITS, bool FP16>
 __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
-    __shared__ int2 place[kMaxTpc];
+    __shared__ KvPlace place[kMaxTpc];
     constexpr int U = 2;
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
+    const int head_row = g.pt * g.row, head_scale = g.pt * g.ngp;  // from one head to the next
+    uint16_t* x0[2];  // this lane's numbers of head 0 of the CTA's first token
+#pragma unroll
+    for (int which = 0; which < 2; ++which) x0[which] = p.x[which] + (int64_t)blockIdx.x * p.tpc * p.token[which] + 8 * me.i;
     grid_wait();
     grid_launch();
     kv_places(p, place);
@@ -212,16 +240,16 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             in[u] = kv_unit(p, n0 + (u * kRowThreads + threadIdx.x) / W, local[u], head[u]) && me.dim_left > 0;
-            const int2 at = in[u] ? place[local[u]] : make_int2(-1, 0);
-            in[u] = at.x >= 0;
-            const int64_t slot = ((int64_t)at.x * g.heads + head[u]) * g.pt + at.y;
+            const KvPlace at = in[u] ? place[local[u]] : KvPlace{-1, 0};
+            in[u] = at.row >= 0;
+            const int64_t row_at = at.row + (int64_t)head[u] * head_row, scale_at = at.scale + (int64_t)head[u] * head_scale + me.grp;
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
                 v[u][which] = make_uint2(0, 0);
                 sc[u][which] = 0;
                 if (!in[u]) continue;
-                const uint8_t* row = p.codes[which] + slot * g.row;
-                sc[u][which] = p.scales[which][slot * g.ngp + me.grp];
+                const uint8_t* row = p.codes[which] + row_at;
+                sc[u][which] = p.scales[which][scale_at];
                 if (BITS == 8) {
                     if (which == 0) {
                         v[u][0] = *reinterpret_cast<const uint2*>(row + me.k_at);
@@ -254,8 +282,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
                 }
                 const uint4 o = make_uint4(pack2(x[0], x[1], FP16), pack2(x[2], x[3], FP16), pack2(x[4], x[5], FP16),
                                            pack2(x[6], x[7], FP16));
-                const int64_t t = (int64_t)blockIdx.x * p.tpc + local[u];
-                store8(p.x[which] + t * p.token[which] + head[u] * p.head[which] + 8 * me.i, o, me.dim_left, p.vec[which]);
+                store8(x0[which] + (int64_t)local[u] * p.token[which] + (int64_t)head[u] * p.head[which], o, me.dim_left, p.vec[which]);
             }
     }
 }
@@ -284,6 +311,8 @@ int kv_rows(const char* what, const bnn_kv_cache* c, const void* k, int64_t k_to
         if (!k || !v || !table || !start) return set_error(BNN_ERR_ARG, "%s: NULL argument", what);
         if (!aligned(k, 2) || !aligned(v, 2) || !aligned(table, 4) || !aligned(start, 4) || !aligned(off, 4))
             return set_error(BNN_ERR_ARG, "%s: an array is not aligned to its type", what);
+        for (int64_t st : {k_token, k_head, v_token, v_head})
+            if (st > INT_MAX || st < -INT_MAX) return set_error(BNN_ERR_ARG, "%s: a stride of 2^31 or more", what);
         if (!WRITE)  // rows of an output must not lie over one another
             for (const auto& s : {std::pair<int64_t, int64_t>(k_token, k_head), std::pair<int64_t, int64_t>(v_token, v_head)})
                 if ((g.heads > 1 && s.second < g.dim) || (n_tokens > 1 && s.first < g.dim))
@@ -298,7 +327,7 @@ int kv_rows(const char* what, const bnn_kv_cache* c, const void* k, int64_t k_to
     p.g = g;
     p.codes[0] = c->kc, p.codes[1] = c->vc, p.scales[0] = c->ks, p.scales[1] = c->vs;
     p.x[0] = (uint16_t*)k, p.x[1] = (uint16_t*)v;
-    p.token[0] = k_token, p.head[0] = k_head, p.token[1] = v_token, p.head[1] = v_head;
+    p.token[0] = (int)k_token, p.head[0] = (int)k_head, p.token[1] = (int)v_token, p.head[1] = (int)v_head;
     p.n_tokens = n_tokens, p.n_seqs = n_seqs, p.width = width;
     p.table = table, p.start = start, p.off = off;
     for (int w = 0; w < 2; ++w)

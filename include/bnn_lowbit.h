@@ -99,8 +99,8 @@ size_t bnn_kv_cache_bytes(const bnn_kv_cache *c); /* device memory it holds */
  * they share): which of the two is kept, code by code, is not defined. */
 
 /* Quantise keys and values as they are stored: k and v in the cache's type,
- * row t and head h at k + t * k_token + h * k_head (elements; the head_dim
- * numbers of a head are contiguous). */
+ * row t and head h at k + t * k_token + h * k_head (elements, below 2^31; the
+ * head_dim numbers of a head are contiguous). */
 int bnn_kv_cache_write(bnn_kv_cache *c, const void *d_k, int64_t k_token,
                        int64_t k_head, const void *d_v, int64_t v_token,
                        int64_t v_head, int n_tokens, int n_seqs,

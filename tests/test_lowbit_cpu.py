@@ -145,6 +145,8 @@ def test_cache_rows_refusals(name):
     for kw in ({"h": None}, {"tokens": -1}, {"seqs": -1}, {"width": -1}, {"k": None}, {"v": None}, {"table": None}, {"start": None},
                {"k": 17}, {"table": 18}, {"start": 18}, {"off": 18}, {"off": None}):
         refused(ARG, "bnn_kv_cache_" + name, *call(**kw))
+    for kw in ({"kt": 1 << 31}, {"vh": -(1 << 31)}):
+        refused(ARG, "stride", *call(**kw))
     refused(CUDA, "without a device", *call(off=None, tokens=2))
     refused(CUDA, "without a device", *call(tokens=0, k=None, v=None, table=None))
     for kw in ({"kh": 63}, {"vh": 0}, {"kt": 63}, {"vt": -64}):  # rows that lie over one another: in an output only
