@@ -56,6 +56,30 @@ __global__ void q4_layout_kernel(Q4Geo g, const uint8_t* codes, const uint16_t* 
     }
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// from the shared memory of CTA `rank` of the cluster
+__device__ __forceinline__ float ld_cluster1(uint32_t addr, uint32_t rank) {
+    uint32_t from;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(from));
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
+    uint32_t from;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(from));
+    return v;
+}
+
 struct Q4Params {
     Q4Geo g;
     const uint4* w;
@@ -66,6 +90,7 @@ struct Q4Params {
     uint16_t* y;
     int64_t ys;
     int M;
+    int shares;       // of K: CTAs of a cluster that make the same outputs
     int gshift;       // group = 32 << gshift, or -1
     bool vec2, vec4, vec8;  // rows of x start 4-byte, 8-byte, 16-byte aligned
 };
@@ -101,7 +126,9 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     grid_launch();
     // Whole chunks first, U blocks at a time, the warps in turn; the blocks
     // that are left over one at a time. A few blocks go one at a time, too.
-    const int whole = g.kb >= U * warps ? g.kb / U : 0;
+    const int share = p.shares > 1 ? (int)cluster_rank() : 0;
+    const int first = (int)((int64_t)g.kb * share / p.shares), blocks = (int)((int64_t)g.kb * (share + 1) / p.shares) - first;
+    const int whole = blocks >= U * warps ? blocks / U : 0;
     int n = whole > warp ? (whole - warp + warps - 1) / warps : 0;
     int kb = warp * U;
 
@@ -111,14 +138,14 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int m = m0 + t * 8 + r;
-        xr[t] = p.x + (m < p.M ? m * p.xs : 0) + 4 * j;
+        xr[t] = p.x + (m < p.M ? m * p.xs : 0) + (int64_t)first * 64 + 4 * j;
     }
     const uint4* wr[MT];
     const uint2* sr[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int tile = min(tile0 + i, g.tiles - 1);  // a tile behind the last repeats it, unused
-        wr[i] = p.w + (int64_t)tile * g.kb * 32 + lane;
+        wr[i] = p.w + ((int64_t)tile * g.kb + first) * 32 + lane;
         sr[i] = p.sz + (int64_t)tile * g.ng * 8 + r;
     }
     float acc[MT][NT][4] = {};
@@ -132,7 +159,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
         }
 #pragma unroll
         for (int h = 0; h < (GM == 0 ? 2 * count : GM == 1 ? count : 1); ++h) {
-            const int b = GM == 0 ? 2 * at + h : 2 * (at + h);  // 32-input block
+            const int b = GM == 0 ? 2 * (first + at) + h : 2 * (first + at + h);  // 32-input block
             int grp = p.gshift >= 0 ? b >> p.gshift : b / (g.group >> 5);
             if (GM == 0) grp = min(grp, g.ng - 1);  // the second half of the last block may be padding alone
 #pragma unroll
@@ -147,7 +174,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
 #pragma unroll
         for (int u = 0; u < count; ++u) {
             uint2 xv[4][NT];
-            const int left = g.K - (at + u) * 64 - 4 * j;
+            const int left = g.K - (first + at + u) * 64 - 4 * j;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -165,11 +192,11 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
                     const uint32_t z0 = __byte_perm(sz.y, 0, 0x1010), z1 = __byte_perm(sz.y, 0, 0x3232);
                     uint32_t a[4];
                     A::weights(a, w[e], z0, z1);
-                    const bool first = GM == 0 ? e % 2 == 0 : GM == 1 ? e == 0 : u == 0 && e == 0;
+                    const bool begins = GM == 0 ? e % 2 == 0 : GM == 1 ? e == 0 : u == 0 && e == 0;
                     const bool last = GM == 0 ? e % 2 == 1 : GM == 1 ? e == 3 : u == count - 1 && e == 3;
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        if (first) A::mma0(c[i][t], a, xv[e][t].x, xv[e][t].y);
+                        if (begins) A::mma0(c[i][t], a, xv[e][t].x, xv[e][t].y);
                         else A::mma(c[i][t], a, xv[e][t].x, xv[e][t].y);
                     }
                     if (last) {
@@ -201,7 +228,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
             kb += step;
             --n;
         }
-        for (kb = whole * U + warp; kb < g.kb; kb += warps) {
+        for (kb = whole * U + warp; kb < blocks; kb += warps) {
             fetch(c0, kb, 1);
             multiply(c0, kb, 1);
         }
@@ -214,24 +241,46 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
             for (int e = 0; e < 4; ++e)
                 red[(warp * 8 * NT + t * 8 + 2 * j + (e & 1)) * PITCH + 16 * i + r + 8 * (e >> 1)] = acc[i][t][e];
     __syncthreads();
-    for (int i = threadIdx.x; i < 128 * NT * MT; i += blockDim.x) {
+    const auto store = [&](int i, float v) {
         const int t = i / (16 * MT), o = i % (16 * MT), m = m0 + t, n = tile0 * 16 + o;
-        if (m >= p.M || n >= g.N) continue;
-        float v = 0.0f;
-        for (int k = 0; k < warps; ++k) v += red[(k * 8 * NT + t) * PITCH + o];
+        if (m >= p.M || n >= g.N) return;
         if (p.bias) v += p.bias[n];
         const typename A::T out = A::from_float(v);
         p.y[m * p.ys + n] = *reinterpret_cast<const uint16_t*>(&out);
+    };
+    const auto sum = [&](int i) {
+        float v = 0.0f;
+        for (int k = 0; k < warps; ++k) v += red[(k * 8 * NT + i / (16 * MT)) * PITCH + i % (16 * MT)];
+        return v;
+    };
+    if (p.shares == 1) {
+        for (int i = threadIdx.x; i < 128 * NT * MT; i += blockDim.x) store(i, sum(i));
+    } else {
+        // the CTAs of a cluster join their sums, a part of the outputs each, in the order of the shares
+        __shared__ float mine[128 * NT * MT];
+        for (int i = threadIdx.x; i < 128 * NT * MT; i += blockDim.x) mine[i] = sum(i);
+        cluster_sync();
+        const int part = 128 * NT * MT / p.shares;
+        for (int i = share * part + threadIdx.x; i < (share + 1) * part; i += blockDim.x) {
+            float v = 0.0f;
+            for (int r = 0; r < p.shares; ++r) v += ld_cluster1(smem_addr(mine + i), r);
+            store(i, v);
+        }
+        cluster_sync();  // nobody leaves while its sums are read
     }
 }
 
 template <class A, int NT, int MT, int U, int GM, int X>
 cudaError_t q4_launch(const Q4Params& p, cudaStream_t st) {
     const dim3 grid((unsigned)cdiv64(p.g.tiles, MT), (unsigned)cdiv64(p.M, 8 * NT));
-    // warps of a CTA: as many as there are chunks, 4 where the tiles alone
-    // give every SM several CTAs
-    const int warps = p.g.kb < kQ4Warps ? p.g.kb : kQ4Warps;
-    return launch(q4_rows_kernel<A, NT, MT, U, GM, X>, grid, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st, true, p);
+    // shares of K where the tiles do not give every SM a CTA, of 16 blocks at least
+    Q4Params q = p;
+    q.shares = 1;
+    while (q.shares < 8 && (int64_t)grid.x * grid.y * q.shares * 2 <= 148 && p.g.kb >= 32 * q.shares) q.shares *= 2;
+    const dim3 whole(grid.x, grid.y, (unsigned)q.shares);
+    const int warps = p.g.kb / q.shares < kQ4Warps ? p.g.kb / q.shares : kQ4Warps;
+    return launch_cluster(q4_rows_kernel<A, NT, MT, U, GM, X>, whole, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st, true,
+                          q.shares > 1 ? q.shares : 0, q);
 }
 template <class A, int NT, int MT, int U, int GM>
 cudaError_t q4_forms(const Q4Params& p, cudaStream_t st) {
@@ -275,7 +324,6 @@ __device__ unsigned int g_q4_wait_timeouts = 0;
 
 struct Q4TileParams {
     Q4Params q;
-    int shares;  // of K: CTAs of a cluster
     bool tma;
 };
 
@@ -284,23 +332,6 @@ constexpr int kTileCols = 512;  // of tensor memory: NTOK sums an issuer, 32 a b
 constexpr int q4_tile_smem(int ntok) {
     const int ring = q4_stages(ntok) * q4_blocks(ntok) * ntok * 128;
     return ring < 116 * 1024 ? 116 * 1024 : ring;
-}
-
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// from the shared memory of CTA `rank` of the cluster
-__device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
-    uint32_t from;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(from));
-    return v;
 }
 
 // 16 columns of this thread's lane, over the issuers
@@ -332,8 +363,8 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     const Q4Geo& g = p.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int tile0 = blockIdx.x * 8, m0 = blockIdx.y * NTOK;
-    const int share = tp.shares > 1 ? (int)cluster_rank() : 0;
-    const int kb0 = (int)((int64_t)g.kb * share / tp.shares), nkb = (int)((int64_t)g.kb * (share + 1) / tp.shares) - kb0;
+    const int share = p.shares > 1 ? (int)cluster_rank() : 0;
+    const int kb0 = (int)((int64_t)g.kb * share / p.shares), nkb = (int)((int64_t)g.kb * (share + 1) / p.shares) - kb0;
     const int nk = (nkb + KB - 1) / KB;  // stages; the last one may have fewer blocks
     const uint32_t full_w = smem_addr(bars), full_x = full_w + 8 * S, empty = full_x + 8 * S, done = empty + 8 * S;
     grid_launch();
@@ -515,7 +546,7 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     const int n = tile0 * 16 + 32 * (warp & 3) + lane;
     const int c0 = 16 * (warp >> 2);  // columns a warp: 16 of every 4 * WW
     constexpr int CSTEP = 4 * WW;
-    if (tp.shares == 1) {
+    if (p.shares == 1) {
         if (warp < WW && ok) {
             const float bias = p.bias && n < g.N ? p.bias[n] : 0.0f;
 #pragma unroll 1
@@ -547,12 +578,12 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
             }
         }
         cluster_sync();
-        const int mine = NTOK / tp.shares;
+        const int mine = NTOK / p.shares;
         for (int i = tid; i < mine * 32; i += q4_tile_threads(NTOK)) {
             const int c = share * mine + (i >> 5), o = 4 * (i & 31), m = m0 + c, out = tile0 * 16 + o;
             if (m >= p.M || out >= g.N) continue;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int r = 0; r < tp.shares; ++r) {
+            for (int r = 0; r < p.shares; ++r) {
                 const float4 x = ld_cluster(smem_addr(sums + c * 128 + o), r);
                 v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
             }
@@ -598,8 +629,8 @@ EncodeTiledFn encode_tiled() {
 
 template <class A, int NTOK, bool G32>
 cudaError_t q4_tiles_launch(const Q4TileParams& p, const CUtensorMap& map, cudaStream_t st) {
-    const dim3 grid((unsigned)cdiv64(p.q.g.tiles, 8), (unsigned)cdiv64(p.q.M, NTOK), (unsigned)p.shares);
-    return launch_cluster(q4_tiles_kernel<A, NTOK, G32>, grid, q4_tile_threads(NTOK), q4_tile_smem(NTOK), st, true, p.shares, p, map);
+    const dim3 grid((unsigned)cdiv64(p.q.g.tiles, 8), (unsigned)cdiv64(p.q.M, NTOK), (unsigned)p.q.shares);
+    return launch_cluster(q4_tiles_kernel<A, NTOK, G32>, grid, q4_tile_threads(NTOK), q4_tile_smem(NTOK), st, true, p.q.shares, p, map);
 }
 
 // Rows a tile and shares of K: the pair with the least estimated clocks of
@@ -626,7 +657,7 @@ cudaError_t q4_tiles(const Q4Params& p, cudaStream_t st) {
     Q4TileParams tp{};
     tp.q = p;
     int ntok = 32;
-    q4_tiles_choose(p, &ntok, &tp.shares);
+    q4_tiles_choose(p, &ntok, &tp.q.shares);
     CUtensorMap map{};
     EncodeTiledFn fn = p.vec8 ? encode_tiled() : nullptr;
     if (fn) {
@@ -658,7 +689,10 @@ cudaError_t q4_run(const Q4Params& p, cudaStream_t st) {
     // for every SM. 8192 x 8192, one row: 11.6 us against 13.4 of one tile a
     // CTA; 4096 x 4096: 5.9 against 5.0.
     if (p.M <= 8) return p.g.tiles >= 3 * 148 ? q4_rows<A, 1, 2, 2>(p, st) : q4_rows<A, 1, 1, 4>(p, st);
-    if (p.M <= 16) return q4_rows<A, 2, 2, 1>(p, st);
+    // 16 rows: reading x for every tile of 16 outputs is what costs in the
+    // rows' kernel, starting in the tiles'. 4096 x 4096: 9.0 us against 7.6,
+    // 4096 x 16384 18.2 against 15.6, 1024 x 1024 3.0 against 4.3.
+    if (p.M <= 16 && (int64_t)p.g.tiles * p.g.kb < 1 << 13) return q4_rows<A, 2, 2, 1>(p, st);
     return p.g.group % 64 ? q4_tiles<A, true>(p, st) : q4_tiles<A, false>(p, st);
 }
 
