@@ -706,21 +706,30 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
         const int seq = n / q_heads, qh = n % q_heads, head = qh / p.share;
         const int row = seq * p.share + qh % p.share;  // of the kv head's query rows
         float m = -INFINITY, l = 0.0f, acc[8] = {};
-        bool todo = true;
+        // on each side the item that the row is in, the row's place in it, and
+        // the CTAs that have its parts
+        int2 own[2];
+        int item[2], i[2];
+#pragma unroll
         for (int w = 0; w < 2; ++w) {
             const JoinSide& s = p.side[w];
+            own[w] = make_int2(0, -1), item[w] = i[w] = 0;
             if (!s.owners) continue;
-            // the item that the row is in, and the CTAs that have its parts
-            const int grp = row / s.rg, in = row % s.rg, i = in % s.R, item = (grp * p.heads + head) * s.rt + in / s.R;
-            const int2 own = (s.lengths ? s.lengths[grp] : s.length) > 0 && p.width[w] > 0 ? s.owners[item] : make_int2(0, -1);
-            todo = p.partial || own.x < own.y;  // else the attention kernel has finished this row itself
-            if (!todo) break;
+            const int grp = row / s.rg, in = row % s.rg;
+            i[w] = in % s.R, item[w] = (grp * p.heads + head) * s.rt + in / s.R;
+            const int2 got = s.owners[item[w]];  // not written where the length is 0
+            if ((s.lengths ? s.lengths[grp] : s.length) > 0 && p.width[w] > 0) own[w] = got;
+        }
+        if (!p.partial && own[0].x >= own[0].y) continue;  // the attention kernel has finished this row itself
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const JoinSide& s = p.side[w];
             // a lane reads the maximum and sum of a part, then all read its values
-            for (int c = own.x + warp; c <= own.y; c += 32 * kJoinWarps) {
+            for (int c = own[w].x + warp; c <= own[w].y; c += 32 * kJoinWarps) {
                 const int mine = c + lane * kJoinWarps;
-                const int64_t slot = own.x == own.y ? 2 * (int64_t)s.ctas + item : 2 * (int64_t)mine + (mine == own.x);
+                const int64_t slot = own[w].x == own[w].y ? 2 * (int64_t)s.ctas + item[w] : 2 * (int64_t)mine + (mine == own[w].x);
                 float2 ml = make_float2(-INFINITY, 0.0f);
-                if (mine <= own.y) ml = s.pml[slot * s.R + i];
+                if (mine <= own[w].y) ml = s.pml[slot * s.R + i[w]];
                 float top = ml.x;
                 for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 top = fmaxf(top, m);
@@ -733,12 +742,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
 #pragma unroll
                 for (int k = 0; k < 8; ++k) acc[k] *= a;
                 // (a part that saw nothing has left zeros)
-                const int parts = min(32, (own.y - c) / kJoinWarps + 1);
+                const int parts = min(32, (own[w].y - c) / kJoinWarps + 1);
 #pragma unroll 8
                 for (int q = 0; q < parts; ++q) {
                     const float f = __shfl_sync(0xffffffffu, b, q);
                     const int64_t from = __shfl_sync(0xffffffffu, slot, q);
-                    const float* x = s.pacc + (from * s.R + i) * p.dp + 4 * lane;
+                    const float* x = s.pacc + (from * s.R + i[w]) * p.dp + 4 * lane;
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
                         if (128 * k + 4 * lane < p.dp) {
@@ -749,7 +758,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
                 }
             }
         }
-        if (!todo) continue;
         if (lane == 0) wml[warp] = make_float2(m, l);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -884,12 +892,13 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
     if (rc) return rc;
     const KvGeo& g = c->geo;
     const bool prefix = prefix_tokens > 0;
-    if (table_pages < 0 || prefix_pages < 0 || !(scale - scale == 0.0f))
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (table_pages < 0 || prefix_pages < 0 || !(scale_log2 - scale_log2 == 0.0f))
         return set_error(BNN_ERR_ARG, "bnn_kv_attend: negative table width, or a scale that is not finite");
     if ((int64_t)table_pages * g.pt > INT_MAX - 256 || (int64_t)prefix_pages * g.pt > INT_MAX - 256)
         return set_error(BNN_ERR_ARG, "bnn_kv_attend: a table of 2^31 tokens or more");
     if (n_seqs > 0 && q_heads > INT_MAX / n_seqs) return set_error(BNN_ERR_ARG, "bnn_kv_attend: %d sequences of %d heads", n_seqs, q_heads);
-    if (((int64_t)n_seqs * table_pages + (prefix ? (int64_t)n_seqs * prefix_pages : 0)) * cdiv64(g.pt, kBlock) > INT_MAX / q_heads)
+    if (n_seqs * (cdiv64((int64_t)table_pages * g.pt, kBlock) + cdiv64(prefix_tokens, kBlock)) > INT_MAX / q_heads)
         return set_error(BNN_ERR_ARG, "bnn_kv_attend: %d sequences of up to %lld tokens are too many for one call", n_seqs,
                          (long long)table_pages * g.pt);
     if (prefix && (!d_prefix || (int64_t)prefix_pages * g.pt < prefix_tokens))
@@ -925,7 +934,7 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
     p.q_vec = aligned(d_q, 16) && (n_seqs == 1 || q_seq % 8 == 0) && (q_heads == 1 || q_head % 8 == 0);
     p.o_vec = aligned(d_out, 8) && (n_seqs == 1 || o_seq % 4 == 0) && (q_heads == 1 || o_head % 4 == 0);
     p.share = share;
-    p.scale_log2 = scale * 1.4426950408889634f;
+    p.scale_log2 = scale_log2;
     p.partial = prefix;
     JoinParams jp{};
     jp.rows = n_seqs * q_heads;

@@ -304,6 +304,7 @@ int kv_rows(const char* what, const bnn_kv_cache* c, const void* k, int64_t k_to
             const int32_t* start, const int32_t* off, void* stream) {
     if (!c || n_tokens < 0 || n_seqs < 0 || width < 0) return set_error(BNN_ERR_ARG, "%s: bad arguments", what);
     const KvGeo& g = c->geo;
+    if (n_tokens > (1 << 30)) return set_error(BNN_ERR_ARG, "%s: %d tokens: at most 2^30", what, n_tokens);
     if (!off && n_tokens != n_seqs)
         return set_error(BNN_ERR_ARG, "%s: %d tokens of %d sequences need offsets", what, n_tokens, n_seqs);
     const bool work = n_tokens > 0 && n_seqs > 0 && width > 0;

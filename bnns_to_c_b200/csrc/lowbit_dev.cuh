@@ -83,6 +83,8 @@ cudaError_t launch(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s
 inline int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---------------------------------------------------------------- device side
+// (What other kernels write is read by plain loads behind the wait: a
+// read-only load may be served, or moved, from before it.)
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 

@@ -127,7 +127,9 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     // Whole chunks first, U blocks at a time, the warps in turn; the blocks
     // that are left over one at a time. A few blocks go one at a time, too.
     const int share = p.shares > 1 ? (int)cluster_rank() : 0;
-    const int first = (int)((int64_t)g.kb * share / p.shares), blocks = (int)((int64_t)g.kb * (share + 1) / p.shares) - first;
+    // shares of whole chunks, which a scale may cover
+    const int64_t chunks = (g.kb + U - 1) / U;
+    const int first = (int)(chunks * share / p.shares) * U, blocks = min(g.kb, (int)(chunks * (share + 1) / p.shares) * U) - first;
     const int whole = blocks >= U * warps ? blocks / U : 0;
     int n = whole > warp ? (whole - warp + warps - 1) / warps : 0;
     int kb = warp * U;
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint16_t* x = xp[t] + u * 64 + e * 16;
-                    if (X == 2 || (X == 1 && e * 16 < left)) xv[e][t] = __ldg(reinterpret_cast<const uint2*>(x));
+                    if (X == 2 || (X == 1 && e * 16 < left)) xv[e][t] = *reinterpret_cast<const uint2*>(x);
                     else xv[e][t] = X == 0 ? load4(x, left - e * 16) : make_uint2(0, 0);
                 }
 #pragma unroll
@@ -518,7 +520,7 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
                         const uint16_t* x = p.x + m * p.xs + k;
                         if (p.vec2 && k + 8 <= g.K) {
                             const uint32_t* x2 = reinterpret_cast<const uint32_t*>(x);
-                            v[a] = make_uint4(__ldg(x2), __ldg(x2 + 1), __ldg(x2 + 2), __ldg(x2 + 3));
+                            v[a] = make_uint4(x2[0], x2[1], x2[2], x2[3]);
                         } else {
                             v[a] = load8(x, g.K - k, false);
                         }

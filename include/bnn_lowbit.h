@@ -98,7 +98,7 @@ size_t bnn_kv_cache_bytes(const bnn_kv_cache *c); /* device memory it holds */
  * not name a position of a page twice (two sequences writing into a page
  * they share): which of the two is kept, code by code, is not defined. */
 
-/* Quantise keys and values as they are stored: k and v in the cache's type,
+/* (n_tokens: at most 2^30.) Quantise keys and values as they are stored: k and v in the cache's type,
  * row t and head h at k + t * k_token + h * k_head (elements, below 2^31; the
  * head_dim numbers of a head are contiguous). */
 int bnn_kv_cache_write(bnn_kv_cache *c, const void *d_k, int64_t k_token,
@@ -126,7 +126,7 @@ int bnn_kv_cache_read(const bnn_kv_cache *c, void *d_k, int64_t k_token,
  * there (see above), a negative length counts as 0. A row that sees no
  * position gets zeros, and a log-sum of -infinity.
  * q and out: the cache's type, sequence b and head i at
- * q + b * q_seq + i * q_head. d_lse, unless NULL: float32 [n_seqs][q_heads],
+ * q + b * q_seq + i * q_head; they must not overlap. d_lse, unless NULL: float32 [n_seqs][q_heads],
  * the natural logarithm of sum_t exp(scale * q . key_t).
  * d_work: bnn_kv_attend_work(...) bytes of device memory, 16-byte aligned,
  * with any content, for this call alone until it has run: two calls (or two

@@ -142,7 +142,7 @@ def test_cache_rows_refusals(name):
     good = dict(h=h, k=16, kt=128, kh=64, v=16, vt=128, vh=64, tokens=5, seqs=2, table=16, width=3, start=16, off=16)
     call = lambda **kw: (fn, *{**good, **kw}.values(), None)  # noqa: E731
     refused(CUDA, "without a device", *call())
-    for kw in ({"h": None}, {"tokens": -1}, {"seqs": -1}, {"width": -1}, {"k": None}, {"v": None}, {"table": None}, {"start": None},
+    for kw in ({"h": None}, {"tokens": -1}, {"tokens": (1 << 30) + 1}, {"seqs": -1}, {"width": -1}, {"k": None}, {"v": None}, {"table": None}, {"start": None},
                {"k": 17}, {"table": 18}, {"start": 18}, {"off": 18}, {"off": None}):
         refused(ARG, "bnn_kv_cache_" + name, *call(**kw))
     for kw in ({"kt": 1 << 31}, {"vh": -(1 << 31)}):
@@ -169,7 +169,7 @@ def test_attend_refusals():
                      ({"heads": 0}, "multiple"), ({"pt": -1}, "bad"), ({"q": None}, "NULL"), ({"out": None}, "NULL"),
                      ({"lengths": None}, "NULL"), ({"table": None}, "NULL"), ({"q": 17}, "aligned"), ({"out": 17}, "aligned"),
                      ({"lse": 18}, "aligned"), ({"lengths": 18}, "aligned"), ({"width": -1}, "negative"), ({"pp": -1}, "negative"),
-                     ({"scale": float("nan")}, "finite"), ({"scale": float("inf")}, "finite"), ({"work": None}, "workspace"),
+                     ({"scale": float("nan")}, "finite"), ({"scale": float("inf")}, "finite"), ({"scale": 3e38}, "finite"), ({"work": None}, "workspace"),
                      ({"work": 24}, "workspace"), ({"bytes": need - 1}, "workspace"), ({"oh": 63}, "strides"), ({"os": 0}, "strides"),
                      ({"pt": 33, "pp": 1, "prefix": 16}, "prefix of 33"), ({"pt": 32, "pp": 1, "prefix": None}, "prefix"),
                      ({"width": 1 << 26}, "2\\^31"), ({"seqs": 16384, "width": (1 << 26) - 9, "bytes": 1 << 40}, "too many")):

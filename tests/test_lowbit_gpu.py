@@ -90,7 +90,9 @@ def linear_ref(d, x, k, group, kind):
     (1, 16384, 64, 128, True, False), (1, 120, 4096, 32, False, True),
     # long rows that TMA cannot load, at every width of a tile: many rounds of its stages
     (40, 4099, 200, 32, False, False), (60, 6002, 140, 128, True, False), (128, 5001, 130, 64, False, True), (260, 4098, 300, 128, True, True),
-    (1000, 3001, 1111, 64, False, False)])
+    (1000, 3001, 1111, 64, False, False),
+    # K shared out in a cluster, at borders that are not a group's
+    (1, 6464, 40, 256, True, False), (3, 4160, 16, 512, False, True), (12, 2176, 33, 128, True, True), (7, 8192, 100, 1024, True, False)])
 def test_linear(m, k, n, group, zeros, bias, kind):
     layer, d = linear_case(m * 7 + k, m, k, n, group, kind, zeros, bias)
     y = torch.full((m + 1, n), 7.0, device="cuda", dtype=TYPES[kind])
@@ -116,6 +118,32 @@ def test_linear_strides_and_alignment(m):
     again = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
     layer.run(d["x"], again)  # the aligned path
     assert torch.equal(again, wide[:, 5:5 + n])
+
+
+@pytest.mark.parametrize("m", [5, 18, 130])
+def test_linear_padded_rows(m):
+    """Rows of 200 of which 197 are x and the rest NaN, 16-byte aligned: what
+    is behind a row's end is not read, or not used."""
+    k, n = 197, 70
+    layer, d = linear_case(m, m, k, n, 32, "fp16", True, False)
+    x = torch.full((m, 200), float("nan"), device="cuda", dtype=torch.float16)
+    x[:, :k] = d["x"]
+    y = torch.empty(m, n, device="cuda", dtype=torch.float16)
+    layer.run(x[:, :k], y)
+    ref, tol = linear_ref(d, d["x"], k, 32, "fp16")
+    within(y, ref, tol)
+
+
+def test_linear_rows_far_apart():
+    """The second row of x and of y 2^31 bytes and more behind the first."""
+    k, n, far = 320, 64, (1 << 30) + 64
+    layer, d = linear_case(1, 2, k, n, 64, "bf16", True, True)
+    xs, ys = (torch.empty(far + 320, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    x, y = (t.as_strided((2, w), (far, 1)) for t, w in ((xs, k), (ys, n)))
+    x.copy_(d["x"])
+    layer.run(x, y)
+    ref, tol = linear_ref(d, d["x"], k, 64, "bf16")
+    within(y, ref, tol)
 
 
 @pytest.mark.parametrize("m", [6, 150])
@@ -603,6 +631,94 @@ def test_decode_step_against_the_definitions():
     step(s)
     torch.cuda.synchronize()
     step_ref(s, before)
+
+
+def test_steps_in_a_row_as_each_alone():
+    """Sixty steps without a wait between them, each reading what the one
+    before it has written, against the same steps with a wait after each
+    kernel: the kernels' early starts overlap nothing that they must not."""
+    s, t = step_state(80), step_state(80)
+    xs = [torch.randn(4, s["hidden"], device="cuda", generator=gen(90 + i)).to(torch.bfloat16) for i in range(60)]
+    outs = []
+    for v, waits in ((s, False), (t, True)):
+        got = [torch.empty_like(v["o"]) for _ in xs]
+        torch.cuda.synchronize()
+        for i, x in enumerate(xs):
+            v["x"].copy_(x)
+            v["lengths"].fill_(i % 50)
+            v["qkv"].run(v["x"], v["y"])
+            if waits:
+                torch.cuda.synchronize()
+            q, k, w = v["y"].unflatten(1, (-1, 64)).split((8, 2, 2), 1)
+            v["cache"].write(k, w, v["table"], v["lengths"])
+            if waits:
+                torch.cuda.synchronize()
+            v["len1"].copy_(v["lengths"] + 1)
+            v["cache"].attend(q, v["len1"], v["table"], v["a"], v["work"])
+            if waits:
+                torch.cuda.synchronize()
+            v["proj"].run(v["a"].flatten(1), v["o"])
+            v["proj"].run(v["a"].flatten(1), got[i])
+            v["x"].add_(v["o"])  # the next projection's input, from this one's output
+            v["qkv"].run(v["x"], v["y"])
+            if waits:
+                torch.cuda.synchronize()
+            got[i].add_(v["y"][:, :192])
+        torch.cuda.synchronize()
+        outs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_captured_attention_behind_a_prefix():
+    """Two graphs of one cache, each with a workspace of its own, replayed on
+    two streams at once on new queries."""
+    lengths = [70, 0, 400]
+    c, table, pre, held = filled(91, lengths, 2, 64, 8, 0, "fp16", 16, prefix=200)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    sides = []
+    for i in range(2):
+        q = torch.randn(3, 8, 64, device="cuda", generator=gen(i)).half()
+        out, work = torch.empty_like(q), torch.empty(c.attend_work(3, 8, 200), device="cuda", dtype=torch.uint8)
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            c.attend(q, n, table, out, work, prefix=pre, prefix_tokens=200, stream=torch.cuda.current_stream())
+        sides.append((g, q, out, work, st))
+    for turn in range(3):
+        for i, (g, q, out, work, st) in enumerate(sides):
+            q.copy_(torch.randn(3, 8, 64, device="cuda", generator=gen(10 * turn + i)).half())
+        torch.cuda.synchronize()
+        for g, q, out, work, st in sides:
+            with torch.cuda.stream(st):
+                for _ in range(5):
+                    g.replay()
+        torch.cuda.synchronize()
+        for g, q, out, work, st in sides:
+            r_out, _, t_out, _ = attend_ref(q, held, 0.125, "fp16")
+            within(out, r_out, t_out)
+
+
+def test_cache_beyond_four_gigabytes():
+    """Pages whose codes lie 2^32 bytes and more from the first."""
+    c = bn.KVCache(0, 34000, 64, 8, 256, bits=8, group=128, dtype="bf16")
+    assert c.nbytes > 2 * 2 ** 32
+    table = torch.tensor([[33999, 3, 33001], [33500, 20000, 1]], dtype=torch.int32, device="cuda")
+    lengths = [150, 131]
+    off, st = ragged(lengths)
+    x = [torch.randn(281, 8, 256, device="cuda", generator=gen(i)).to(torch.bfloat16) for i in (1, 2)]
+    c.write(*x, table, st, offsets=off)
+    got = [torch.empty_like(v) for v in x]
+    c.read(*got, table, st, offsets=off)
+    kv = [values(*quantise(v, 8, 128), 128) for v in x]
+    for v, y in zip(kv, got):
+        assert torch.equal(y, v.to(torch.bfloat16))
+    q = torch.randn(2, 8, 256, device="cuda", generator=gen(3)).to(torch.bfloat16)
+    out, lse = attend(c, q, lengths, table)
+    held = [tuple(v[a:b] for v in kv) for a, b in ((0, 150), (150, 281))]
+    r_out, r_lse, t_out, t_lse = attend_ref(q, held, 256 ** -0.5, "bf16")
+    within(out, r_out, t_out)
+    within(lse, r_lse, t_lse)
 
 
 def test_two_streams_at_once():
