@@ -158,7 +158,7 @@ __device__ __forceinline__ uint32_t opaque(uint32_t v) {
 template <int W, int BITS, bool FP16>
 __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
     __shared__ KvPlace place[kMaxTpc];
-    constexpr int U = 2;
+    constexpr int U = 1;
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
 template <int W, int BITS, bool FP16>
 __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
     __shared__ KvPlace place[kMaxTpc];
-    constexpr int U = 2;
+    constexpr int U = 1;
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
