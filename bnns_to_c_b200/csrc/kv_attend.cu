@@ -30,13 +30,8 @@ __host__ __device__ constexpr int attend_halves(int nt, int row) { return nt == 
 
 // CTAs of an attention kernel on an SM: as many as the registers allow, dp * nt
 // sums over a CTA's warps among them
-#ifndef OCC1
-#define OCC1 4
-#define OCC2 2
-#define OCC3 2
-#endif
 __host__ __device__ constexpr int attend_ctas(int dp, int nt) {
-    return dp * nt <= 128 ? OCC1 : dp * nt <= 256 ? OCC2 : OCC3;
+    return dp * nt <= 128 ? 4 : 2;
 }
 
 struct AttendParams {
@@ -184,6 +179,13 @@ __device__ __forceinline__ void load_scales(float* f, const uint16_t* at) {  // 
 
 // DP: head_dim rounded up; NT: tiles of 8 query rows; BPG: 32-blocks of
 // channels that share a scale (8: all).
+// The floor is the codes' bytes; decoding them holds it at 2.4 to 2.6 of an
+// SM's 4 instructions a clock, half of them bit operations and conversions, at
+// 16 warps of 127 registers an SM. 100003 tokens, 8 kv heads of 128 in 8 bits,
+// 32 query heads: 46 us with the join (4.5 TB/s of codes). 179457 tokens of 64
+// sequences, 64 query heads, in 4 bits and groups of 32: 82 us (2.6 TB/s). The
+// work is cut into one equal share a CTA, in blocks of tokens, whatever
+// sequence they belong to; what is cut is joined by join_kernel.
 template <int DP, int BITS, int NT, int BPG>
 __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kernel(const AttendParams p) {
     constexpr int NB = DP / 32, R = 8 * NT, ROW = DP * BITS / 8, CODES = kSub * ROW;

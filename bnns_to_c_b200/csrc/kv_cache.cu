@@ -60,8 +60,13 @@ __device__ __forceinline__ void kv_places(const KvRows& p, KvPlace* place) {
 
 // Both kernels: W = dp / 8 neighbouring lanes (32 for dp = 192) have one head
 // of one token, 8 numbers each: 16 bytes of the caller's row of keys and as
-// many of values, for two heads at a time. Bound by those rows' bytes: they
+// many of values, one such unit at a time: many resident warps hide the
+// loads better than more units a lane do (two at a time: 31.0 us against 28.8,
+// and 4.9 against 3.7 for one token each of 64 sequences). A write's loads
 // are on their way while the tokens' places are looked up.
+// 17828 tokens, 8 heads of 128, 4 bits, groups of 32: written in 29 us, read in
+// 23 (in a row of such launches): 3.2 and 4.1 TB/s. Bound by instructions
+// (3.0 and 2.7 a clock of an SM's 4), not yet by the bytes (14.5 us each).
 template <int W, int BITS>
 struct KvLane {
     int i, dim_left;      // numbers 8 * i .. of a head; how many of them there are from there on
@@ -158,7 +163,6 @@ __device__ __forceinline__ uint32_t opaque(uint32_t v) {
 template <int W, int BITS, bool FP16>
 __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
     __shared__ KvPlace place[kMaxTpc];
-    constexpr int U = 1;
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
@@ -170,49 +174,41 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
     grid_wait();
     grid_launch();
     bool looked = false;
-    for (int n0 = 0; n0 < units; n0 += U * kRowThreads / W) {
-        uint4 v[U][2];
-        int local[U], head[U];
+    for (int n0 = 0; n0 < units; n0 += kRowThreads / W) {
+        uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        int local, head;
+        if (kv_unit(p, n0 + threadIdx.x / W, local, head) && me.dim_left > 0)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = kv_unit(p, n0 + (u * kRowThreads + threadIdx.x) / W, local[u], head[u]) && me.dim_left > 0;
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                v[u][which] = make_uint4(0, 0, 0, 0);
-                if (in) v[u][which] = load8(x0[which] + (int64_t)local[u] * p.token[which] + (int64_t)head[u] * p.head[which], me.dim_left, p.vec[which]);
-            }
-        }
+            for (int which = 0; which < 2; ++which)
+                v[which] = load8(x0[which] + (int64_t)local * p.token[which] + (int64_t)head * p.head[which], me.dim_left, p.vec[which]);
         if (!looked) kv_places(p, place);
         looked = true;
+        const KvPlace at = local < p.tpc ? place[local] : KvPlace{-1, 0};
+        const bool store = at.row >= 0 && 8 * me.i < g.dp;
+        const int64_t row_at = at.row + (int64_t)head * head_row, scale_at = at.scale + (int64_t)head * head_scale + me.grp;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const KvPlace at = local[u] < p.tpc ? place[local[u]] : KvPlace{-1, 0};
-            const bool store = at.row >= 0 && 8 * me.i < g.dp;
-            const int64_t row_at = at.row + (int64_t)head[u] * head_row, scale_at = at.scale + (int64_t)head[u] * head_scale + me.grp;
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                uint32_t code[8];
-                uint16_t scale;
-                kv_quantise<BITS, FP16>(v[u][which], me.lanes, code, scale);
-                if (!store) continue;
-                if (me.owner) p.scales[which][scale_at] = scale;
-                uint8_t* row = p.codes[which] + row_at;
-                if (BITS == 8) {
-                    const uint32_t a = side_by_side<4, 1>(code, base, whole_sum(4, 8)), b = side_by_side<4, 1>(code + 4, base, whole_sum(4, 8));
-                    if (which == 0) {
-                        *reinterpret_cast<uint2*>(row + me.k_at) = make_uint2(a, b);
-                    } else {
-                        *reinterpret_cast<uint32_t*>(row + me.v_at) = a;
-                        *reinterpret_cast<uint32_t*>(row + me.v_at + next) = b;
-                    }
-                } else if (which == 0) {  // even numbers in the low half, odd ones in the high
-                    const uint32_t a = side_by_side<4, 2>(code, base, whole_sum(4, 4)), b = side_by_side<4, 2>(code + 1, base, whole_sum(4, 4));
-                    *reinterpret_cast<uint32_t*>(row + me.k_at) = __byte_perm(a, b, 0x5410);
+        for (int which = 0; which < 2; ++which) {
+            uint32_t code[8];
+            uint16_t scale;
+            kv_quantise<BITS, FP16>(v[which], me.lanes, code, scale);
+            if (!store) continue;
+            if (me.owner) p.scales[which][scale_at] = scale;
+            uint8_t* row = p.codes[which] + row_at;
+            if (BITS == 8) {
+                const uint32_t a = side_by_side<4, 1>(code, base, whole_sum(4, 8)), b = side_by_side<4, 1>(code + 4, base, whole_sum(4, 8));
+                if (which == 0) {
+                    *reinterpret_cast<uint2*>(row + me.k_at) = make_uint2(a, b);
                 } else {
-                    const uint32_t a = side_by_side<8, 1>(code, base, whole_sum(8, 4));
-                    *reinterpret_cast<uint16_t*>(row + me.v_at) = (uint16_t)a;
-                    *reinterpret_cast<uint16_t*>(row + me.v_at + next) = (uint16_t)(a >> 16);
+                    *reinterpret_cast<uint32_t*>(row + me.v_at) = a;
+                    *reinterpret_cast<uint32_t*>(row + me.v_at + next) = b;
                 }
+            } else if (which == 0) {  // even numbers in the low half, odd ones in the high
+                const uint32_t a = side_by_side<4, 2>(code, base, whole_sum(4, 4)), b = side_by_side<4, 2>(code + 1, base, whole_sum(4, 4));
+                *reinterpret_cast<uint32_t*>(row + me.k_at) = __byte_perm(a, b, 0x5410);
+            } else {
+                const uint32_t a = side_by_side<8, 1>(code, base, whole_sum(8, 4));
+                *reinterpret_cast<uint16_t*>(row + me.v_at) = (uint16_t)a;
+                *reinterpret_cast<uint16_t*>(row + me.v_at + next) = (uint16_t)(a >> 16);
             }
         }
     }
@@ -221,7 +217,6 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
 template <int W, int BITS, bool FP16>
 __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
     __shared__ KvPlace place[kMaxTpc];
-    constexpr int U = 1;
     const KvGeo& g = p.g;
     const KvLane<W, BITS> me(g);
     const int units = p.tpc * g.heads, next = kv_v_next<BITS>(g);
@@ -232,58 +227,50 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const KvRows p) {
     grid_wait();
     grid_launch();
     kv_places(p, place);
-    for (int n0 = 0; n0 < units; n0 += U * kRowThreads / W) {
-        uint2 v[U][2];
-        uint16_t sc[U][2];
-        int local[U], head[U];
-        bool in[U];
+    for (int n0 = 0; n0 < units; n0 += kRowThreads / W) {
+        int local, head;
+        if (!kv_unit(p, n0 + threadIdx.x / W, local, head) || me.dim_left <= 0) continue;
+        const KvPlace at = place[local];
+        if (at.row < 0) continue;
+        const int64_t row_at = at.row + (int64_t)head * head_row, scale_at = at.scale + (int64_t)head * head_scale + me.grp;
+        uint2 v[2];
+        uint16_t sc[2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            in[u] = kv_unit(p, n0 + (u * kRowThreads + threadIdx.x) / W, local[u], head[u]) && me.dim_left > 0;
-            const KvPlace at = in[u] ? place[local[u]] : KvPlace{-1, 0};
-            in[u] = at.row >= 0;
-            const int64_t row_at = at.row + (int64_t)head[u] * head_row, scale_at = at.scale + (int64_t)head[u] * head_scale + me.grp;
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                v[u][which] = make_uint2(0, 0);
-                sc[u][which] = 0;
-                if (!in[u]) continue;
-                const uint8_t* row = p.codes[which] + row_at;
-                sc[u][which] = p.scales[which][scale_at];
-                if (BITS == 8) {
-                    if (which == 0) {
-                        v[u][0] = *reinterpret_cast<const uint2*>(row + me.k_at);
-                    } else {
-                        v[u][1].x = *reinterpret_cast<const uint32_t*>(row + me.v_at);
-                        v[u][1].y = *reinterpret_cast<const uint32_t*>(row + me.v_at + next);
-                    }
-                } else if (which == 0) {
-                    v[u][0].x = *reinterpret_cast<const uint32_t*>(row + me.k_at);
+        for (int which = 0; which < 2; ++which) {
+            const uint8_t* row = p.codes[which] + row_at;
+            sc[which] = p.scales[which][scale_at];
+            v[which] = make_uint2(0, 0);
+            if (BITS == 8) {
+                if (which == 0) {
+                    v[0] = *reinterpret_cast<const uint2*>(row + me.k_at);
                 } else {
-                    v[u][1].x = *reinterpret_cast<const uint16_t*>(row + me.v_at) |
-                                (uint32_t)*reinterpret_cast<const uint16_t*>(row + me.v_at + next) << 16;
+                    v[1].x = *reinterpret_cast<const uint32_t*>(row + me.v_at);
+                    v[1].y = *reinterpret_cast<const uint32_t*>(row + me.v_at + next);
                 }
+            } else if (which == 0) {
+                v[0].x = *reinterpret_cast<const uint32_t*>(row + me.k_at);
+            } else {
+                v[1].x = *reinterpret_cast<const uint16_t*>(row + me.v_at) |
+                         (uint32_t)*reinterpret_cast<const uint16_t*>(row + me.v_at + next) << 16;
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int which = 0; which < 2; ++which) {
+            const float s = bf16_float(sc[which]), zero = -(8388608.0f + (BITS == 8 ? 128.0f : 8.0f));
+            uint32_t o[4];
 #pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                if (!in[u]) continue;
-                const float s = bf16_float(sc[u][which]);
-                float x[8];
+            for (int c = 0; c < 8; c += 2) {
+                // on 2^23 as a float; then 7 bits times 8: exact, rounded once below
+                uint32_t b[2];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    // on 2^23 as a float; then 7 bits times 8: exact, rounded once below
-                    uint32_t b;
-                    if (BITS == 8) b = __byte_perm(c < 4 ? v[u][which].x : v[u][which].y, 0x4b000000u, 0x7440 + (c & 3));
-                    else b = and_or(v[u][which].x >> (which ? 4 * c : 4 * (c >> 1) + 16 * (c & 1)), 15u, 0x4b000000u);
-                    x[c] = (__uint_as_float(b) - (8388608.0f + (BITS == 8 ? 128.0f : 8.0f))) * s;
-                }
-                const uint4 o = make_uint4(pack2(x[0], x[1], FP16), pack2(x[2], x[3], FP16), pack2(x[4], x[5], FP16),
-                                           pack2(x[6], x[7], FP16));
-                store8(x0[which] + (int64_t)local[u] * p.token[which] + (int64_t)head[u] * p.head[which], o, me.dim_left, p.vec[which]);
+                for (int e = 0; e < 2; ++e)
+                    if (BITS == 8) b[e] = __byte_perm(c < 4 ? v[which].x : v[which].y, 0x4b000000u, 0x7440 + (c & 3) + e);
+                    else b[e] = and_or(v[which].x >> (which ? 4 * (c + e) : 2 * c + 16 * e), 15u, 0x4b000000u);
+                const float2 x = apart(mul2(add2(both(__uint_as_float(b[0]), __uint_as_float(b[1])), both(zero, zero)), both(s, s)));
+                o[c / 2] = pack2(x.x, x.y, FP16);
             }
+            store8(x0[which] + (int64_t)local * p.token[which] + (int64_t)head * p.head[which], make_uint4(o[0], o[1], o[2], o[3]), me.dim_left, p.vec[which]);
+        }
     }
 }
 
@@ -334,7 +321,7 @@ int kv_rows(const char* what, const bnn_kv_cache* c, const void* k, int64_t k_to
     for (int w = 0; w < 2; ++w)
         p.vec[w] = aligned(p.x[w], 16) && (n_tokens == 1 || p.token[w] % 8 == 0) && (g.heads == 1 || p.head[w] % 8 == 0);
     const int W = g.dp == 64 ? 8 : g.dp == 128 ? 16 : 32;
-    // a CTA's two heads at a time: more tokens a CTA only where every SM has several CTAs
+    // four units a thread of a CTA, where every SM has several CTAs then
     p.tpc = 1;
     while (p.tpc < kMaxTpc && p.tpc * g.heads * W < 4 * kRowThreads && n_tokens / (2 * p.tpc) >= 8 * c->sms) p.tpc *= 2;
     p.head_magic = (uint32_t)((0x100000000ull + g.heads - 1) / g.heads);

@@ -96,10 +96,13 @@ struct Q4Params {
 };
 
 // ---------------------------------------------------------------- rows on mma.sync
-// Up to 16 rows: bound by reading the weights. A CTA makes MT tiles of 16
-// outputs for 8 * NT rows of x; its warps take chunks of U 64-input blocks in
-// turn and their sums are joined in shared memory. The weights of the next
-// chunk are on their way while one is multiplied: U * MT * 512 bytes a warp.
+// Few rows. A CTA makes MT tiles of 16 outputs for 8 * NT rows of x; its
+// warps take chunks of U 64-input blocks in turn and their sums are joined in
+// shared memory. The weights of the next chunk are on their way while one is
+// multiplied: U * MT * 512 bytes a warp. Bound by reading the weights and, as
+// much, by taking the codes apart (and-or, shift and subtract, 83 instructions
+// a 16 x 64 block). One row, launches in a row: 8192 x 8192 9.8 us (3.6 TB/s),
+// 4096 x 4096 4.0 us (2.2 TB/s), 512 x 512 1.6 us.
 // (q - z) is exact in 16 bits (|q - z| <= 15), so a group's sum of products
 // has only the rounding of 32-bit sums, and its scale is applied to that sum.
 // X: how x can be read: 2 = 8 bytes at a time, K a multiple of 64; 1 = 8 bytes
@@ -297,14 +300,18 @@ cudaError_t q4_rows(const Q4Params& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- tiles on tcgen05
-// More rows: bound by the products. A CTA makes 128 outputs x NTOK rows of x
-// (of K, or of a cluster's share of K): D[output][row] in tensor memory. The
-// weights are the A operand: eight warps turn codes into (q - z) * s in 16
-// bits and store them into tensor memory as they come from their word
-// (16x256b), so that shared memory carries x alone: B, 64 inputs a stage,
-// 128-byte swizzle, by TMA, or by four warps where x is not aligned for it.
-// One thread issues the products. With weights in shared memory, too, its
-// 128 bytes a clock would hold an NTOK = 256 tile to two thirds of the rate.
+// More rows. A CTA makes 128 outputs x NTOK rows of x (of K, or of a
+// cluster's share of K): D[output][row] in tensor memory. The weights are the
+// A operand: eight warps turn codes into (q - z) * s in 16 bits and store them
+// into tensor memory as they come from their word (16x256b), so that shared
+// memory carries x alone: B, 64 inputs a block, 128-byte swizzle, by TMA, or
+// by eight warps where x is not aligned for it. With weights in shared
+// memory, too, its 128 bytes a clock would hold an NTOK = 256 tile to two
+// thirds of the rate. 2048 rows, 4096 x 4096: 53 us alone (1.30 PFLOP/s), 64
+// in a long row of launches under the power cap (1.07; the 16-bit library
+// product of that shape 52 then); tensor pipe busy 71% of the time, the rest
+// the start and end of 256 CTAs in two rounds. 16 rows, 4096 x 16384: 15.6 us,
+// bound by taking the codes apart.
 // Rounding a weight to 16 bits costs 2^-9 (bf16; fp16 2^-12) of a product, as
 // much as the rounding of the result costs; the products' errors are
 // independent, so the result stays within sqrt(2) of its own rounding.
@@ -689,10 +696,10 @@ template <class A>
 cudaError_t q4_run(const Q4Params& p, cudaStream_t st) {
     // Two tiles a CTA share their loads of x, where there are tiles enough
     // for every SM. 8192 x 8192, one row: 11.6 us against 13.4 of one tile a
-    // CTA; 4096 x 4096: 5.9 against 5.0.
+    // CTA; 4096 x 4096: 5.9 against 5.0 (both before launches overlapped).
     if (p.M <= 8) return p.g.tiles >= 3 * 148 ? q4_rows<A, 1, 2, 2>(p, st) : q4_rows<A, 1, 1, 4>(p, st);
-    // 16 rows: reading x for every tile of 16 outputs is what costs in the
-    // rows' kernel, starting in the tiles'. 4096 x 4096: 9.0 us against 7.6,
+    // 9 to 16 rows: reading x for every tile of 16 outputs is what costs in the
+    // rows' kernel, starting in the tiles' (all 16 rows). 4096 x 4096: 9.0 us against 7.6,
     // 4096 x 16384 18.2 against 15.6, 1024 x 1024 3.0 against 4.3.
     if (p.M <= 16 && (int64_t)p.g.tiles * p.g.kb < 1 << 13) return q4_rows<A, 2, 2, 1>(p, st);
     return p.g.group % 64 ? q4_tiles<A, true>(p, st) : q4_tiles<A, false>(p, st);

@@ -49,12 +49,13 @@ int bnn_q4_layer_create(int device, int n_in, int n_out, int group, int type,
                         const uint8_t *zeros, const float *bias,
                         bnn_q4_layer **out);
 
-/* rows >= 0 vectors: x [rows] at a distance of x_stride elements (>= n_in)
- * -> y [rows] at y_stride (>= n_out), both in the layer's type, any
- * alignment of the type. x and y must not overlap. Up to 16 rows the codes
- * are multiplied exactly and a group's scale is applied to its 32-bit sum;
- * with more rows each weight (q - z) * s is rounded to the type first (tensor
- * memory operands), which adds half a step of the type to each product. */
+/* rows (0 .. 2^19) vectors: x [rows] at a distance of x_stride elements
+ * (>= n_in) -> y [rows] at y_stride (>= n_out), both in the layer's type, any
+ * alignment of the type. x and y must not overlap. Up to 8 rows, and up to 16
+ * in a layer of fewer than 2^23 weights, the codes are multiplied exactly and
+ * a group's scale is applied to its 32-bit sum; else each weight (q - z) * s
+ * is rounded to the type first (tensor memory operands), which adds half a
+ * step of the type to each product. */
 int bnn_q4_layer_run(const bnn_q4_layer *L, const void *d_x, int64_t x_stride,
                      int rows, void *d_y, int64_t y_stride, void *stream);
 void bnn_q4_layer_destroy(bnn_q4_layer *L);
@@ -98,9 +99,9 @@ size_t bnn_kv_cache_bytes(const bnn_kv_cache *c); /* device memory it holds */
  * not name a position of a page twice (two sequences writing into a page
  * they share): which of the two is kept, code by code, is not defined. */
 
-/* (n_tokens: at most 2^30.) Quantise keys and values as they are stored: k and v in the cache's type,
+/* Quantise keys and values as they are stored: k and v in the cache's type,
  * row t and head h at k + t * k_token + h * k_head (elements, below 2^31; the
- * head_dim numbers of a head are contiguous). */
+ * head_dim numbers of a head are contiguous). n_tokens: at most 2^30. */
 int bnn_kv_cache_write(bnn_kv_cache *c, const void *d_k, int64_t k_token,
                        int64_t k_head, const void *d_v, int64_t v_token,
                        int64_t v_head, int n_tokens, int n_seqs,
@@ -126,8 +127,9 @@ int bnn_kv_cache_read(const bnn_kv_cache *c, void *d_k, int64_t k_token,
  * there (see above), a negative length counts as 0. A row that sees no
  * position gets zeros, and a log-sum of -infinity.
  * q and out: the cache's type, sequence b and head i at
- * q + b * q_seq + i * q_head; they must not overlap. d_lse, unless NULL: float32 [n_seqs][q_heads],
- * the natural logarithm of sum_t exp(scale * q . key_t).
+ * q + b * q_seq + i * q_head; they must not overlap. d_lse, unless NULL:
+ * float32 [n_seqs][q_heads], the natural logarithm of
+ * sum_t exp(scale * q . key_t).
  * d_work: bnn_kv_attend_work(...) bytes of device memory, 16-byte aligned,
  * with any content, for this call alone until it has run: two calls (or two
  * captured graphs) that may overlap need one each. q_heads is a multiple of

@@ -68,15 +68,15 @@ def linear_weights(d, k, group):
 
 
 def linear_ref(d, x, k, group, kind):
-    """Result and bound. Beside the sums: in the many-row kernel a weight
-    (q - z) * s is rounded to the type before it is multiplied, h * |x w| a
-    term."""
+    """Result and bound. Beside the sums: with more than 8 rows a weight
+    (q - z) * s may be rounded to the type before it is multiplied, h * |x w|
+    a term."""
     w = linear_weights(d, k, group)
     ref = x.double() @ w.T
     size = x.double().abs() @ w.abs().T
     if d["bias"] is not None:
         ref, size = ref + d["bias"].double(), size + d["bias"].double().abs()
-    h = torch.finfo(TYPES[kind]).eps / 2 if x.shape[0] > 1 else 0.0
+    h = torch.finfo(TYPES[kind]).eps / 2 if x.shape[0] > 8 else 0.0
     tol = size * (2 * (k + 64) * U + h)
     return ref, tol + rounding(ref.abs() + tol, TYPES[kind])
 
