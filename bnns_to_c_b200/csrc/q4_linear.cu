@@ -310,7 +310,7 @@ cudaError_t q4_rows(const Q4Params& p, cudaStream_t st) {
 // thirds of the rate. 2048 rows, 4096 x 4096: 53 us alone (1.30 PFLOP/s), 64
 // in a long row of launches under the power cap (1.07; the 16-bit library
 // product of that shape 52 then); tensor pipe busy 71% of the time, the rest
-// the start and end of 256 CTAs in two rounds. 16 rows, 4096 x 16384: 15.6 us,
+// the start and end of 256 CTAs in two rounds. 16 rows, 4096 to 16384: 15.6 us,
 // bound by taking the codes apart.
 // Rounding a weight to 16 bits costs 2^-9 (bf16; fp16 2^-12) of a product, as
 // much as the rounding of the result costs; the products' errors are
