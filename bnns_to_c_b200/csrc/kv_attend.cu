@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 #pragma unroll
                 for (int c = 0; c < 4; ++c) h[c] = pack2(x[2 * c] * up, x[2 * c + 1] * up, true);
                 if (lane < DP / 8) qf[((lane >> 2) * NT + (i >> 3)) * 32 + (i & 7) * 4 + (lane & 3)] = make_uint4(h[0], h[1], h[2], h[3]);
-                if (lane == 0) factor[i] = p.scale_log2 * __int_as_float((127 - sh) << 23);
+                // a row with an infinity or a NaN has only infinite scores and NaN: its softmax is NaN
+                if (lane == 0) factor[i] = e == 255 ? NAN : p.scale_log2 * __int_as_float((127 - sh) << 23);
             }
         }
         __syncthreads();

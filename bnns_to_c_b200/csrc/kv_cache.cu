@@ -76,10 +76,9 @@ struct KvLane {
     __device__ __forceinline__ explicit KvLane(const KvGeo& g) {
         i = threadIdx.x % W;
         dim_left = g.dim - 8 * i;
-        const int per = g.ng == 1 ? W : g.group / 8;  // a power of two
-        lanes = per;
-        grp = i / per;
-        owner = i % per == 0 && grp < g.ng;
+        lanes = g.ng == 1 ? W : g.group / 8;  // a power of two, 4 at least
+        grp = i >> (31 - __clz(lanes));
+        owner = (i & (lanes - 1)) == 0 && grp < g.ng;
         k_at = kv_k_at(g, i), v_at = kv_v_at(g, 2 * i);
     }
 };
@@ -104,13 +103,21 @@ __device__ __forceinline__ bool kv_unit(const KvRows& p, int unit, int& local, i
 // bf16 (none can be hit: 127 or 7 times an odd number of 9 bits has more than
 // 11), so it rounds as the exact quotient does.
 constexpr uint32_t kWhole = 0x4b400000u;  // 0x1.8p23f: on it, a whole number is in the low bits of a float
-template <int BITS, bool FP16>
+template <int W, int BITS, bool FP16>
 __device__ __forceinline__ void kv_quantise(uint4 v, int lanes, uint32_t* code, uint16_t& scale) {
     constexpr int most = BITS == 8 ? 127 : 7;
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     // |x| as bits, two at a time: an order that puts NaN above infinity above all numbers
     uint32_t big = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-    for (int s = 1; s < lanes; s <<= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, s));
+    const auto over = [&](int s) { big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, s)); };
+    over(1), over(2);
+    if (lanes > 4) {
+        over(4);
+        if (W > 8 && lanes > 8) {
+            over(8);
+            if (W > 16 && lanes > 16) over(16);
+        }
+    }
     big = max(big & 0xffffu, big >> 16);
     const bool bad = big >= (FP16 ? 0x7c00u : 0x7f80u);
     const float top = bad ? 0.0f : unpack2(big, FP16).x;
@@ -190,7 +197,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRows p) {
         for (int which = 0; which < 2; ++which) {
             uint32_t code[8];
             uint16_t scale;
-            kv_quantise<BITS, FP16>(v[which], me.lanes, code, scale);
+            kv_quantise<W, BITS, FP16>(v[which], me.lanes, code, scale);
             if (!store) continue;
             if (me.owner) p.scales[which][scale_at] = scale;
             uint8_t* row = p.codes[which] + row_at;

@@ -55,7 +55,7 @@ int bnn_q4_layer_create(int device, int n_in, int n_out, int group, int type,
  * in a layer of fewer than 2^23 weights, the codes are multiplied exactly and
  * a group's scale is applied to its 32-bit sum; else each weight (q - z) * s
  * is rounded to the type first (tensor memory operands), which adds half a
- * step of the type to each product. */
+ * step of the type to each product, and has to be in the type's range. */
 int bnn_q4_layer_run(const bnn_q4_layer *L, const void *d_x, int64_t x_stride,
                      int rows, void *d_y, int64_t y_stride, void *stream);
 void bnn_q4_layer_destroy(bnn_q4_layer *L);
@@ -125,7 +125,9 @@ int bnn_kv_cache_read(const bnn_kv_cache *c, void *d_k, int64_t k_token,
  * are d_prefix[0 ..] (prefix_tokens = 0: none). The prefix is read once for
  * the whole batch, not once per sequence. Positions without a page are not
  * there (see above), a negative length counts as 0. A row that sees no
- * position gets zeros, and a log-sum of -infinity.
+ * position gets zeros, and a log-sum of -infinity. A NaN in a key, value or
+ * query (in a query an infinity, too) makes NaN of what depends on it, and of
+ * nothing else.
  * q and out: the cache's type, sequence b and head i at
  * q + b * q_seq + i * q_head; they must not overlap. d_lse, unless NULL:
  * float32 [n_seqs][q_heads], the natural logarithm of

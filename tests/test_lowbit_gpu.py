@@ -494,6 +494,32 @@ def test_attend_only_nan_is_not_empty():
     assert out.isnan().all() and lse.isnan().all()
 
 
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_attend_query_that_is_not_finite(bad, prefix):
+    """Its scores are infinities of one sign at best: the softmax is NaN, in
+    that row alone; one that sees nothing is still empty."""
+    c = bn.KVCache(0, 8, 16, 1, 64, bits=8, dtype="bf16")
+    x = torch.rand(80, 1, 64, device="cuda", generator=gen(1)).to(torch.bfloat16) + 0.5
+    own, pre = (torch.arange(a, b, dtype=torch.int32, device="cuda") for a, b in ((0, 5), (5, 8)))
+    for pages, n in ((own, 80), (pre, 40)):
+        c.write(x[:n], x[:n], pages[None], torch.zeros(1, dtype=torch.int32, device="cuda"),
+                offsets=torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    q = torch.randn(2, 4, 64, device="cuda", generator=gen(2)).to(torch.bfloat16)
+    table, args = own[None].repeat(2, 1), (pre, prefix) if prefix else ()
+    base, base_lse = attend(c, q, [80, 0], table, *args)
+    q[:, 2, 7] = bad
+    out, lse = attend(c, q, [80, 0], table, *args)
+    for b in range(2):
+        for i in range(4):
+            if i == 2 and (b == 0 or prefix):
+                assert out[b, i].isnan().all() and lse[b, i].isnan()
+            else:
+                assert torch.equal(out[b, i], base[b, i]) and lse[b, i] == base_lse[b, i]
+    if not prefix:
+        assert (out[1] == 0).all() and (lse[1] == -math.inf).all()
+
+
 def test_attend_missing_pages_and_odd_lengths():
     """Positions without a page are not there: in the middle, at the end,
     behind the table, in the prefix; a negative length is an empty one."""
