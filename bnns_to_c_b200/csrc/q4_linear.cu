@@ -15,6 +15,9 @@ struct bnn_q4_layer {
     const uint32_t* codes;   //   q4_words
     const uint2* sz;         //   q4_scales / 2 times: scales and zero points of two rows
     const float* bias;       //   [n_out] or nullptr
+    int mt;                  // for up to 8 rows: tiles of 16 outputs a CTA,
+    int shares8;             //   CTAs that share K; for 9 to 16
+    int shares16;
 };
 
 namespace bnn {
@@ -91,6 +94,7 @@ struct Q4Params {
     int64_t ys;
     int M;
     int shares;       // of K: CTAs of a cluster that make the same outputs
+    int mt;           // tiles of 16 outputs a CTA, up to 8 rows
     int gshift;       // group = 32 << gshift, or -1
     bool vec2, vec4, vec8;  // rows of x start 4-byte, 8-byte, 16-byte aligned
 };
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be one number a warp
     const int r = lane >> 2, j = lane & 3;
-    const int tile0 = blockIdx.x * MT, m0 = blockIdx.y * 8 * NT;
+    const int tile0 = blockIdx.x * MT;
     const Q4Geo g = p.g;
     grid_launch();
     // Whole chunks first, U blocks at a time, the warps in turn; the blocks
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     const uint16_t* xr[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int m = m0 + t * 8 + r;
+        const int m = t * 8 + r;
         xr[t] = p.x + (m < p.M ? m * p.xs : 0) + (int64_t)first * 64 + 4 * j;
     }
     const uint4* wr[MT];
@@ -247,7 +251,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
                 red[(warp * 8 * NT + t * 8 + 2 * j + (e & 1)) * PITCH + 16 * i + r + 8 * (e >> 1)] = acc[i][t][e];
     __syncthreads();
     const auto store = [&](int i, float v) {
-        const int t = i / (16 * MT), o = i % (16 * MT), m = m0 + t, n = tile0 * 16 + o;
+        const int m = i / (16 * MT), o = i % (16 * MT), n = tile0 * 16 + o;
         if (m >= p.M || n >= g.N) return;
         if (p.bias) v += p.bias[n];
         const typename A::T out = A::from_float(v);
@@ -265,8 +269,8 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
         __shared__ float mine[128 * NT * MT];
         for (int i = threadIdx.x; i < 128 * NT * MT; i += blockDim.x) mine[i] = sum(i);
         cluster_sync();
-        const int part = 128 * NT * MT / p.shares;
-        for (int i = share * part + threadIdx.x; i < (share + 1) * part; i += blockDim.x) {
+        const int part = (128 * NT * MT + p.shares - 1) / p.shares, end = min(128 * NT * MT, (share + 1) * part);
+        for (int i = share * part + threadIdx.x; i < end; i += blockDim.x) {
             float v = 0.0f;
             for (int r = 0; r < p.shares; ++r) v += ld_cluster1(smem_addr(mine + i), r);
             store(i, v);
@@ -275,17 +279,36 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     }
 }
 
+// CTAs in clusters of c that run at a time with one on each SM: clusters do not fill every GPC
+constexpr int kAtOnce[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+
+// Shares of K (of 16 blocks at least) for tiles of MT: the ones with the
+// least estimated time. Two CTAs run on an SM; a warp's chunk costs 1.05 us
+// where they do not, 1.3 (MT = 1) or 1.1 (MT = 2) where they do: it waits for
+// memory. Blocks too few for a chunk for each warp go one at a time. A join
+// costs 1.2 us. One row, 8192 x 1024: 2 shares 4.4 us, 4 shares 3.7; 16384 x
+// 2048: 1 share 10.1, 2 shares 7.5; 4096 x 1024: 1 share 3.0, 2 shares 3.2.
+double q4_rows_shares(const Q4Geo& g, int mt, int chunk_blocks, int* shares) {
+    double best = 1e30;
+    for (int c = 1; c <= 8; ++c) {
+        if (c > 1 && g.kb < 16 * c) break;
+        const int64_t ctas = cdiv64(g.tiles, mt) * c;
+        const int blocks = (g.kb + c - 1) / c;
+        const double chunk = ctas <= 148 ? 1.05 : mt == 1 ? 1.3 : 1.1;
+        const bool alone = chunk_blocks == 1 || blocks < kQ4Warps * chunk_blocks;
+        const double rounds = alone ? 0.6 * cdiv64(blocks, kQ4Warps) : chunk * cdiv64(blocks, kQ4Warps * chunk_blocks);
+        const double us = 0.8 + (double)cdiv64(ctas, 2 * kAtOnce[c]) * (0.6 + rounds) + (c > 1 ? 1.2 : 0.0);
+        if (us < best) best = us, *shares = c;
+    }
+    return best;
+}
+
 template <class A, int NT, int MT, int U, int GM, int X>
 cudaError_t q4_launch(const Q4Params& p, cudaStream_t st) {
-    const dim3 grid((unsigned)cdiv64(p.g.tiles, MT), (unsigned)cdiv64(p.M, 8 * NT));
-    // shares of K where the tiles do not give every SM a CTA, of 16 blocks at least
-    Q4Params q = p;
-    q.shares = 1;
-    while (q.shares < 8 && (int64_t)grid.x * grid.y * q.shares * 2 <= 148 && p.g.kb >= 32 * q.shares) q.shares *= 2;
-    const dim3 whole(grid.x, grid.y, (unsigned)q.shares);
-    const int warps = p.g.kb / q.shares < kQ4Warps ? p.g.kb / q.shares : kQ4Warps;
-    return launch_cluster(q4_rows_kernel<A, NT, MT, U, GM, X>, whole, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st, true,
-                          q.shares > 1 ? q.shares : 0, q);
+    const dim3 grid((unsigned)cdiv64(p.g.tiles, MT), 1, (unsigned)p.shares);
+    const int warps = p.g.kb / p.shares < kQ4Warps ? p.g.kb / p.shares : kQ4Warps;
+    return launch_cluster(q4_rows_kernel<A, NT, MT, U, GM, X>, grid, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st, true,
+                          p.shares > 1 ? p.shares : 0, p);
 }
 template <class A, int NT, int MT, int U, int GM>
 cudaError_t q4_forms(const Q4Params& p, cudaStream_t st) {
@@ -587,10 +610,10 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
             }
         }
         cluster_sync();
-        const int mine = NTOK / p.shares;
+        const int mine = (NTOK + p.shares - 1) / p.shares;
         for (int i = tid; i < mine * 32; i += q4_tile_threads(NTOK)) {
             const int c = share * mine + (i >> 5), o = 4 * (i & 31), m = m0 + c, out = tile0 * 16 + o;
-            if (m >= p.M || out >= g.N) continue;
+            if (c >= NTOK || m >= p.M || out >= g.N) continue;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int r = 0; r < p.shares; ++r) {
                 const float4 x = ld_cluster(smem_addr(sums + c * 128 + o), r);
@@ -650,12 +673,11 @@ void q4_tiles_choose(const Q4Params& p, int* ntok, int* shares) {
     double best = 1e30;
     for (int t = 32; t <= 256; t *= 2) {
         if (t > 32 && t / 2 >= p.M) break;
-        for (int c = 1; c <= 8; c *= 2) {
+        const double tiles = (double)(cdiv64(p.g.tiles, 8) * cdiv64(p.M, t));
+        const double stage = (t <= 64 ? 220 : t == 128 ? 290 : 560) * (p.vec8 ? 1.0 : p.vec2 ? 1 + t / 128.0 : 1 + t / 64.0);
+        for (int c = 1; c <= 8; ++c) {
             if (c > 1 && p.g.kb < 8 * c) break;
-            const int64_t ctas = cdiv64(p.g.tiles, 8) * cdiv64(p.M, t) * c;
-            const double stage = (t <= 64 ? 220 : t == 128 ? 290 : 560) * (p.vec8 ? 1.0 : p.vec2 ? 1 + t / 128.0 : 1 + t / 64.0);
-            // clusters of one CTA an SM do not fill every GPC
-            const double clocks = (double)cdiv64(ctas, c == 1 ? 148 : c == 2 ? 144 : c == 4 ? 136 : 128) * ((double)p.g.kb / c * stage + 4000 + (c > 1 ? 1500 : 0));
+            const double clocks = std::ceil(tiles * c / kAtOnce[c]) * ((double)p.g.kb / c * stage + 4000 + (c > 1 ? 1500 : 0));
             if (clocks < best) best = clocks, *ntok = t, *shares = c;
         }
     }
@@ -694,10 +716,10 @@ cudaError_t q4_tiles_setup() {
 
 template <class A>
 cudaError_t q4_run(const Q4Params& p, cudaStream_t st) {
-    // Two tiles a CTA share their loads of x, where there are tiles enough
-    // for every SM. 8192 x 8192, one row: 11.6 us against 13.4 of one tile a
-    // CTA; 4096 x 4096: 5.9 against 5.0 (both before launches overlapped).
-    if (p.M <= 8) return p.g.tiles >= 3 * 148 ? q4_rows<A, 1, 2, 2>(p, st) : q4_rows<A, 1, 1, 4>(p, st);
+    // Two tiles a CTA share their loads of x, and fewer inputs make a chunk;
+    // one gives more CTAs. 8192 x 8192, one row: 9.9 us with two, 12.2 with
+    // one; 4096 x 4096: 5.6 and 4.1; 4096 x 6144: 5.8 and 7.2.
+    if (p.M <= 8) return p.mt == 2 ? q4_rows<A, 1, 2, 2>(p, st) : q4_rows<A, 1, 1, 4>(p, st);
     // 9 to 16 rows: reading x for every tile of 16 outputs is what costs in the
     // rows' kernel, starting in the tiles' (all 16 rows). 4096 x 4096: 9.0 us against 7.6,
     // 4096 x 16384 18.2 against 15.6, 1024 x 1024 3.0 against 4.3.
@@ -765,6 +787,10 @@ BNN_API int bnn_q4_layer_create(int device, int n_in, int n_out, int group, int 
     L->device = device;
     L->type = type;
     L->geo = q4_geo(n_in, n_out, group);
+    int two = 1;
+    L->mt = q4_rows_shares(L->geo, 2, 2, &two) < q4_rows_shares(L->geo, 1, 4, &L->shares8) ? 2 : 1;
+    if (L->mt == 2) L->shares8 = two;
+    q4_rows_shares(L->geo, 2, 1, &L->shares16);
     const int rc = device < 0 ? BNN_OK : q4_create(L, codes, scales, zeros, bias);
     if (rc) {
         bnn_q4_layer_destroy(L);
@@ -797,6 +823,8 @@ BNN_API int bnn_q4_layer_run(const bnn_q4_layer* L, const void* d_x, int64_t x_s
     p.y = (uint16_t*)d_y;
     p.ys = y_stride;
     p.M = rows;
+    p.mt = L->mt;
+    p.shares = rows <= 8 ? L->shares8 : L->shares16;
     p.vec2 = aligned(d_x, 4) && (rows == 1 || x_stride % 2 == 0);
     p.vec4 = aligned(d_x, 8) && (rows == 1 || x_stride % 4 == 0);
     p.vec8 = aligned(d_x, 16) && (rows == 1 || x_stride % 8 == 0);

@@ -92,7 +92,12 @@ def linear_ref(d, x, k, group, kind):
     (40, 4099, 200, 32, False, False), (60, 6002, 140, 128, True, False), (128, 5001, 130, 64, False, True), (260, 4098, 300, 128, True, True),
     (1000, 3001, 1111, 64, False, False),
     # K shared out in a cluster, at borders that are not a group's
-    (1, 6464, 40, 256, True, False), (3, 4160, 16, 512, False, True), (12, 2176, 33, 128, True, True), (7, 8192, 100, 1024, True, False)])
+    (1, 6464, 40, 256, True, False), (3, 4160, 16, 512, False, True), (12, 2176, 33, 128, True, True), (7, 8192, 100, 1024, True, False),
+    # by three, five, six and seven, few rows and many, at every width of a tile
+    (3, 4160, 100, 64, True, True), (5, 6464, 300, 32, False, False), (8, 9000, 90, 128, True, False), (1, 7168, 600, 256, True, True),
+    (4, 5120, 2560, 512, False, True), (12, 3200, 100, 32, True, False), (10, 6464, 33, 128, True, True), (16, 9000, 300, 64, False, False),
+    (70, 3200, 100, 32, True, True), (33, 2704, 90, 128, False, True), (200, 1800, 130, 64, True, False), (515, 2704, 130, 96, True, False),
+    (65, 3264, 1000, 128, True, True), (1000, 1600, 300, 256, False, True), (700, 2704, 1000, 64, True, False)])
 def test_linear(m, k, n, group, zeros, bias, kind):
     layer, d = linear_case(m * 7 + k, m, k, n, group, kind, zeros, bias)
     y = torch.full((m + 1, n), 7.0, device="cuda", dtype=TYPES[kind])
