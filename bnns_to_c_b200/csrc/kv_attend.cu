@@ -183,7 +183,7 @@ __device__ __forceinline__ void load_scales(float* f, const uint16_t* at) {  // 
 // SM's 4 instructions a clock, half of them bit operations and conversions, at
 // 16 warps of 127 registers an SM. 100003 tokens, 8 kv heads of 128 in 8 bits,
 // 32 query heads: 46 us with the join (4.5 TB/s of codes). 179457 tokens of 64
-// sequences, 64 query heads, in 4 bits and groups of 32: 82 us (2.6 TB/s). The
+// sequences, 64 query heads, in 4 bits and groups of 32: 75 us (2.8 TB/s). The
 // work is cut into one equal share a CTA, in blocks of tokens, whatever
 // sequence they belong to; what is cut is joined by join_kernel.
 template <int DP, int BITS, int NT, int BPG>
@@ -675,8 +675,14 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 }
 
 // ---------------------------------------------------------------- join
-// One CTA a query row: the parts of its items, of its own positions (and of
-// the prefix), each a sum with its maximum, joined with their weights.
+// For each query row the parts of its items, of its own positions (and of the
+// prefix), each a sum with its maximum, joined with their weights. PER = 4: a
+// CTA a row, whose warps share the parts, where there are few rows, of many
+// parts each; PER = 1: a warp a row, which saves the join of the warps. Whole
+// attentions: 64 ragged sequences of 64 heads 75 us with 1, 82 with 4; 82
+// sequences of 64 heads behind 64 tokens 32 and 47; 96 of 16 behind 8190 41
+// and 43; 48 of 16 behind 8190 32.5 and 30.6; 16 ragged ones of 64 28 and 25;
+// one of 32 heads, 100003 tokens, 64 and 46.
 struct JoinSide {
     const int2* owners;  // nullptr: this side has nothing
     const float* pacc;
@@ -693,19 +699,22 @@ struct JoinParams {
     uint16_t* out;
     int64_t o_seq, o_head;
     float* lse;
-    bool fp16, partial;
+    bool fp16, partial, o_vec;
 };
 
 constexpr int kJoinWarps = 4;
 
+template <int PER>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams p) {
-    __shared__ __align__(16) float sums[kJoinWarps][256];
-    __shared__ float2 wml[kJoinWarps];
+    __shared__ __align__(16) float sums[PER][256];
+    __shared__ float2 wml[PER];
     grid_wait();
     grid_launch();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = PER == 1 ? 0 : threadIdx.x >> 5;  // of the row's
     const int q_heads = p.heads * p.share;
-    for (int n = blockIdx.x; n < p.rows; n += gridDim.x) {
+    constexpr int ROWS = kJoinWarps / PER;  // of a CTA at a time
+    const int row0 = blockIdx.x * ROWS + (PER == 1 ? threadIdx.x >> 5 : 0);
+    for (int n = row0; n < p.rows; n += gridDim.x * ROWS) {
         const int seq = n / q_heads, qh = n % q_heads, head = qh / p.share;
         const int row = seq * p.share + qh % p.share;  // of the kv head's query rows
         float m = -INFINITY, l = 0.0f, acc[8] = {};
@@ -728,8 +737,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
         for (int w = 0; w < 2; ++w) {
             const JoinSide& s = p.side[w];
             // a lane reads the maximum and sum of a part, then all read its values
-            for (int c = own[w].x + warp; c <= own[w].y; c += 32 * kJoinWarps) {
-                const int mine = c + lane * kJoinWarps;
+            for (int c = own[w].x + warp; c <= own[w].y; c += 32 * PER) {
+                const int mine = c + lane * PER;
                 const int64_t slot = own[w].x == own[w].y ? 2 * (int64_t)s.ctas + item[w] : 2 * (int64_t)mine + (mine == own[w].x);
                 float2 ml = make_float2(-INFINITY, 0.0f);
                 if (mine <= own[w].y) ml = s.pml[slot * s.R + i[w]];
@@ -745,7 +754,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
 #pragma unroll
                 for (int k = 0; k < 8; ++k) acc[k] *= a;
                 // (a part that saw nothing has left zeros)
-                const int parts = min(32, (own[w].y - c) / kJoinWarps + 1);
+                const int parts = min(32, (own[w].y - c) / PER + 1);
 #pragma unroll 8
                 for (int q = 0; q < parts; ++q) {
                     const float f = __shfl_sync(0xffffffffu, b, q);
@@ -761,25 +770,43 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
                 }
             }
         }
+        if constexpr (PER == 1) {
+            const float norm = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int d = 128 * k + 4 * lane;
+                if (d >= p.dim) continue;
+                uint16_t* to = p.out + seq * p.o_seq + qh * p.o_head + d;
+                const uint32_t lo = pack2(acc[4 * k] * norm, acc[4 * k + 1] * norm, p.fp16);
+                const uint32_t hi = pack2(acc[4 * k + 2] * norm, acc[4 * k + 3] * norm, p.fp16);
+                if (p.o_vec) {
+                    *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+                } else {
+                    to[0] = (uint16_t)lo, to[1] = (uint16_t)(lo >> 16), to[2] = (uint16_t)hi, to[3] = (uint16_t)(hi >> 16);
+                }
+            }
+            if (p.lse && lane == 0) p.lse[(int64_t)seq * q_heads + qh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+            continue;
+        }
         if (lane == 0) wml[warp] = make_float2(m, l);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
             if (128 * k + 4 * lane < p.dp)
                 *reinterpret_cast<float4*>(&sums[warp][128 * k + 4 * lane]) = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
         __syncthreads();
-        float top = -INFINITY, c[kJoinWarps], sum = 0.0f;
+        float top = -INFINITY, c[PER], sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, wml[w].x);
+        for (int w = 0; w < PER; ++w) top = fmaxf(top, wml[w].x);
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
+        for (int w = 0; w < PER; ++w) {
             c[w] = wml[w].x == -INFINITY ? 0.0f : exp2_fast(wml[w].x - top);
             sum += wml[w].x == -INFINITY ? 0.0f : c[w] * wml[w].y;
         }
         const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (int d = threadIdx.x; d < p.dim; d += 32 * kJoinWarps) {
+        for (int d = threadIdx.x; d < p.dim; d += 32 * PER) {
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w)
+            for (int w = 0; w < PER; ++w)
                 if (c[w] != 0.0f) v = fmaf(c[w], sums[w][d], v);
             p.out[seq * p.o_seq + qh * p.o_head + d] = (uint16_t)pack2(v * norm, 0.0f, p.fp16);
         }
@@ -943,7 +970,7 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
     jp.rows = n_seqs * q_heads;
     jp.heads = g.heads, jp.share = share, jp.dim = g.dim, jp.dp = g.dp;
     jp.out = p.out, jp.o_seq = o_seq, jp.o_head = o_head, jp.lse = d_lse;
-    jp.fp16 = p.fp16, jp.partial = prefix;
+    jp.fp16 = p.fp16, jp.partial = prefix, jp.o_vec = p.o_vec;
     uint8_t* work = (uint8_t*)d_work;
     for (int side = prefix ? 1 : 0; side >= 0; --side) {
         const Plan s = side ? attend_plan(c, 1, n_seqs * share, true) : attend_plan(c, n_seqs, share, prefix);
@@ -959,7 +986,7 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
         p.second = prefix && side == 0 && pdl_on();
         // Started early, its CTAs would find the places of an SM taken by
         // those of the kernel before, and their shares are equal: 94 us
-        // against 82 for 64 ragged sequences in 4 bits.
+        // against 82 for 64 ragged sequences in 4 bits (before the join had two forms).
         const cudaError_t e = attend_any(g, s.nt, [&](auto k) { return launch(k, dim3(s.ctas), 32 * kWarps, s.smem, st, p.second, p); });
         if (e != cudaSuccess) return cuda_error("bnn_kv_attend", e);
         jp.side[side] = JoinSide{p.owners, p.pacc, p.pml, p.lengths, p.length, s.rg, s.rt, 8 * s.nt, s.ctas};
@@ -967,6 +994,8 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
     }
     // no sequence can be longer than a block: none is cut
     if (!prefix && (int64_t)table_pages * g.pt <= kLong) return BNN_OK;
-    const cudaError_t e = launch(join_kernel, dim3((unsigned)min(jp.rows, c->sms * 12)), 32 * kJoinWarps, 0, st, true, jp);
+    const bool alone = jp.rows > 10 * c->sms;
+    const int ctas = alone ? (int)cdiv64(jp.rows, kJoinWarps) : jp.rows;
+    const cudaError_t e = launch(alone ? join_kernel<1> : join_kernel<kJoinWarps>, dim3((unsigned)min(ctas, c->sms * 12)), 32 * kJoinWarps, 0, st, true, jp);
     return e == cudaSuccess ? BNN_OK : cuda_error("bnn_kv_attend", e);
 }

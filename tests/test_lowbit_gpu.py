@@ -439,6 +439,31 @@ def test_attend_shared_prefix(prefix, lengths, heads, share, dim, bits, kind):
     check_attend(prefix, lengths, heads, share, dim, bits, 32, kind, 16, prefix=prefix)
 
 
+@pytest.mark.parametrize("prefix,length", [(0, 700), (90, 5), (300, 0), (1030, 300)])
+@pytest.mark.parametrize("seqs,dim,kind", [(100, 64, "bf16"), (480, 80, "fp16"), (130, 256, "bf16")])
+def test_attend_many_rows(seqs, dim, kind, prefix, length):
+    """Thousands of query rows, all of one sequence (and of an empty one), so
+    that one reference serves; rows of the output at an odd distance."""
+    heads, share = 2, 8
+    c, table, pre, held = filled(seqs, [length], heads, dim, 4, 32, kind, 16, prefix)
+    q1 = torch.randn(1, heads * share, dim, device="cuda", generator=gen(4)).to(TYPES[kind])
+    r_out, r_lse, t_out, t_lse = attend_ref(q1, held, dim ** -0.5, kind)
+    lengths = torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+    lengths[7] = 0
+    work = torch.full((c.attend_work(seqs, heads * share, prefix),), 0xFF, device="cuda", dtype=torch.uint8)
+    wide = torch.full((seqs, heads * share, dim + 3), 3.0, device="cuda", dtype=TYPES[kind])
+    out, lse = wide[:, :, 1:dim + 1], torch.full((seqs, heads * share), 3.0, device="cuda")
+    c.attend(q1.expand(seqs, -1, -1), lengths, table.expand(seqs, -1).contiguous(), out, work, lse=lse,
+             prefix=pre if prefix else None, prefix_tokens=prefix)
+    assert (wide[:, :, 0] == 3).all() and (wide[:, :, dim + 1:] == 3).all()
+    others = [i for i in range(seqs) if i != 7]
+    within(out[others], r_out.expand(seqs - 1, -1, -1), t_out.expand(seqs - 1, -1, -1), "out")
+    within(lse[others], r_lse.expand(seqs - 1, -1), t_lse.expand(seqs - 1, -1), "lse")
+    r_out, r_lse, t_out, t_lse = attend_ref(q1, [tuple(x[:prefix] for x in held[0])], dim ** -0.5, kind)
+    within(out[7:8], r_out, t_out, "out of the empty one")
+    within(lse[7:8], r_lse, t_lse, "lse of the empty one")
+
+
 @pytest.mark.parametrize("mag", [1e-3, 40.0, 1e4])
 def test_attend_magnitudes(mag):
     """Flat and peaked weights; values far from one in size."""
