@@ -21,6 +21,7 @@ namespace lowbit {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kMostInv = 127 + 118;  // exponent field of the largest 1 / unit: times 2^8 a float
 constexpr int kSub = 16;  // tokens of an instruction
 // 16-token blocks that a warp takes at a time: two where the sums leave it the
 // registers and a row is short (of `row` bytes), so that shared memory holds
@@ -56,7 +57,7 @@ struct AttendParams {
     bool partial;            // leave every item to the join kernel
     bool second;             // runs beside the prefix's kernel
     int2* owners;            // [group][kv head][tile]: first and last CTA of an item, for the join
-    float* pacc;             // [slot][row][dp] sums of exp2(s - m) * value
+    float* pacc;             // [slot][row][dp] means of the values with weights exp2(s - m)
     float2* pml;             // [slot][row] (m, sum of exp2(s - m))
     int stages;
 };
@@ -81,6 +82,8 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
     return d;
 }
+// 2^e for e <= 0; 0 below the range of normal numbers
+__device__ __forceinline__ float pow2(int e) { return e < -126 ? 0.0f : __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -367,11 +370,15 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
         __syncthreads();
 
         float acc[NB][2][NT][4], m[NT][2], l[NT][2], f[NT][2];
-        // sums of values are kept in units of a power of two for each scale
-        // group, near its largest scale so far: bf16 scales reach beyond fp16
-        float inv[NG];  // 1 / unit
+        // Sums of weight * scale * code are kept in a unit of a power of two for
+        // each query row and scale group, so that a unit follows what the row
+        // sees: neither a token without weight in it nor another row's values
+        // move it. inv: 1 / unit beside exp2(s - m).
+        float inv[NG][NT][2];
 #pragma unroll
-        for (int q = 0; q < NG; ++q) inv[q] = __uint_as_float(250u << 23);
+        for (int q = 0; q < NG; ++q)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) inv[q][t][0] = inv[q][t][1] = __uint_as_float((uint32_t)kMostInv << 23);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -475,10 +482,8 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                         }
                     }
                 }
-                // The running maximum and the units are lazy: raised when a
-                // score is 2^8 above the maximum, or a scale 2^6 above its
-                // unit, so most steps need no reduction over the lanes.
-                // weight * scale / unit stays below 2^14, in fp16.
+                // The running maximum is lazy: raised when a score is 2^8 above
+                // it, so most steps need no reduction over the lanes.
                 bool raise = false;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -488,12 +493,6 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                         if constexpr (HV == 2) x = fmaxf(x, fmaxf(s[1][t][e], s[1][t][2 + e]));
                         raise |= x > m[t][e] + 8.0f;
                     }
-#pragma unroll
-                for (int q = 0; q < NG; ++q) {
-                    float x = fmaxf(v0[0][q], v1[0][q]);
-                    if constexpr (HV == 2) x = fmaxf(x, fmaxf(v0[1][q], v1[1][q]));
-                    raise |= x * inv[q] > 64.0f;
-                }
                 if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
@@ -505,36 +504,22 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                             x = fmaxf(x, m[t][e]);
-                            const float corr = x == m[t][e] ? 1.0f : exp2_fast(m[t][e] - x);
+                            // inv takes the increase in whole powers of two, no fewer than it
+                            // is, so that exp2(s - m) * inv never becomes less; the sums the rest
+                            const float d = x == m[t][e] ? 0.0f : fminf(x - m[t][e], 252.0f), n = ceilf(d), part = exp2_fast(n - d);
                             m[t][e] = x;
-                            l[t][e] *= corr;
+                            l[t][e] *= part * pow2(-(int)n);
 #pragma unroll
-                            for (int b = 0; b < NB; ++b)
+                            for (int q = 0; q < NG; ++q) {
+                                const int to = (int)(__float_as_uint(inv[q][t][e]) >> 23) + (int)n, over = max(0, to - kMostInv);
+                                inv[q][t][e] = __uint_as_float((uint32_t)(to - over) << 23);
+                                const float corr = part * pow2(-over);
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) acc[b][h][t][e] *= corr, acc[b][h][t][2 + e] *= corr;
+                                for (int b = q * BPG; b < (q + 1) * BPG && b < NB; ++b)
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) acc[b][h][t][e] *= corr, acc[b][h][t][2 + e] *= corr;
+                            }
                         }
-#pragma unroll
-                    for (int q = 0; q < NG; ++q) {
-                        uint32_t big = 0;
-#pragma unroll
-                        for (int h = 0; h < HV; ++h) {
-                            const uint32_t u0 = __float_as_uint(v0[h][q]), u1 = __float_as_uint(v1[h][q]);  // NaN: bits above infinity's
-                            big = max(big, max(u0 < 0x7f800000u ? u0 : 0u, u1 < 0x7f800000u ? u1 : 0u));
-                        }
-                        big = __reduce_max_sync(0xffffffffu, big);
-                        const uint32_t unit = (254u << 23) - __float_as_uint(inv[q]), now = max(unit, min(big & 0x7f800000u, 253u << 23));
-                        const int down = (int)((now - unit) >> 23);
-                        const float corr = down > 126 ? 0.0f : __int_as_float((127 - down) << 23);
-                        inv[q] = __uint_as_float((254u << 23) - now);
-#pragma unroll
-                        for (int b = q * BPG; b < (q + 1) * BPG && b < NB; ++b)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) acc[b][h][t][e] *= corr;
-                    }
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -548,10 +533,74 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                             l[t][e] += s[h][t][e] + s[h][t][2 + e];
                         }
                     }
-                // output: channels in rows, query rows in columns, the tokens
-                // summed. The values' scales go with the weights, rounded
-                // once to fp16: 2^-12 of each term, independent of one
-                // another, next to a result of 8 or 11 bits.
+                // The values' scales go with the weights, in the row's units,
+                // rounded once to fp16: 2^-11 of each term at most, independent of
+                // one another, next to a result of 8 or 11 bits. A unit is raised
+                // when one is 2^15 or more, and puts it at 2^8: the largest of a
+                // row and group is at least that, so that only those below 2^-22
+                // of it lose bits (are 2^-33 of it off). At 2^11, raised more often,
+                // 16 sequences of 32 rows a kv head took 77 us, at 2^8 70.
+                uint32_t wt[HV][NG][NT][2];
+                const auto weigh = [&] {
+#pragma unroll
+                    for (int h = 0; h < HV; ++h)
+#pragma unroll
+                        for (int q = 0; q < NG; ++q)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {  // (weight * inv) * scale: no infinity on the way to a number
+                                const uint64_t u = both(inv[q][t][0], inv[q][t][1]);
+                                const float2 w0 = apart(mul2(mul2(both(s[h][t][0], s[h][t][1]), u), both(v0[h][q], v0[h][q])));
+                                const float2 w1 = apart(mul2(mul2(both(s[h][t][2], s[h][t][3]), u), both(v1[h][q], v1[h][q])));
+                                wt[h][q][t][0] = pack2(w0.x, w0.y, true);
+                                wt[h][q][t][1] = pack2(w1.x, w1.y, true);
+                            }
+                };
+                weigh();
+                uint32_t most[4] = {};  // two halves each, none of them negative
+#pragma unroll
+                for (int h = 0; h < HV; ++h)
+#pragma unroll
+                    for (int q = 0; q < NG; ++q)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            uint32_t& x = most[((h * NG + q) * NT + t) & 3];
+                            x = __vimax3_u16x2(x, wt[h][q][t][0], wt[h][q][t][1]);
+                        }
+                const uint32_t top = __vimax3_u16x2(__vmaxu2(most[0], most[1]), most[2], most[3]);
+                if (__builtin_expect(__any_sync(0xffffffffu, (top + 0x08000800u) & 0x80008000u), 0)) {
+#pragma unroll
+                    for (int q = 0; q < NG; ++q)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            uint32_t f[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float x = 0.0f;  // (a NaN is passed over)
+#pragma unroll
+                                for (int h = 0; h < HV; ++h)  // 2^-8: the weights are at most 2^8
+                                    x = fmaxf(x, fmaxf(s[h][t][e] * 0x1p-8f * v0[h][q], s[h][t][2 + e] * 0x1p-8f * v1[h][q]));
+                                f[e] = __float_as_uint(x);
+                            }
+                            uint32_t x = __byte_perm(f[0], f[1], 0x7632);  // both at their upper 16 bits
+                            x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, 16));
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                // the largest to 2^8 .. 2^9, unless it is below that already
+                                const int was = (int)(__float_as_uint(inv[q][t][e]) >> 23);
+                                const int now = min(was, 2 * 127 + 8 - 8 - (int)(x >> (16 * e + 7) & 255u));
+                                inv[q][t][e] = __uint_as_float((uint32_t)now << 23);
+                                const float corr = pow2(now - was);
+#pragma unroll
+                                for (int b = q * BPG; b < (q + 1) * BPG && b < NB; ++b)
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) acc[b][h][t][e] *= corr, acc[b][h][t][2 + e] *= corr;
+                            }
+                        }
+                    weigh();
+                }
+                // output: channels in rows, query rows in columns, the tokens summed
 #pragma unroll
                 for (int h = 0; h < HV; ++h) {
                     const uint8_t* vb = step + h * HALF + CODES;
@@ -562,11 +611,10 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
                         if (b % BPG == 0) {
-                            const float w0 = v0[h][b / BPG] * inv[b / BPG], w1 = v1[h][b / BPG] * inv[b / BPG];
 #pragma unroll
                             for (int t = 0; t < NT; ++t) {
-                                wb[t][0] = movm_t(pack2(s[h][t][0] * w0, s[h][t][1] * w0, true));
-                                wb[t][1] = movm_t(pack2(s[h][t][2] * w1, s[h][t][3] * w1, true));
+                                wb[t][0] = movm_t(wt[h][b / BPG][t][0]);
+                                wb[t][1] = movm_t(wt[h][b / BPG][t][1]);
                             }
                         }
                         uint32_t a[2][4];
@@ -599,7 +647,8 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
         cp_wait<0>();
         __syncthreads();
 
-        // join the warps
+        // join the warps: each leaves the mean of its values, which are in the
+        // range of a float whatever the number of tokens, and its sum of weights
         float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -612,13 +661,14 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                 if (m[t][e] == -INFINITY && l[t][e] != 0.0f) m[t][e] = 0.0f;
                 const int row = t * 8 + 2 * j + e;
                 if (r == 0) wml[warp * R + row] = make_float2(m[t][e], l[t][e]);
+                const float norm = l[t][e] == 0.0f ? 0.0f : 1.0f / l[t][e];
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const float unit = __uint_as_float((254u << 23) - __float_as_uint(inv[b / BPG]));
+                    const float unit = __uint_as_float((254u << 23) - __float_as_uint(inv[b / BPG][t][e]));
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                         *reinterpret_cast<float2*>(sums + (warp * R + row) * (DP + 8) + 32 * b + 4 * r + 2 * h) =
-                            make_float2(acc[b][h][t][e] * unit, acc[b][h][t][2 + e] * unit);
+                            make_float2(acc[b][h][t][e] * norm * unit, acc[b][h][t][2 + e] * norm * unit);
                 }
             }
         __syncthreads();
@@ -633,10 +683,10 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float2 ml = wml[w * R + tid];
-                c[w] = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
-                sum += ml.x == -INFINITY ? 0.0f : c[w] * ml.y;
+                c[w] = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top) * ml.y;
+                sum += c[w];
             }
-            const float norm = direct ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+            const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) wml[w * R + tid].x = c[w] * norm;
             const int row = row0 + tid;
@@ -676,7 +726,7 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 
 // ---------------------------------------------------------------- join
 // For each query row the parts of its items, of its own positions (and of the
-// prefix), each a sum with its maximum, joined with their weights. PER = 4: a
+// prefix), each a mean with the maximum and the sum of its weights. PER = 4: a
 // CTA a row, whose warps share the parts, where there are few rows, of many
 // parts each; PER = 1: a warp a row, which saves the join of the warps. Whole
 // attentions: 64 ragged sequences of 64 heads 75 us with 1, 82 with 4; 82
@@ -747,17 +797,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
                 top = fmaxf(top, m);
                 const float a = m == -INFINITY ? 0.0f : exp2_fast(m - top);
                 const float b = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);  // 0: this part saw nothing
-                float sum = ml.x == -INFINITY ? 0.0f : b * ml.y;
+                const float part = ml.x == -INFINITY ? 0.0f : b * ml.y;
+                float sum = part;
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 m = top;
-                l = l * a + sum;
+                sum += l * a;
+                const float norm = sum == 0.0f ? 0.0f : 1.0f / sum, old = l * a * norm;
+                l = sum;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) acc[k] *= a;
+                for (int k = 0; k < 8; ++k) acc[k] *= old;
                 // (a part that saw nothing has left zeros)
                 const int parts = min(32, (own[w].y - c) / PER + 1);
 #pragma unroll 8
                 for (int q = 0; q < parts; ++q) {
-                    const float f = __shfl_sync(0xffffffffu, b, q);
+                    const float f = __shfl_sync(0xffffffffu, part * norm, q);
                     const int64_t from = __shfl_sync(0xffffffffu, slot, q);
                     const float* x = s.pacc + (from * s.R + i[w]) * p.dp + 4 * lane;
 #pragma unroll
@@ -771,14 +824,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
             }
         }
         if constexpr (PER == 1) {
-            const float norm = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int d = 128 * k + 4 * lane;
                 if (d >= p.dim) continue;
                 uint16_t* to = p.out + seq * p.o_seq + qh * p.o_head + d;
-                const uint32_t lo = pack2(acc[4 * k] * norm, acc[4 * k + 1] * norm, p.fp16);
-                const uint32_t hi = pack2(acc[4 * k + 2] * norm, acc[4 * k + 3] * norm, p.fp16);
+                const uint32_t lo = pack2(acc[4 * k], acc[4 * k + 1], p.fp16);
+                const uint32_t hi = pack2(acc[4 * k + 2], acc[4 * k + 3], p.fp16);
                 if (p.o_vec) {
                     *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
                 } else {
@@ -799,16 +851,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinParams 
         for (int w = 0; w < PER; ++w) top = fmaxf(top, wml[w].x);
 #pragma unroll
         for (int w = 0; w < PER; ++w) {
-            c[w] = wml[w].x == -INFINITY ? 0.0f : exp2_fast(wml[w].x - top);
-            sum += wml[w].x == -INFINITY ? 0.0f : c[w] * wml[w].y;
+            c[w] = wml[w].x == -INFINITY ? 0.0f : exp2_fast(wml[w].x - top) * wml[w].y;
+            sum += c[w];
         }
         const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
         for (int d = threadIdx.x; d < p.dim; d += 32 * PER) {
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < PER; ++w)
-                if (c[w] != 0.0f) v = fmaf(c[w], sums[w][d], v);
-            p.out[seq * p.o_seq + qh * p.o_head + d] = (uint16_t)pack2(v * norm, 0.0f, p.fp16);
+                if (c[w] != 0.0f) v = fmaf(c[w] * norm, sums[w][d], v);
+            p.out[seq * p.o_seq + qh * p.o_head + d] = (uint16_t)pack2(v, 0.0f, p.fp16);
         }
         if (p.lse && threadIdx.x == 0)
             p.lse[(int64_t)seq * q_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;

@@ -128,6 +128,11 @@ int bnn_kv_cache_read(const bnn_kv_cache *c, void *d_k, int64_t k_token,
  * position gets zeros, and a log-sum of -infinity. A NaN in a key, value or
  * query (in a query an infinity, too) makes NaN of what depends on it, and of
  * nothing else.
+ * Scores, their maximum and sum, and the sums of values are 32-bit. A weight
+ * times the scale of a value is rounded to 11 bits: a term of the sum is off by
+ * 2^-11 of itself, or, where it is less than 2^-22 of the largest such product
+ * of the row in the scale group, by 2^-33 of that product for each step of its
+ * code. Keys of 2^100 and more make scores that are not finite.
  * q and out: the cache's type, sequence b and head i at
  * q + b * q_seq + i * q_head; they must not overlap. d_lse, unless NULL:
  * float32 [n_seqs][q_heads], the natural logarithm of
