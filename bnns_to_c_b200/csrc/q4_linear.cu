@@ -18,6 +18,7 @@ struct bnn_q4_layer {
     int mt;                  // for up to 8 rows: tiles of 16 outputs a CTA,
     int shares8;             //   CTAs that share K; for 9 to 16
     int shares16;
+    bool exact;              // some weight (q - z) * s is outside the type's range
 };
 
 namespace bnn {
@@ -26,9 +27,12 @@ namespace {
 
 // ---------------------------------------------------------------- layout, once
 // Padding: an input behind the last has code = zero point (weight 0), a row
-// behind the last has scale 0.
-__global__ void q4_layout_kernel(Q4Geo g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, uint32_t magic,
-                                 uint32_t* wo, uint16_t* szo) {
+// behind the last has scale 0. *exact is set where a weight (q - z) * s with a
+// finite scale would round to an infinity of the type.
+template <class A>
+__global__ void q4_layout_kernel(Q4Geo g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
+                                 uint32_t* wo, uint16_t* szo, int* exact) {
+    constexpr uint32_t magic = A::kMagic & 0xffffu;
     const int64_t words = q4_words(g), step = (int64_t)gridDim.x * blockDim.x;
     const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t half = ((int64_t)g.K + 1) / 2;
@@ -41,9 +45,12 @@ __global__ void q4_layout_kernel(Q4Geo g, const uint8_t* codes, const uint16_t* 
             const int row = tile * 16 + q4_row(lane, nib), k = kb * 64 + q4_in(lane, i, nib);
             uint32_t q = 8;
             if (row < g.N) {
-                if (k < g.K)
+                if (k < g.K) {
                     q = (codes[row * half + (k >> 1)] >> (4 * (k & 1))) & 15u;
-                else if (zeros)
+                    const int64_t at = (int64_t)row * g.ng + k / g.group;
+                    const float s = A::unpack(scales[at]).x, w = (float)((int)q - (zeros ? zeros[at] & 15 : 8)) * s;
+                    if (isinf(A::to_float(A::from_float(w))) && !isinf(s)) *exact = 1;
+                } else if (zeros)
                     q = zeros[(int64_t)row * g.ng + min(k / g.group, g.ng - 1)] & 15u;
             }
             v |= q << (4 * (nib & 3) + 16 * (nib >> 2));
@@ -96,11 +103,13 @@ struct Q4Params {
     int shares;       // of K: CTAs of a cluster that make the same outputs
     int mt;           // tiles of 16 outputs a CTA, up to 8 rows
     int gshift;       // group = 32 << gshift, or -1
+    bool exact;       // weights are not to be rounded to the type
     bool vec2, vec4, vec8;  // rows of x start 4-byte, 8-byte, 16-byte aligned
 };
 
 // ---------------------------------------------------------------- rows on mma.sync
-// Few rows. A CTA makes MT tiles of 16 outputs for 8 * NT rows of x; its
+// Few rows, or (in slices of 16) any number where the weights do not fit the
+// type. A CTA makes MT tiles of 16 outputs for 8 * NT rows of x; its
 // warps take chunks of U 64-input blocks in turn and their sums are joined in
 // shared memory. The weights of the next chunk are on their way while one is
 // multiplied: U * MT * 512 bytes a warp. Bound by reading the weights and, as
@@ -128,7 +137,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be one number a warp
     const int r = lane >> 2, j = lane & 3;
-    const int tile0 = blockIdx.x * MT;
+    const int tile0 = blockIdx.x * MT, m0 = blockIdx.y * 8 * NT, rows = min(8 * NT, p.M - m0);
     const Q4Geo g = p.g;
     grid_launch();
     // Whole chunks first, U blocks at a time, the warps in turn; the blocks
@@ -147,7 +156,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int m = t * 8 + r;
-        xr[t] = p.x + (m < p.M ? m * p.xs : 0) + (int64_t)first * 64 + 4 * j;
+        xr[t] = p.x + (m < rows ? m0 + m : m0) * p.xs + (int64_t)first * 64 + 4 * j;
     }
     const uint4* wr[MT];
     const uint2* sr[MT];
@@ -252,10 +261,10 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     __syncthreads();
     const auto store = [&](int i, float v) {
         const int m = i / (16 * MT), o = i % (16 * MT), n = tile0 * 16 + o;
-        if (m >= p.M || n >= g.N) return;
+        if (m >= rows || n >= g.N) return;
         if (p.bias) v += p.bias[n];
         const typename A::T out = A::from_float(v);
-        p.y[m * p.ys + n] = *reinterpret_cast<const uint16_t*>(&out);
+        p.y[(m0 + m) * p.ys + n] = *reinterpret_cast<const uint16_t*>(&out);
     };
     const auto sum = [&](int i) {
         float v = 0.0f;
@@ -305,7 +314,7 @@ double q4_rows_shares(const Q4Geo& g, int mt, int chunk_blocks, int* shares) {
 
 template <class A, int NT, int MT, int U, int GM, int X>
 cudaError_t q4_launch(const Q4Params& p, cudaStream_t st) {
-    const dim3 grid((unsigned)cdiv64(p.g.tiles, MT), 1, (unsigned)p.shares);
+    const dim3 grid((unsigned)cdiv64(p.g.tiles, MT), (unsigned)cdiv64(p.M, 8 * NT), (unsigned)p.shares);
     const int warps = p.g.kb / p.shares < kQ4Warps ? p.g.kb / p.shares : kQ4Warps;
     return launch_cluster(q4_rows_kernel<A, NT, MT, U, GM, X>, grid, 32 * warps, warps * 8 * NT * (16 * MT + 1) * 4, st, true,
                           p.shares > 1 ? p.shares : 0, p);
@@ -743,7 +752,7 @@ cudaError_t q4_run(const Q4Params& p, cudaStream_t st) {
     // 9 to 16 rows: reading x for every tile of 16 outputs is what costs in the
     // rows' kernel, starting in the tiles' (all 16 rows). 4096 x 4096: 9.0 us against 7.6,
     // 4096 x 16384 18.2 against 15.6, 1024 x 1024 3.0 against 4.3.
-    if (p.M <= 16 && (int64_t)p.g.tiles * p.g.kb < 1 << 13) return q4_rows<A, 2, 2, 1>(p, st);
+    if (p.exact || (p.M <= 16 && (int64_t)p.g.tiles * p.g.kb < 1 << 13)) return q4_rows<A, 2, 2, 1>(p, st);
     return p.g.group % 64 ? q4_tiles<A, true>(p, st) : q4_tiles<A, false>(p, st);
 }
 
@@ -768,20 +777,24 @@ int q4_create(bnn_q4_layer* L, const uint8_t* codes, const void* scales, const u
     const int64_t half = ((int64_t)g.K + 1) / 2, ns = (int64_t)g.N * g.ng;
     const size_t rw = up(g.N * half), rs = up(ns * 2), rz = zeros ? up(ns) : 0;
     void* tmp = nullptr;
-    if ((rc = device_alloc(&tmp, rw + rs + rz, "of a 4-bit layer's raw arrays"))) return rc;
+    if ((rc = device_alloc(&tmp, rw + rs + rz + 256, "of a 4-bit layer's raw arrays"))) return rc;
     uint8_t *dw = (uint8_t*)tmp, *ds = dw + rw, *dz = ds + rs;
-    e = cudaMemcpy(dw, codes, g.N * half, cudaMemcpyDefault);
+    int *flag = (int*)(dz + rz), exact = 0;
+    e = cudaMemset(flag, 0, sizeof(int));
+    if (e == cudaSuccess) e = cudaMemcpy(dw, codes, g.N * half, cudaMemcpyDefault);
     if (e == cudaSuccess) e = cudaMemcpy(ds, scales, ns * 2, cudaMemcpyDefault);
     if (e == cudaSuccess && zeros) e = cudaMemcpy(dz, zeros, ns, cudaMemcpyDefault);
     if (e == cudaSuccess && bias) e = cudaMemcpy((void*)L->bias, bias, (size_t)g.N * 4, cudaMemcpyDefault);
     if (e == cudaSuccess) {
         const int64_t blocks = cdiv64(q4_words(g), 256);
-        q4_layout_kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256>>>(
-            g, dw, (const uint16_t*)ds, zeros ? dz : nullptr, (L->type == BNN_BF16 ? Bf16::kMagic : Fp16::kMagic) & 0xffffu,
-            (uint32_t*)L->codes, (uint16_t*)L->sz);
+        const auto kernel = L->type == BNN_BF16 ? q4_layout_kernel<Bf16> : q4_layout_kernel<Fp16>;
+        kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256>>>(g, dw, (const uint16_t*)ds, zeros ? dz : nullptr,
+                                                                           (uint32_t*)L->codes, (uint16_t*)L->sz, flag);
         e = cudaGetLastError();
     }
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpy(&exact, flag, sizeof(int), cudaMemcpyDeviceToHost);
+    L->exact = exact != 0;
     cudaFree(tmp);
     return e == cudaSuccess ? BNN_OK : cuda_error("bnn_q4_layer_create", e);
 }
@@ -844,6 +857,7 @@ BNN_API int bnn_q4_layer_run(const bnn_q4_layer* L, const void* d_x, int64_t x_s
     p.ys = y_stride;
     p.M = rows;
     p.mt = L->mt;
+    p.exact = L->exact;
     p.shares = rows <= 8 ? L->shares8 : L->shares16;
     p.vec2 = aligned(d_x, 4) && (rows == 1 || x_stride % 2 == 0);
     p.vec4 = aligned(d_x, 8) && (rows == 1 || x_stride % 4 == 0);

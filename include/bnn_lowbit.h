@@ -55,7 +55,9 @@ int bnn_q4_layer_create(int device, int n_in, int n_out, int group, int type,
  * in a layer of fewer than 2^23 weights, the codes are multiplied exactly and
  * a group's scale is applied to its 32-bit sum; else each weight (q - z) * s
  * is rounded to the type first (tensor memory operands), which adds half a
- * step of the type to each product, and has to be in the type's range. */
+ * step of the type to each product. So a row's result depends, within that, on
+ * how many rows share the call. A layer with a weight that would round to an
+ * infinity of the type is multiplied in the first way with any number of rows. */
 int bnn_q4_layer_run(const bnn_q4_layer *L, const void *d_x, int64_t x_stride,
                      int rows, void *d_y, int64_t y_stride, void *stream);
 void bnn_q4_layer_destroy(bnn_q4_layer *L);

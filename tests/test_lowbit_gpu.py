@@ -820,3 +820,40 @@ def test_failing_allocations_are_reported():
     finally:
         bn.inject_fault(0)
     assert torch.cuda.mem_get_info()[0] == free
+
+
+# ------------------------------------------------------------------ weights outside the type's range
+@pytest.mark.parametrize("kind,scale", [("fp16", 8000.0), ("bf16", 2.0 ** 125)])
+@pytest.mark.parametrize("m", [1, 9, 16, 17, 40, 300, 1000])
+def test_linear_weights_beyond_the_type(m, kind, scale):
+    """(q - z) * s leaves the type's range for some weights of a layer; the
+    results do not, with any number of rows. Such a layer's weights are never
+    rounded: a group's scale is applied to its 32-bit sum."""
+    k, n, group = 640, 136, 64
+    _, d = linear_case(m, m, k, n, group, kind, True, True)
+    d["scales"][5::16] = (d["scales"][5::16].float() * scale).to(TYPES[kind])
+    layer = bn.Q4Linear(0, k, n, d["codes"], d["scales"], zeros=d["zeros"], bias=d["bias"], group=group, dtype=kind)
+    x = (d["x"].float() * 2.0 ** -10).to(TYPES[kind])
+    y = torch.full((m + 1, n), 7.0, device="cuda", dtype=TYPES[kind])
+    layer.run(x, y[:m])
+    w = linear_weights(d, k, group)
+    assert (w.abs() > torch.finfo(TYPES[kind]).max).any()
+    ref, size = x.double() @ w.T + d["bias"].double(), x.double().abs() @ w.abs().T + d["bias"].double().abs()
+    assert ref.abs().max() < torch.finfo(TYPES[kind]).max
+    tol = size * (2 * (k + 64) * U)
+    within(y[:m], ref, tol + rounding(ref.abs() + tol, TYPES[kind]))
+    assert (y[m] == 7).all()
+
+
+@pytest.mark.parametrize("scale,zero", [(65504 / 15 - 2, 0), (4370.0, 0), (65504 / 7 - 4, 8), (9368.0, 8)])
+def test_linear_weights_next_to_the_end_of_the_type(scale, zero):
+    """The largest weight just inside and just outside of fp16."""
+    scales = torch.full((16, 2), scale, device="cuda", dtype=torch.float16)
+    zeros = torch.full((16, 2), zero, device="cuda", dtype=torch.uint8)
+    d = {"codes": torch.full((16, 32), 0xFF, device="cuda", dtype=torch.uint8), "scales": scales, "zeros": zeros, "bias": None}
+    layer = bn.Q4Linear(0, 64, 16, d["codes"], scales, zeros=zeros, group=32, dtype="fp16")
+    x = torch.rand(40, 64, device="cuda", generator=gen(1)).half() * 2.0 ** -8
+    y = torch.empty(40, 16, device="cuda", dtype=torch.float16)
+    layer.run(x, y)
+    ref, tol = linear_ref(d, x, 64, 32, "fp16")
+    within(y, ref, tol)
