@@ -408,7 +408,6 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     const int kb0 = (int)((int64_t)g.kb * share / p.shares), nkb = (int)((int64_t)g.kb * (share + 1) / p.shares) - kb0;
     const int nk = (nkb + KB - 1) / KB;  // stages; the last one may have fewer blocks
     const uint32_t full_w = smem_addr(bars), full_x = full_w + 8 * S, empty = full_x + 8 * S, done = empty + 8 * S;
-    grid_launch();
     if (warp == WW) t5_alloc(smem_addr(&tmem_s), kTileCols);
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
@@ -423,6 +422,9 @@ __global__ void __launch_bounds__(q4_tile_threads(NTOK), 1)
     t5_before();
     __syncthreads();
     t5_after();
+    // Only now: a dependent that started before, took tensor memory that this
+    // CTA waits for and then waited for this grid would hold up both.
+    grid_launch();
     const uint32_t tmem = tmem_s;
     if (warp >= WW) grid_wait();  // the weights need not wait for the kernels before
 

@@ -222,3 +222,14 @@ def test_create_without_a_gpu_reports_it():
     buf = np.zeros(4096, np.uint8)
     rc, h = q4(device=0, codes=buf.ctypes.data, scales=buf.ctypes.data)
     assert rc == CUDA and not h.value
+
+
+def test_dependents_start_behind_the_tensor_memory_allocation():
+    """A programmatic dependent that takes tensor memory and waits for the
+    grid before it must not start while a CTA of that grid still waits for its
+    own: the order in the source of the one kernel that allocates some."""
+    src = open(os.path.join(ROOT, "bnns_to_c_b200", "csrc", "q4_linear.cu")).read()
+    body = src[src.index("q4_tiles_kernel(const"):]
+    alloc, barrier, start = body.index("t5_alloc("), body.index("__syncthreads()"), body.index("grid_launch()")
+    assert alloc < barrier < start
+    assert src.count("t5_alloc(") == 1

@@ -857,3 +857,28 @@ def test_linear_weights_next_to_the_end_of_the_type(scale, zero):
     layer.run(x, y)
     ref, tol = linear_ref(d, x, 64, 32, "fp16")
     within(y, ref, tol)
+
+
+def test_layers_beside_a_network_on_another_stream():
+    """The linear layer's tensor-memory kernel and the binary network's, at
+    once on two streams: each result is that of the call alone."""
+    import os
+
+    from oracle_util import synth
+
+    m = bn.Model(os.path.join(os.path.dirname(__file__), "golden", "unet_c8_mixed_s1.blob"))
+    patches = torch.from_numpy(synth(7, 0, 8, m.n_bands, 32, 32)).cuda()
+    layer, d = linear_case(1, 200, 2048, 1024, 64, "bf16", True, False)
+    y0, logits0 = torch.empty(200, 1024, device="cuda", dtype=torch.bfloat16), torch.empty(8, 3, 32, 32, device="cuda")
+    layer.run(d["x"], y0)
+    m.forward_device(0, patches, 8, 32, 32, logits0)
+    torch.cuda.synchronize()
+    ys = [torch.empty_like(y0) for _ in range(20)]
+    logits = [torch.empty_like(logits0) for _ in range(20)]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for y, z in zip(ys, logits):
+        layer.run(d["x"], y, stream=a)
+        m.forward_device(0, patches, 8, 32, 32, z, b.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, y0) for y in ys) and all(torch.equal(z, logits0) for z in logits)
