@@ -995,6 +995,9 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
         if ((q_heads > 1 && o_head < g.dim) || (n_seqs > 1 && o_seq < g.dim))
             return set_error(BNN_ERR_ARG, "bnn_kv_attend: strides %lld, %lld of the output: at least %d", (long long)o_seq,
                              (long long)o_head, g.dim);
+        if (rows_share(n_seqs, o_seq, q_heads, o_head, g.dim))
+            return set_error(BNN_ERR_ARG, "bnn_kv_attend: strides %lld, %lld put heads of the output over one another", (long long)o_seq,
+                             (long long)o_head);
         const size_t need = bnn_kv_attend_work(c, n_seqs, q_heads, prefix_tokens);
         if (!d_work || work_bytes < need || !aligned(d_work, 16))
             return set_error(BNN_ERR_ARG, "bnn_kv_attend: %zu bytes of workspace, 16-byte aligned, are needed (%zu given)", need,

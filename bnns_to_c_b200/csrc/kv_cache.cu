@@ -313,6 +313,9 @@ int kv_rows(const char* what, const bnn_kv_cache* c, const void* k, int64_t k_to
                 if ((g.heads > 1 && s.second < g.dim) || (n_tokens > 1 && s.first < g.dim))
                     return set_error(BNN_ERR_ARG, "%s: strides %lld, %lld of an output: at least %d", what, (long long)s.first,
                                      (long long)s.second, g.dim);
+                else if (rows_share(n_tokens, s.first, g.heads, s.second, g.dim))
+                    return set_error(BNN_ERR_ARG, "%s: strides %lld, %lld put heads of an output over one another", what,
+                                     (long long)s.first, (long long)s.second);
     }
     if (c->device < 0) return no_device(what);
     if (!work) return BNN_OK;

@@ -42,6 +42,21 @@ inline int no_device(const char* what) {
     return set_error(BNN_ERR_CUDA, "%s: the handle was made without a device", what);
 }
 inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// Whether rows of `dim` elements, n of them `row` apart in each of `heads`
+// heads `head` apart (each at least dim), share elements. Heads woven into
+// rows, or rows into heads, are told at once; else each head's start is
+// compared with the rows next to it.
+inline bool rows_share(int64_t n, int64_t row, int64_t heads, int64_t head, int64_t dim) {
+    if (n <= 1 || heads <= 1 || (__int128)row >= (__int128)(heads - 1) * head + dim || (__int128)head >= (__int128)(n - 1) * row + dim)
+        return false;
+    for (int64_t h = 1; h < heads; ++h) {
+        const __int128 at = (__int128)h * head;
+        if (at >= (__int128)n * row) break;  // behind the last row, which is dim wide at most
+        const int64_t i = (int64_t)(at / row), behind = (int64_t)(at - (__int128)i * row);
+        if (behind < dim || (i + 1 < n && row - behind < dim)) return true;
+    }
+    return false;
+}
 // Kernels here are launched as programmatic dependents of what is before them
 // in the stream: they may start while it ends, and wait for it (grid_wait)
 // before they touch anything that another kernel can have written or still

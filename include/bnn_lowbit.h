@@ -111,7 +111,8 @@ int bnn_kv_cache_write(bnn_kv_cache *c, const void *d_k, int64_t k_token,
                        const int32_t *d_start, const int32_t *d_offsets,
                        void *stream);
 
-/* The values that such tokens have in the cache, rounded to its type. */
+/* The values that such tokens have in the cache, rounded to its type. Strides
+ * that put two heads of an output over one another are refused. */
 int bnn_kv_cache_read(const bnn_kv_cache *c, void *d_k, int64_t k_token,
                       int64_t k_head, void *d_v, int64_t v_token,
                       int64_t v_head, int n_tokens, int n_seqs,
@@ -136,7 +137,8 @@ int bnn_kv_cache_read(const bnn_kv_cache *c, void *d_k, int64_t k_token,
  * of the row in the scale group, by 2^-33 of that product for each step of its
  * code. Keys of 2^100 and more make scores that are not finite.
  * q and out: the cache's type, sequence b and head i at
- * q + b * q_seq + i * q_head; they must not overlap. d_lse, unless NULL:
+ * q + b * q_seq + i * q_head; they must not overlap (strides of out that put
+ * two heads over one another are refused). d_lse, unless NULL:
  * float32 [n_seqs][q_heads], the natural logarithm of
  * sum_t exp(scale * q . key_t).
  * d_work: bnn_kv_attend_work(...) bytes of device memory, 16-byte aligned,

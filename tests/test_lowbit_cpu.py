@@ -233,3 +233,24 @@ def test_dependents_start_behind_the_tensor_memory_allocation():
     alloc, barrier, start = body.index("t5_alloc("), body.index("__syncthreads()"), body.index("grid_launch()")
     assert alloc < barrier < start
     assert src.count("t5_alloc(") == 1
+
+
+def test_outputs_that_lie_over_one_another_are_refused():
+    """Rows and heads that share numbers, although each stride alone is wide
+    enough; layouts that only look alike are taken."""
+    _, h = kv()
+    read = lambda tokens, kt, kh: (bn.lib().bnn_kv_cache_read, h, 16, kt, kh, 16, 128, 64, tokens, 2, 16, 3, 16, 16, None)  # noqa: E731
+    other = lambda tokens, vt, vh: (bn.lib().bnn_kv_cache_read, h, 16, 128, 64, 16, vt, vh, tokens, 2, 16, 3, 16, 16, None)  # noqa: E731
+    need = bn.lib().bnn_kv_attend_work(h, 3, 8, 0)
+    att = lambda os, oh: (bn.lib().bnn_kv_attend, h, 16, 512, 64, 3, 8, 16, 16, 3, None, 0, 0, 0.125, 16, os, oh, None, 16, need, None)  # noqa: E731
+    for fn in (read, other):
+        for tokens, st, hd in ((5, 64, 64), (2, 64, 64), (5, 64, 256), (5, 100, 64), (5, 64, 319), (5, 65, 130), (9, 127, 64)):
+            refused(ARG, "over one another", *fn(tokens, st, hd))
+        # heads outside, tokens outside, woven into one another, one token, a gap that just fits
+        for tokens, st, hd in ((5, 64, 320), (5, 128, 64), (5, 128, 192), (1, 0, 64), (3, 200, 100), (5, 130, 65), (5, 1 << 30, 1 << 30 | 64)):
+            refused(CUDA, "without a device", *fn(tokens, st, hd))
+    for st, hd in ((64, 64), (511, 64), (64, 128), (200, 100), (300, 75), (64, 191)):
+        refused(ARG, "over one another", *att(st, hd))
+    for st, hd in ((512, 64), (64, 192), (128, 448), (1 << 62, 64), (64, 1 << 62)):
+        refused(CUDA, "without a device", *att(st, hd))
+    bn.lib().bnn_kv_cache_destroy(h)
