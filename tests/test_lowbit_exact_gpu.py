@@ -1,0 +1,146 @@
+"""The low-bit operators (include/bnn_lowbit.h) on the GPU on inputs whose
+answer is exact, or whose every part shows: a token or an input that is lost,
+doubled or weighted wrongly anywhere changes a result by far more than what
+is allowed."""
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import bnns_to_c_b200 as bn  # noqa: E402
+
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module", autouse=True)
+def need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    yield
+    assert bn.q4_wait_timeouts(0) == 0
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def whole(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------ linear
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,k,n,group", [
+    (1, 31, 17, 32), (2, 512, 512, 128), (1, 16384, 64, 128), (8, 8192, 130, 64), (3, 4160, 100, 64), (5, 6464, 300, 32), (1, 7168, 600, 256),
+    (9, 1030, 77, 32), (16, 9000, 300, 64), (16, 4096, 2048, 64), (12, 3200, 100, 32), (16, 4096, 4096, 128), (33, 2704, 90, 128),
+    (64, 640, 300, 64), (70, 3200, 100, 32), (129, 448, 128, 64), (200, 1800, 130, 64), (128, 5001, 130, 64), (40, 4099, 200, 32),
+    (260, 4098, 300, 128), (700, 2704, 1000, 64), (2048, 1024, 512, 128), (1000, 3001, 1111, 64)])
+def test_linear_sums_without_any_rounding(m, k, n, group, kind):
+    """x of -1, 0 and 1, scales that are powers of two: weights, products and
+    sums are exact in any order, so the result is the exact one, rounded."""
+    g, t = gen(m + k), TYPES[kind]
+    ng = -(-k // group)
+    x = torch.randint(-1, 2, (m, k), device="cuda", generator=g).to(t)
+    codes = torch.randint(0, 256, (n, (k + 1) // 2), device="cuda", generator=g, dtype=torch.uint8)
+    scales = torch.exp2(-torch.randint(0, 4, (n, ng), device="cuda", generator=g).float()).to(t)
+    zeros = torch.randint(0, 16, (n, ng), device="cuda", generator=g, dtype=torch.uint8)
+    bias = torch.randint(-64, 65, (n,), device="cuda", generator=g).float() / 8
+    layer = bn.Q4Linear(0, k, n, codes, scales, zeros=zeros, bias=bias, group=group, dtype=kind)
+    y = torch.empty(m, n, device="cuda", dtype=t)
+    layer.run(x, y)
+    q = torch.stack((codes & 15, codes >> 4), -1).flatten(1)[:, :k].double()
+    of = torch.arange(k, device="cuda") // group
+    w = (q - zeros.double()[:, of]) * scales.double()[:, of]
+    ref = x.double() @ w.T + bias.double()
+    assert ref.abs().max() < 2 ** 14 and torch.equal(ref * 8, (ref * 8).round())
+    assert torch.equal(y, ref.to(t))
+
+
+# ------------------------------------------------------------------ attention
+def cache_of(k, v, bits, group, kind, page, cut):
+    """A cache of these tokens in shuffled pages, the first `cut` of them as a
+    prefix: (cache, table, prefix pages)."""
+    n, heads, dim = k.shape
+    n_pre, n_own = -(-cut // page), max(1, -(-(n - cut) // page))
+    c = bn.KVCache(0, n_pre + n_own + 3, page, heads, dim, bits=bits, group=group, dtype=kind)
+    order = torch.randperm(n_pre + n_own + 3, device="cuda", generator=gen(n)).to(torch.int32)
+    pre, own = order[:n_pre].contiguous(), order[n_pre:n_pre + n_own][None].contiguous()
+    if cut:
+        c.write(k[:cut], v[:cut], pre[None], whole(0), offsets=whole(0, cut))
+    c.write(k[cut:], v[cut:], own, whole(0), offsets=whole(0, n - cut))
+    return c, own, pre
+
+
+def attend(c, q, n, own, pre, cut):
+    out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 3.0, device="cuda")
+    seqs = q.shape[0]
+    work = torch.full((c.attend_work(seqs, q.shape[1], cut),), 0xFF, device="cuda", dtype=torch.uint8)
+    c.attend(q, torch.full((seqs,), n - cut, dtype=torch.int32, device="cuda"), own.repeat(seqs, 1), out, work, lse=lse, scale=1.0,
+             prefix=pre if cut else None, prefix_tokens=cut)
+    return out, lse
+
+
+SHAPES = [(1, 1, 4, 64, 8, 0, 16), (777, 2, 4, 64, 4, 32, 16), (20011, 1, 8, 128, 8, 0, 64), (20011, 8, 8, 128, 8, 0, 64),
+          (20011, 2, 16, 128, 4, 32, 64), (9001, 2, 32, 64, 8, 32, 32), (5003, 1, 5, 256, 4, 64, 128), (30000, 3, 2, 192, 8, 64, 256),
+          (100003, 2, 4, 128, 8, 128, 64)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,heads,share,dim,bits,group,page", SHAPES)
+@pytest.mark.parametrize("prefix", [False, True])
+def test_attend_counts_every_token(n, heads, share, dim, bits, group, page, prefix, kind):
+    """All weights are equal (q = 0), and each token has one channel with a
+    value of its own group's scale 1, the others 0: a channel's result is the
+    number of its tokens over n, the log-sum ln n. Weights, codes and sums are
+    exact; 2^-20 for the joins, and a rounding to the type."""
+    cut = n * 2 // 3 if prefix else 0
+    top = 2 ** (bits - 1) - 1
+    at = (torch.arange(n, device="cuda") * 7) % dim
+    v = torch.zeros(n, heads, dim, device="cuda")
+    v[torch.arange(n, device="cuda"), :, at] = float(top)
+    k = torch.randn(n, heads, dim, device="cuda", generator=gen(1))
+    c, own, pre = cache_of(k.to(TYPES[kind]), v.to(TYPES[kind]), bits, group, kind, page, cut)
+    q = torch.zeros(2, heads * share, dim, device="cuda", dtype=TYPES[kind])
+    out, lse = attend(c, q, n, own, pre, cut)
+    ref = torch.bincount(at, minlength=dim).double() * top / n
+    tol = ref * (torch.finfo(TYPES[kind]).eps / 2 + 2.0 ** -20)
+    assert ((out.double() - ref).abs() <= tol).all()
+    assert ((lse.double() - math.log(n)).abs() <= 2.0 ** -20 + 4 * U * math.log(n)).all()
+
+
+@pytest.mark.parametrize("n,heads,share,dim,bits,group,page", SHAPES)
+@pytest.mark.parametrize("prefix", [False, True])
+def test_attend_finds_each_position(n, heads, share, dim, bits, group, page, prefix):
+    """Keys spell their position in 17 channels of +-1, queries the position
+    they want, 96 nats above every other: the result is that token's value as
+    the cache holds it, bit for bit. Positions at the borders of steps, blocks,
+    pages and the prefix, and others at random."""
+    kind, cut = "bf16", n * 2 // 3 if prefix else 0
+    bit = torch.arange(17, device="cuda")
+    spell = lambda p: ((p[..., None] >> bit) & 1) * 2.0 - 1.0  # noqa: E731
+    k = torch.zeros(n, heads, dim, device="cuda")
+    k[:, :, :17] = spell(torch.arange(n, device="cuda"))[:, None]
+    v = torch.randn(n, heads, dim, device="cuda", generator=gen(2)).to(TYPES[kind])
+    c, own, pre = cache_of(k.to(TYPES[kind]), v, bits, group, kind, page, cut)
+    held = torch.empty_like(v)
+    if cut:
+        c.read(torch.empty_like(v[:cut]), held[:cut], pre[None], whole(0), offsets=whole(0, cut))
+    c.read(torch.empty_like(v[cut:]), held[cut:], own, whole(0), offsets=whole(0, n - cut))
+    want = {0, n - 1, cut, max(0, cut - 1)}
+    for step in (16, 32, 64, 256, page, 1024, 4096):
+        for base in (0, cut, n // 2 // step * step):
+            want |= {base + step - 1, base + step, base + 2 * step - 1}
+    want = torch.tensor(sorted(p for p in want if p < n), device="cuda")
+    seqs = -(-want.numel() // (heads * share)) + 1
+    fill = torch.randint(0, n, (seqs * heads * share,), device="cuda", generator=gen(3))
+    fill[: want.numel()] = want
+    fill = fill[torch.randperm(fill.numel(), device="cuda", generator=gen(4))].view(seqs, heads * share)
+    q = torch.zeros(seqs, heads * share, dim, device="cuda")
+    q[:, :, :17] = spell(fill) * 48.0
+    out, _ = attend(c, q.to(TYPES[kind]), n, own, pre, cut)
+    of = torch.arange(heads * share, device="cuda") // share
+    assert torch.equal(out, held[fill, of[None].expand_as(fill)])

@@ -882,3 +882,61 @@ def test_layers_beside_a_network_on_another_stream():
         m.forward_device(0, patches, 8, 32, 32, z, b.cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(y, y0) for y in ys) and all(torch.equal(z, logits0) for z in logits)
+
+
+FIRST_CALLS = """
+import sys
+import torch
+import bnns_to_c_b200 as bn
+
+def run(eager):
+    t, g = torch.bfloat16, torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g).to(t)
+    whole = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    layers = [bn.Q4Linear(0, k, n, torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8),
+                          rnd(n, k // 64).abs(), group=64) for k, n in ((512, 256), (4096, 64))]
+    xs = [rnd(m, l.n_in) for l in layers for m in (1, 12, 300)]
+    ys = [torch.zeros(x.shape[0], l.n_out, device="cuda", dtype=t) for l, x in zip([l for l in layers for _ in range(3)], xs)]
+    c = bn.KVCache(0, 40, 64, 2, 128, bits=8)
+    k, v, q = rnd(900, 2, 128), rnd(900, 2, 128), rnd(3, 16, 128)
+    table, pre = torch.arange(30, dtype=torch.int32, device="cuda").view(3, 10), torch.arange(30, 35, dtype=torch.int32, device="cuda")
+    start, off, n = whole(0, 0, 0), whole(0, 300, 310, 900), whole(300, 10, 590)
+    gk, gv, outs = torch.zeros_like(k), torch.zeros_like(v), [torch.zeros_like(q) for _ in range(2)]
+    works = [torch.empty(c.attend_work(3, 16, p), device="cuda", dtype=torch.uint8) for p in (0, 200)]
+    def calls(st):
+        for i, (x, y) in enumerate(zip(xs, ys)):
+            layers[i // 3].run(x, y, stream=st)
+        c.write(k, v, table, start, offsets=off, stream=st)
+        c.read(gk, gv, table, start, offsets=off, stream=st)
+        c.attend(q, n, table, outs[0], works[0], stream=st)
+        c.attend(q, n, table, outs[1], works[1], prefix=pre, prefix_tokens=200, stream=st)
+    torch.cuda.synchronize()
+    if eager:
+        calls(torch.cuda.current_stream())
+    else:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            calls(torch.cuda.current_stream())
+        graph.replay()
+    torch.cuda.synchronize()
+    return ys + [gk, gv] + outs
+
+captured, eager = run(False), run(True)
+assert all(torch.equal(a, b) and a.abs().sum() > 0 for a, b in zip(captured, eager))
+assert bn.q4_wait_timeouts(0) == 0
+print("same")
+"""
+
+
+@pytest.mark.parametrize("pdl", ["1", "0"])
+def test_first_calls_of_a_process_are_captured(pdl):
+    """No call needs one before it: the first ones of a process go into a
+    graph (with and without programmatic launches)."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, env={**os.environ, "BNN_PDL": pdl}, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stdout[-2000:] + r.stderr[-2000:]
