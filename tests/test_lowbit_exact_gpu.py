@@ -144,3 +144,62 @@ def test_attend_finds_each_position(n, heads, share, dim, bits, group, page, pre
     out, _ = attend(c, q.to(TYPES[kind]), n, own, pre, cut)
     of = torch.arange(heads * share, device="cuda") // share
     assert torch.equal(out, held[fill, of[None].expand_as(fill)])
+
+
+# ------------------------------------------------------------------ streams joined by events
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_behind_another_streams_event(captured):
+    """Each call starts early behind the one before it in its stream, but not
+    before what its stream waits for: inputs that a second stream writes late,
+    behind an event, while the first stream's last kernel allows early starts."""
+    t = torch.bfloat16
+    layer = bn.Q4Linear(0, 512, 256, torch.randint(0, 256, (256, 256), device="cuda", generator=gen(1), dtype=torch.uint8),
+                        torch.ones(256, 8, device="cuda", dtype=t), group=64)
+    c = bn.KVCache(0, 4, 64, 2, 128, bits=8)
+    table, start, n = whole(0, 1, 2, 3).view(1, 4), whole(0), whole(200)
+    off = whole(0, 200)
+    src = {"x": torch.randn(40, 512, device="cuda", generator=gen(2)).to(t), "q": torch.randn(1, 8, 128, device="cuda", generator=gen(3)).to(t),
+           "k": torch.randn(200, 2, 128, device="cuda", generator=gen(4)).to(t), "v": torch.randn(200, 2, 128, device="cuda", generator=gen(5)).to(t)}
+    late = {k: torch.zeros_like(v) for k, v in src.items()}
+    warm = torch.zeros(3, 512, device="cuda", dtype=t)
+    y0, ys = torch.empty(3, 256, device="cuda", dtype=t), [torch.empty(m, 256, device="cuda", dtype=t) for m in (3, 12, 40)]
+    gk, gv, out = torch.empty_like(src["k"]), torch.empty_like(src["v"]), torch.empty_like(src["q"])
+    work = torch.empty(c.attend_work(1, 8), device="cuda", dtype=torch.uint8)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def run():
+        """Every call on a, right behind a short kernel of a and an event of b."""
+        calls = [(("x",), lambda m=m, y=y: layer.run(late["x"][:m], y, stream=a)) for m, y in zip((3, 12, 40), ys)]
+        calls += [(("k", "v"), lambda: c.write(late["k"], late["v"], table, start, offsets=off, stream=a)),
+                  ((), lambda: c.read(gk, gv, table, start, offsets=off, stream=a)),
+                  (("q",), lambda: c.attend(late["q"], n, table, out, work, stream=a))]
+        for names, call in calls:
+            b.wait_stream(a)
+            with torch.cuda.stream(b):
+                torch.cuda._sleep(400_000)  # 0.2 ms
+                for k in names:
+                    late[k].copy_(src[k])
+            layer.run(warm, y0, stream=a)
+            a.wait_stream(b)
+            call()
+
+    torch.cuda.synchronize()
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=a):
+            run()
+    for _ in range(3):
+        for v in late.values():
+            v.zero_()
+        torch.cuda.synchronize()
+        g.replay() if captured else run()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in ys + [gk, gv, out]]
+        for m, y in zip((3, 12, 40), ys):
+            layer.run(src["x"][:m], y)
+        c.write(src["k"], src["v"], table, start, offsets=off)
+        c.read(gk, gv, table, start, offsets=off)
+        c.attend(src["q"], n, table, out, work)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, z) for x, z in zip(got, ys + [gk, gv, out]))
+        assert got[2].abs().sum() > 0 and got[5].abs().sum() > 0
