@@ -25,8 +25,8 @@ constexpr int kMostInv = 127 + 118;  // exponent field of the largest 1 / unit: 
 constexpr int kSub = 16;  // tokens of an instruction
 // 16-token blocks that a warp takes at a time: two where the sums leave it the
 // registers and a row is short (of `row` bytes), so that shared memory holds
-// enough steps: 64 ragged sequences in 4 bits 82 us against 90 of one at a
-// time, but 100003 tokens in 8 bits, 128-byte rows, 58 against 47.
+// enough steps: 64 ragged sequences in 4 bits 78 us against 85 of one at a
+// time, but 100003 tokens in 8 bits, 128-byte rows, 62 against 48.
 __host__ __device__ constexpr int attend_halves(int nt, int row) { return nt == 1 && row <= 64 ? 2 : 1; }
 
 // CTAs of an attention kernel on an SM: as many as the registers allow, dp * nt
@@ -182,12 +182,13 @@ __device__ __forceinline__ void load_scales(float* f, const uint16_t* at) {  // 
 
 // DP: head_dim rounded up; NT: tiles of 8 query rows; BPG: 32-blocks of
 // channels that share a scale (8: all).
-// The floor is the codes' bytes; decoding them holds it at 2.4 to 2.6 of an
+// The floor is the codes' bytes; decoding them holds it at 2.3 to 2.6 of an
 // SM's 4 instructions a clock, half of them bit operations and conversions, at
 // 16 warps of 127 registers an SM. 100003 tokens, 8 kv heads of 128 in 8 bits,
-// 32 query heads: 46 us with the join (4.5 TB/s of codes). 179457 tokens of 64
-// sequences, 64 query heads, in 4 bits and groups of 32: 75 us (2.8 TB/s). The
-// work is cut into one equal share a CTA, in blocks of tokens, whatever
+// 32 query heads: 48 us with the join (4.3 TB/s of codes). 179457 tokens of 64
+// sequences, 64 query heads, in 4 bits and groups of 32: 78 us (2.7 TB/s). 16
+// such sequences of 256 query heads in 8 bits (32 rows a tile, a unit for each
+// row and group): 72 us, bound by fetching instructions too. The work is cut into one equal share a CTA, in blocks of tokens, whatever
 // sequence they belong to; what is cut is joined by join_kernel.
 template <int DP, int BITS, int NT, int BPG>
 __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kernel(const AttendParams p) {
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
                 // when one is 2^15 or more, and puts it at 2^8: the largest of a
                 // row and group is at least that, so that only those below 2^-22
                 // of it lose bits (are 2^-33 of it off). At 2^11, raised more often,
-                // 16 sequences of 32 rows a kv head took 77 us, at 2^8 70.
+                // 16 sequences of 32 rows a kv head took 77 us, at 2^8 71.
                 uint32_t wt[HV][NG][NT][2];
                 const auto weigh = [&] {
 #pragma unroll
@@ -729,10 +730,10 @@ __global__ void __launch_bounds__(32 * kWarps, attend_ctas(DP, NT)) attend_kerne
 // prefix), each a mean with the maximum and the sum of its weights. PER = 4: a
 // CTA a row, whose warps share the parts, where there are few rows, of many
 // parts each; PER = 1: a warp a row, which saves the join of the warps. Whole
-// attentions: 64 ragged sequences of 64 heads 75 us with 1, 82 with 4; 82
-// sequences of 64 heads behind 64 tokens 32 and 47; 96 of 16 behind 8190 41
-// and 43; 48 of 16 behind 8190 32.5 and 30.6; 16 ragged ones of 64 28 and 25;
-// one of 32 heads, 100003 tokens, 64 and 46.
+// attentions: 64 ragged sequences of 64 heads 78 us with 1, 85 with 4; 82
+// sequences of 64 heads behind 64 tokens 42 and 56; 96 of 16 behind 8190 44
+// and 46.5; 48 of 16 behind 8190 34.6 and 33.2; 16 ragged ones of 64 28.7 and
+// 27.0; one of 32 heads, 100003 tokens, 60 and 49.
 struct JoinSide {
     const int2* owners;  // nullptr: this side has nothing
     const float* pacc;
@@ -1040,8 +1041,8 @@ BNN_API int bnn_kv_attend(const bnn_kv_cache* c, const void* d_q, int64_t q_seq,
         work += s.bytes();
         p.second = prefix && side == 0 && pdl_on();
         // Started early, its CTAs would find the places of an SM taken by
-        // those of the kernel before, and their shares are equal: 94 us
-        // against 82 for 64 ragged sequences in 4 bits (before the join had two forms).
+        // those of the kernel before, and their shares are equal: 85 us
+        // against 78 for 64 ragged sequences in 4 bits.
         const cudaError_t e = attend_any(g, s.nt, [&](auto k) { return launch(k, dim3(s.ctas), 32 * kWarps, s.smem, st, p.second, p); });
         if (e != cudaSuccess) return cuda_error("bnn_kv_attend", e);
         jp.side[side] = JoinSide{p.owners, p.pacc, p.pml, p.lengths, p.length, s.rg, s.rt, 8 * s.nt, s.ctas};

@@ -112,10 +112,12 @@ struct Q4Params {
 // type. A CTA makes MT tiles of 16 outputs for 8 * NT rows of x; its
 // warps take chunks of U 64-input blocks in turn and their sums are joined in
 // shared memory. The weights of the next chunk are on their way while one is
-// multiplied: U * MT * 512 bytes a warp. Bound by reading the weights and, as
-// much, by taking the codes apart (and-or, shift and subtract, 83 instructions
-// a 16 x 64 block). One row, launches in a row: 8192 x 8192 9.8 us (3.6 TB/s),
-// 4096 x 4096 4.0 us (2.2 TB/s), 512 x 512 1.6 us.
+// multiplied: U * MT * 512 bytes a warp. A 16 x 64 block takes 83 instructions
+// (and-or, shift and subtract). One row, launches in a row over layers that
+// together are larger than the L2: 8192 x 8192 10.0 us (3.5 TB/s; one layer
+// again and again 9.8), 4096 x 4096 4.1 us, 512 x 512 1.6 us. Neither the bytes
+// nor the instructions (1.6 of 4 a clock in a lone cold launch, ALU 38%) bound
+// it: a warp has one chunk on its way, and of 148 SMs 108 have two CTAs, 40 one.
 // (q - z) is exact in 16 bits (|q - z| <= 15), so a group's sum of products
 // has only the rounding of 32-bit sums, and its scale is applied to that sum.
 // X: how x can be read: 2 = 8 bytes at a time, K a multiple of 64; 1 = 8 bytes
@@ -288,7 +290,8 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 2) q4_rows_kernel(const Q4Param
     }
 }
 
-// CTAs in clusters of c that run at a time with one on each SM: clusters do not fill every GPC
+// CTAs in clusters of c that run at a time with one on each of a B200's 148 SMs (as its
+// occupancy calls say): clusters do not fill every GPC
 constexpr int kAtOnce[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
 
 // Shares of K (of 16 blocks at least) for tiles of MT: the ones with the
@@ -342,11 +345,14 @@ cudaError_t q4_rows(const Q4Params& p, cudaStream_t st) {
 // thirds of the rate. 2048 rows, 4096 x 4096: 53 us alone (1.30 PFLOP/s), 64
 // in a long row of launches under the power cap (1.07; the 16-bit library
 // product of that shape 52 then); tensor pipe busy 71% of the time, the rest
-// the start and end of 256 CTAs in two rounds. 16 rows, 4096 to 16384: 15.6 us,
-// bound by taking the codes apart.
-// Rounding a weight to 16 bits costs 2^-9 (bf16; fp16 2^-12) of a product, as
-// much as the rounding of the result costs; the products' errors are
-// independent, so the result stays within sqrt(2) of its own rounding.
+// the start and end of 256 CTAs in two rounds. 16 rows, 4096 to 16384: 15.6 us
+// (layers in turn, larger than the L2 together), of 128 CTAs on 148 SMs, each a
+// chain through tensor memory (2.2 of 4 instructions a clock, ALU 43% in a
+// lone cold launch).
+// Rounding a weight to 16 bits costs half a step of the type, 2^-8 (bf16; fp16
+// 2^-11) of a product at most: the result is off by that much of sum |x w| at
+// most, beside its own rounding, and typically, for independent products that
+// do not cancel, by no more than its own rounding.
 // Codes to tensor memory is a chain of about 800 clocks a stage (arithmetic,
 // store, wait, hand over), so two groups of eight warps take the stages in
 // turn. One thread's products start 70 to 100 clocks apart, so below NTOK =

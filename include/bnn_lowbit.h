@@ -9,7 +9,8 @@
  * stream), enqueue, and return without synchronising; status codes and
  * bnn_last_error as in bnn_b200.h. The handle's device is made current for
  * the call and the caller's device restored. No call but the create and
- * destroy ones allocates, so all others can be captured into a graph. A
+ * destroy ones allocates, so all others can be captured into a graph (whose
+ * last replay a handle has to outlive). A
  * handle may be used from several host threads and streams; calls that
  * overlap must not write what another one reads (positions of a cache,
  * outputs, the workspace of an attention).
@@ -52,12 +53,14 @@ int bnn_q4_layer_create(int device, int n_in, int n_out, int group, int type,
 /* rows (0 .. 2^19) vectors: x [rows] at a distance of x_stride elements
  * (>= n_in) -> y [rows] at y_stride (>= n_out), both in the layer's type, any
  * alignment of the type. x and y must not overlap. Up to 8 rows, and up to 16
- * in a layer of fewer than 2^23 weights, the codes are multiplied exactly and
- * a group's scale is applied to its 32-bit sum; else each weight (q - z) * s
- * is rounded to the type first (tensor memory operands), which adds half a
- * step of the type to each product. So a row's result depends, within that, on
- * how many rows share the call. A layer with a weight that would round to an
- * infinity of the type is multiplied in the first way with any number of rows. */
+ * in a layer of fewer than 2^23 weights (n_out rounded up to a multiple of 16
+ * times n_in to one of 64), the codes are multiplied exactly and a group's
+ * scale is applied to its 32-bit sum (finite for |x| below 2^112); else each
+ * weight (q - z) * s is rounded to the type first (tensor memory operands),
+ * which adds half a step of the type to each product. So a row's result
+ * depends, within that, on how many rows share the call. A layer with a weight
+ * that would round to an infinity of the type is multiplied in the first way
+ * with any number of rows. */
 int bnn_q4_layer_run(const bnn_q4_layer *L, const void *d_x, int64_t x_stride,
                      int rows, void *d_y, int64_t y_stride, void *stream);
 void bnn_q4_layer_destroy(bnn_q4_layer *L);
