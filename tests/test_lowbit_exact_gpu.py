@@ -203,3 +203,98 @@ def test_calls_behind_another_streams_event(captured):
         torch.cuda.synchronize()
         assert all(torch.equal(x, z) for x, z in zip(got, ys + [gk, gv, out]))
         assert got[2].abs().sum() > 0 and got[5].abs().sum() > 0
+
+
+# ------------------------------------------------------------------ the ends of the documented ranges
+@pytest.mark.parametrize("heavy", [False, True])
+def test_linear_most_rows(heavy):
+    """2^19 rows, the most of a call; heavy: with weights outside fp16."""
+    m, k, n = 1 << 19, 64, 40
+    x = torch.randint(-1, 2, (m, k), device="cuda", generator=gen(1)).half()
+    codes = torch.randint(0, 256, (n, k // 2), device="cuda", generator=gen(2), dtype=torch.uint8)
+    scales = torch.full((n, 2), 0.25, device="cuda", dtype=torch.float16)
+    if heavy:
+        zeros = torch.full((n, 2), 8, device="cuda", dtype=torch.uint8)
+        scales[7], codes[7], zeros[7, 0] = 8192.0, 0x8F, 0  # weights 15 * 8192 and 8 * 8192, then 7 * 8192 and 0
+        x[:, :32] = 0.0
+        x[:, 32::2] = torch.where(torch.arange(16, device="cuda") == 3, x[:, 32::2], 0.0)  # one of them in each sum
+    else:
+        zeros = None
+    layer = bn.Q4Linear(0, k, n, codes, scales, zeros=zeros, group=32, dtype="fp16")
+    y = torch.empty(m, n, device="cuda", dtype=torch.float16)
+    layer.run(x, y)
+    q = torch.stack((codes & 15, codes >> 4), -1).flatten(1).float()
+    z = zeros.float().repeat_interleave(32, 1) if heavy else 8.0
+    w = (q - z) * scales.float().repeat_interleave(32, 1)
+    assert (w.abs().max() > 65504) == heavy
+    ref = x.float() @ w.T  # exact: whole multiples of a quarter below 2^24 of them
+    assert torch.equal(y, ref.half())
+
+
+def test_cache_most_heads():
+    """4096 kv heads, written and read back; a group wider than the head."""
+    for dim, bits, group in ((8, 8, 32), (16, 4, 0)):
+        c = bn.KVCache(0, 3, 16, 4096, dim, bits=bits, group=group)
+        top = 2 ** (bits - 1) - 1
+        x = [torch.randint(-top, top + 1, (37, 4096, dim), device="cuda", generator=gen(i)).float() for i in (1, 2)]
+        for v in x:
+            v[..., 0] = top  # scale 1: every code is held exactly
+        x = [v.to(torch.bfloat16) for v in x]
+        table, off = whole(2, 0, 1)[None], whole(0, 37)
+        c.write(*x, table, whole(5), offsets=off)
+        got = [torch.zeros_like(v) for v in x]
+        c.read(*got, table, whole(5), offsets=off)
+        assert all(torch.equal(a, b) for a, b in zip(x, got))
+
+
+def counted(n, heads, dim, kind):
+    """Values with 127 in one channel a token, keys of any kind."""
+    at = (torch.arange(n, device="cuda") * 7) % dim
+    v = torch.zeros(n, heads, dim, device="cuda")
+    v[torch.arange(n, device="cuda"), :, at] = 127.0
+    return torch.randn(n, heads, dim, device="cuda", generator=gen(1)).to(kind), v.to(kind), torch.nn.functional.one_hot(at, dim).double() * 127
+
+
+@pytest.mark.parametrize("prefix", [0, 50])
+@pytest.mark.parametrize("dim,share", [(64, 2), (256, 9)])
+def test_attend_most_sequences(dim, share, prefix):
+    """16384 sequences, the most of a call, of 0 to 70 tokens, all in the same
+    pages; every weight is the same."""
+    seqs, n = 16384, 70
+    k, v, one = counted(n + prefix, 1, dim, torch.float16)
+    c = bn.KVCache(0, 9, 16, 1, dim, bits=8, dtype="fp16")
+    own, pre = whole(0, 1, 2, 3, 4), whole(5, 6, 7, 8)
+    c.write(k[prefix:], v[prefix:], own[None], whole(0), offsets=whole(0, n))
+    if prefix:
+        c.write(k[:prefix], v[:prefix], pre[None], whole(0), offsets=whole(0, prefix))
+    lengths = torch.randint(0, n + 1, (seqs,), device="cuda", generator=gen(2), dtype=torch.int32)
+    q, out = torch.zeros(seqs, share, dim, device="cuda", dtype=torch.float16), torch.full((seqs, share, dim), 3.0, device="cuda", dtype=torch.float16)
+    lse = torch.full((seqs, share), 3.0, device="cuda")
+    work = torch.full((c.attend_work(seqs, share, prefix),), 0xFF, device="cuda", dtype=torch.uint8)
+    c.attend(q, lengths, own[None].repeat(seqs, 1), out, work, lse=lse, prefix=pre if prefix else None, prefix_tokens=prefix)
+    sums = torch.cat((torch.zeros(1, dim, device="cuda", dtype=torch.float64), one[prefix:].cumsum(0))) + one[:prefix].sum(0)
+    count = (lengths + prefix).double()
+    ref = (sums[lengths.long()] / count.clamp(min=1)[:, None])[:, None].expand(-1, share, -1)
+    assert ((out.double() - ref).abs() <= ref * (2.0 ** -11 + 2.0 ** -20)).all()
+    want = count.log()[:, None].expand(-1, share)
+    near = (lse.double() - want).abs() <= 2.0 ** -20 + 4 * U * want.abs()
+    assert (near | ((lse == want) & (count == 0)[:, None])).all()
+
+
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_attend_most_query_heads(prefix):
+    """65536 query heads of one kv head, the most of a call."""
+    dim, n, heads = 64, 300, 65536
+    k, v, one = counted(n + prefix, 1, dim, torch.bfloat16)
+    c = bn.KVCache(0, 22, 16, 1, dim, bits=8)
+    own, pre = torch.arange(19, device="cuda", dtype=torch.int32), whole(19, 20, 21)
+    c.write(k[prefix:], v[prefix:], own[None], whole(0), offsets=whole(0, n))
+    if prefix:
+        c.write(k[:prefix], v[:prefix], pre[None], whole(0), offsets=whole(0, prefix))
+    q, out = torch.zeros(1, heads, dim, device="cuda", dtype=torch.bfloat16), torch.full((1, heads, dim), 3.0, device="cuda", dtype=torch.bfloat16)
+    lse = torch.full((1, heads), 3.0, device="cuda")
+    work = torch.full((c.attend_work(1, heads, prefix),), 0xFF, device="cuda", dtype=torch.uint8)
+    c.attend(q, whole(n), own[None], out, work, lse=lse, prefix=pre if prefix else None, prefix_tokens=prefix)
+    ref = one.sum(0) / (n + prefix)
+    assert ((out.double() - ref).abs() <= ref * (2.0 ** -8 + 2.0 ** -20)).all()
+    assert ((lse.double() - math.log(n + prefix)).abs() <= 2.0 ** -20 + 4 * U * math.log(n + prefix)).all()
